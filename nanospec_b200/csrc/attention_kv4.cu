@@ -1,0 +1,167 @@
+// Attention over the 4-bit cache (kv4.cuh) for every head size, page size and type: softmax(q k^T scale) v over the positions
+// max(0, p - window + 1) .. p of a token at position p, in float from the cached values on.
+//
+// A block takes a token and up to eight query heads of a kv head; its four warps take tiles of 32 keys in turn, each with a running
+// maximum and sum of its own, and are joined at the end.  Scores: a lane holds a key; weighted values: a lane holds features.
+#include "kv4.cuh"
+
+namespace {
+
+constexpr int kWarps = 4, kThreads = 32 * kWarps, kHeads = 8;
+
+template <typename T, int kChunks>  // kChunks of 128 features
+__global__ void __launch_bounds__(kThreads)
+attention_kv4_kernel(const T* __restrict__ q, long long ldq, const uint8_t* __restrict__ k_pages, const uint8_t* __restrict__ v_pages,
+                     const int* __restrict__ block_table, int table_stride, const int* __restrict__ token_req, const int* __restrict__ positions,
+                     const int* __restrict__ rows, T* __restrict__ out, long long ldo, int nq, int nkv, int D, int page_size, float scale, int window,
+                     const float* __restrict__ sink) {
+    ns_pdl_launch_dependents();
+    ns_pdl_wait();
+    __shared__ __align__(16) float qs[kHeads][128 * kChunks];
+    __shared__ float ps[kWarps][32][kHeads];
+    __shared__ float os[kWarps][kHeads][128 * kChunks], ms[kWarps][kHeads], ls[kWarps][kHeads];
+    const int n = rows ? rows[blockIdx.x] : blockIdx.x;
+    const int req = token_req[n];
+    if (req < 0) return;
+    const int G = nq / nkv, tiles = (G + kHeads - 1) / kHeads;
+    const int hk = blockIdx.y / tiles, h0 = hk * G + (blockIdx.y % tiles) * kHeads;
+    const int heads = min(kHeads, hk * G + G - h0);
+    const int pos = positions[n], first = window > 0 ? max(0, pos - window + 1) : 0;
+    const int* bt = block_table + (size_t)req * table_stride;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    for (int i = threadIdx.x; i < kHeads * D; i += kThreads) {
+        const int h = i / D, f = i % D;
+        qs[h][f] = h < heads ? ns_ld(q, (size_t)n * ldq + (size_t)(h0 + h) * D + f) * scale : 0.f;
+    }
+    __syncthreads();
+    float m[kHeads], l[kHeads], o[kHeads][kChunks][4];
+#pragma unroll
+    for (int h = 0; h < kHeads; ++h) {
+        m[h] = -INFINITY;
+        l[h] = 0.f;
+#pragma unroll
+        for (int c = 0; c < kChunks; ++c)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) o[h][c][i] = 0.f;
+    }
+    for (int k0 = first + warp * 32; k0 <= pos; k0 += kThreads) {
+        const int key = k0 + lane, count = min(32, pos + 1 - k0);
+        const bool seen = key <= pos;
+        size_t block = 0;
+        int slot = 0;
+        float s[kHeads];
+#pragma unroll
+        for (int h = 0; h < kHeads; ++h) s[h] = 0.f;
+        if (seen) {
+            slot = key % page_size;
+            block = ((size_t)bt[key / page_size] * nkv + hk) * kv4_block_bytes(page_size, D);
+            const uint32_t* codes = reinterpret_cast<const uint32_t*>(k_pages + block + (size_t)slot * (D / 2));
+            const uint32_t* pairs = reinterpret_cast<const uint32_t*>(k_pages + block + (size_t)page_size * (D / 2) + (size_t)slot * (D / 8));
+            for (int w = 0; w < D / 8; ++w) {
+                uint32_t S2, B2, v[4];
+                kv4_pair(pairs[w / 4], S2, B2);
+                kv4_word(codes[w], S2, B2, v);
+#pragma unroll
+                for (int p = 0; p < 4; ++p) {
+                    const float2 x = kv4_floats(v[p]);
+#pragma unroll
+                    for (int h = 0; h < kHeads; ++h) s[h] = fmaf(qs[h][8 * w + p], x.x, fmaf(qs[h][8 * w + 4 + p], x.y, s[h]));
+                }
+            }
+        }
+#pragma unroll
+        for (int h = 0; h < kHeads; ++h) {
+            const float top = ns_warp_max(seen ? s[h] : -INFINITY), now = fmaxf(m[h], top), use = now == -INFINITY ? 0.f : now;
+            const float keep = expf(m[h] - use), p = seen ? expf(s[h] - use) : 0.f;
+            m[h] = now;
+            l[h] = l[h] * keep + p;
+#pragma unroll
+            for (int c = 0; c < kChunks; ++c)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) o[h][c][i] *= keep;
+            ps[warp][lane][h] = p;
+        }
+        __syncwarp();
+        for (int j = 0; j < count; ++j) {
+            const size_t b = __shfl_sync(0xffffffffu, block, j);
+            const int at = __shfl_sync(0xffffffffu, slot, j);
+#pragma unroll
+            for (int c = 0; c < kChunks; ++c) {
+                const int f = c * 128 + lane * 4;
+                if (f >= D) continue;
+                const uint32_t code = *reinterpret_cast<const uint16_t*>(v_pages + b + (size_t)at * (D / 2) + f / 2);
+                uint32_t S2, B2;
+                kv4_pair(*reinterpret_cast<const uint32_t*>(v_pages + b + (size_t)page_size * (D / 2) + ((size_t)at * (D / kGroup) + f / kGroup) * 4), S2, B2);
+                // codes 0 and 1 beside each other, then 2 and 3
+                const float2 x = kv4_floats(kv4_fma((code << 3) | (code & 0xf0u) << 15, S2, B2));
+                const float2 y = kv4_floats(kv4_fma((code >> 5) | (code & 0xf000u) << 7, S2, B2));
+#pragma unroll
+                for (int h = 0; h < kHeads; ++h) {
+                    const float p = ps[warp][j][h];
+                    o[h][c][0] = fmaf(p, x.x, o[h][c][0]);
+                    o[h][c][1] = fmaf(p, x.y, o[h][c][1]);
+                    o[h][c][2] = fmaf(p, y.x, o[h][c][2]);
+                    o[h][c][3] = fmaf(p, y.y, o[h][c][3]);
+                }
+            }
+        }
+        __syncwarp();
+    }
+#pragma unroll
+    for (int h = 0; h < kHeads; ++h) {
+        l[h] = ns_warp_sum(l[h]);
+        if (lane == 0) { ms[warp][h] = m[h]; ls[warp][h] = l[h]; }
+#pragma unroll
+        for (int c = 0; c < kChunks; ++c)
+            *reinterpret_cast<float4*>(&os[warp][h][c * 128 + lane * 4]) = make_float4(o[h][c][0], o[h][c][1], o[h][c][2], o[h][c][3]);
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < heads * D; i += kThreads) {
+        const int h = i / D, f = i % D;
+        float top = sink ? sink[h0 + h] : -INFINITY;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) top = fmaxf(top, ms[w][h]);
+        float sum = sink ? expf(sink[h0 + h] - top) : 0.f, acc = 0.f;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) {
+            // (a warp that saw no key adds nothing, one whose scores are all NaN makes the row NaN)
+            const float part = ms[w][h] == -INFINITY ? 0.f * ls[w][h] : expf(ms[w][h] - top);
+            sum += part * ls[w][h];
+            acc += part * os[w][h][f];
+        }
+        ns_st(out, (size_t)n * ldo + (size_t)(h0 + h) * D + f, acc / sum);
+    }
+}
+
+template <typename T>
+int launch(const void* q, long long ldq, const void* k, const void* v, const int* table, int table_stride, const int* token_req, const int* positions,
+           const int* rows, int n_rows, void* out, long long ldo, int nq, int nkv, int D, int page_size, float scale, int window, const float* sink,
+           cudaStream_t stream) {
+    const int G = nq / nkv;
+    dim3 grid(n_rows, nkv * ((G + kHeads - 1) / kHeads));
+    if (D <= 128)
+        NS_LAUNCH((attention_kv4_kernel<T, 1>), grid, kThreads, 0, stream, (const T*)q, ldq, (const uint8_t*)k, (const uint8_t*)v, table, table_stride, token_req,
+                  positions, rows, (T*)out, ldo, nq, nkv, D, page_size, scale, window, sink);
+    else
+        NS_LAUNCH((attention_kv4_kernel<T, 2>), grid, kThreads, 0, stream, (const T*)q, ldq, (const uint8_t*)k, (const uint8_t*)v, table, table_stride, token_req,
+                  positions, rows, (T*)out, ldo, nq, nkv, D, page_size, scale, window, sink);
+    NS_CHECK_LAUNCH("ns_attention_kv4");
+    return NS_OK;
+}
+
+}  // namespace
+
+// q [tokens, ldq], out [tokens, ldo]; rows [n_rows]: the tokens to take (null: all n_rows); sink [nq] or null.
+NS_API int ns_attention_kv4(const void* q, long long ldq, const void* k, const void* v, const int* table, int table_stride, const int* token_req,
+                            const int* positions, const int* rows, int n_rows, void* out, long long ldo, int nq, int nkv, int D, int page_size, float scale,
+                            int window, const float* sink, int dtype, cudaStream_t stream) {
+    if (n_rows <= 0) return NS_OK;
+    if (D < kGroup || D % kGroup || D > 256 || nkv < 1 || nq < 1 || nq % nkv || page_size < 1 || window < 0)
+        NS_FAIL(NS_ERR_UNSUPPORTED, "ns_attention_kv4: %d heads of %d over %d, pages of %d, a window of %d", nq, D, nkv, page_size, window);
+    if (nkv * ((nq / nkv + kHeads - 1) / kHeads) > 65535) NS_FAIL(NS_ERR_UNSUPPORTED, "ns_attention_kv4: too many heads (%d)", nq);
+    if (dtype == NS_BF16)
+        return launch<__nv_bfloat16>(q, ldq, k, v, table, table_stride, token_req, positions, rows, n_rows, out, ldo, nq, nkv, D, page_size, scale, window, sink, stream);
+    if (dtype == NS_F32)
+        return launch<float>(q, ldq, k, v, table, table_stride, token_req, positions, rows, n_rows, out, ldo, nq, nkv, D, page_size, scale, window, sink, stream);
+    NS_FAIL(NS_ERR_UNSUPPORTED, "ns_attention_kv4: float32 and bfloat16, not type %d", dtype);
+}

@@ -1,0 +1,264 @@
+// Store into the 4-bit cache, with the rotation of q and k, and reading values back (the format: kv4.cuh).
+//
+// What the cache holds is the definition's to the last bit: angles, their sines and the rotation of k run in double and are rounded once to
+// the activations' type, S and B are rounded once from double, and codes are decided by the exact remainder.  One rounding that fell on
+// the other side of a border would move a feature by a whole code, or a group by its S.  q, which is rounded to the activations' type and not
+// quantised, is rotated in float.
+#include "kv4.cuh"
+
+namespace {
+
+constexpr int kThreads = 256;
+
+// a double to the nearest bfloat16, ties to even, in one rounding: to float towards zero with the last bit marking that something was
+// dropped (float has more than two bits beyond bfloat16's), then to bfloat16
+__device__ __forceinline__ float odd_float(double d) {
+    const float f = __double2float_rz(d);
+    return (double)f == d ? f : __uint_as_float(__float_as_uint(f) | 1u);
+}
+__device__ __forceinline__ __nv_bfloat16 nearest_bf16(double d) { return __float2bfloat16_rn(odd_float(d)); }
+
+__device__ __forceinline__ float as_stored(const float*, double d) { return __double2float_rn(d); }
+__device__ __forceinline__ float as_stored(const __nv_bfloat16*, double d) { return __bfloat162float(nearest_bf16(d)); }
+
+__device__ __forceinline__ void ld4(const float* p, float (&v)[4]) {
+    const float4 a = *reinterpret_cast<const float4*>(p);
+    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+}
+__device__ __forceinline__ void ld4(const __nv_bfloat16* p, float (&v)[4]) {
+    const uint2 u = *reinterpret_cast<const uint2*>(p);
+    const float2 a = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&u.x)), b = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&u.y));
+    v[0] = a.x; v[1] = a.y; v[2] = b.x; v[3] = b.y;
+}
+__device__ __forceinline__ void st4(float* p, const float (&v)[4]) { *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]); }
+__device__ __forceinline__ void st4(__nv_bfloat16* p, const float (&v)[4]) {
+    const __nv_bfloat162 a = __floats2bfloat162_rn(v[0], v[1]), b = __floats2bfloat162_rn(v[2], v[3]);
+    *reinterpret_cast<uint2*>(p) = make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
+}
+
+// the code of x in a group: the integer nearest to 16 (x - B) / S - 16, ties to even, within 0 .. 15
+__device__ __forceinline__ uint32_t code_of(float x, float S, float B, float inv) {
+    // d + rest = x - B without error
+    const float d = __fsub_rn(x, B), back = __fsub_rn(d, x);
+    const float rest = __fadd_rn(__fsub_rn(x, __fsub_rn(d, back)), __fsub_rn(-B, back));
+    const float step = S * 0.0625f, half = 0.5f * step;
+    float k = rintf(d * inv);
+    const float e = fmaf(-k, step, d);  // exact where the code is not clamped: d is at most 33 steps
+    const bool odd = ((int)k) & 1;
+    if (e > half || (e == half && (rest > 0.f || (rest == 0.f && odd)))) k += 1.f;
+    else if (e < -half || (e == -half && (rest < 0.f || (rest == 0.f && odd)))) k -= 1.f;
+    return (uint32_t)fminf(fmaxf(k - 16.f, 0.f), 15.f);
+}
+
+struct Group { __nv_bfloat16 S, B; };
+
+// S and B of a group that lies over 8 neighbouring lanes, four features each; S is NaN where the group is not finite
+__device__ __forceinline__ Group group_of(const float (&x)[4], bool live) {
+    float lo = fminf(fminf(x[0], x[1]), fminf(x[2], x[3])), hi = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
+    // (x - x is NaN for infinities and NaN, whose presence the minimum and maximum would hide)
+    bool bad = live && !((x[0] - x[0]) + (x[1] - x[1]) + (x[2] - x[2]) + (x[3] - x[3]) == 0.f);
+#pragma unroll
+    for (int o = 1; o < 8; o <<= 1) {
+        lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+        hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+        bad |= (bool)__shfl_xor_sync(0xffffffffu, (int)bad, o);
+    }
+    const double spread = ((double)hi - (double)lo) * 16.0 / 15.0;
+    Group g;
+    g.S = spread < 7.888609052210118e-31 /* 2^-100 */ ? __float2bfloat16_rn(0.f) : nearest_bf16(spread);
+    g.B = nearest_bf16((double)lo - (double)__bfloat162float(g.S));
+    const float s = __bfloat162float(g.S), b = __bfloat162float(g.B);
+    if (bad || !((s - s) + (b - b) == 0.f)) g.S = g.B = __ushort_as_bfloat16(0x7fff);
+    return g;
+}
+
+// four neighbouring codes and, from one lane of the group, its pair (codes of 0 where S is not a positive number)
+__device__ __forceinline__ void put_group(const float (&x)[4], Group g, uint8_t* codes, uint8_t* pair, bool first) {
+    const float S = __bfloat162float(g.S), B = __bfloat162float(g.B);
+    uint32_t c = 0u;
+    if (S > 0.f) {
+        const float inv = __fdiv_rn(16.f, S);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) c |= code_of(x[i], S, B, inv) << (4 * i);
+    }
+    *reinterpret_cast<uint16_t*>(codes) = (uint16_t)c;
+    if (first) *reinterpret_cast<__nv_bfloat162*>(pair) = __halves2bfloat162(g.S, g.B);
+}
+
+// One block (or `gridDim.y` blocks, which share its heads) per token; a warp takes a head of q, or a kv head's key and value.
+// A lane holds four neighbouring features of every 128, eight lanes a group.
+template <typename T, int kChunks>
+__global__ void __launch_bounds__(kThreads)
+kv4_store_kernel(const T* __restrict__ qkv, long long ld, T* __restrict__ q_out, long long ldq, const int* __restrict__ positions,
+                 const int* __restrict__ token_req, const int* __restrict__ block_table, int table_stride, const float* __restrict__ inv_freq,
+                 int pairs, uint8_t* __restrict__ k_pages, uint8_t* __restrict__ v_pages, int page_size, int nq, int nkv, int D) {
+    ns_pdl_launch_dependents();
+    __shared__ double cs[256];  // cos of the token's angles, then their sines
+    const int n = blockIdx.x, half = D / 2;
+    const int req = token_req[n];
+    if (req < 0) { ns_pdl_wait(); return; }  // a padding row (it waits all the same: see common.cuh)
+    const int pos = positions[n];
+    const int page = block_table[(size_t)req * table_stride + pos / page_size];
+    for (int j = threadIdx.x; j < half; j += kThreads) {
+        double s = 0.0, c = 1.0;
+        if (j < pairs) sincos((double)pos * (double)inv_freq[j], &s, &c);
+        cs[j] = c;
+        cs[half + j] = s;
+    }
+    __syncthreads();
+    ns_pdl_wait();
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = kThreads / 32 * gridDim.y;
+    const T* row = qkv + (size_t)n * ld;
+    const int first = blockIdx.y * (kThreads / 32) + warp;
+    // heads 0 .. nkv - 1 here are the kv heads, which take longer, then those of q (none without a rotation whose output stays in place)
+    const int units = nkv + (pairs > 0 || q_out != qkv ? nq : 0);
+    for (int u = first; u < units; u += warps) {
+        if (u >= nkv) {
+            const T* x = row + (size_t)(u - nkv) * D;
+            T* y = q_out + (size_t)n * ldq + (size_t)(u - nkv) * D;
+            // (both halves of a pair in one lane: q may be rotated in place)
+            for (int f = lane * 4; f < half; f += 128) {
+                float a[4], b[4], oa[4], ob[4];
+                ld4(x + f, a);
+                ld4(x + half + f, b);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float c = (float)cs[f + i], s = (float)cs[half + f + i];
+                    oa[i] = __fmaf_rn(a[i], c, -__fmul_rn(b[i], s));
+                    ob[i] = __fmaf_rn(b[i], c, __fmul_rn(a[i], s));
+                }
+                st4(y + f, oa);
+                st4(y + half + f, ob);
+            }
+            continue;
+        }
+        const T* kx = row + (size_t)(nq + u) * D;
+        const T* vx = kx + (size_t)nkv * D;
+        float k[kChunks][4], v[kChunks][4];
+        Group gk[kChunks], gv[kChunks];
+        bool bad = false;  // the token's key or value is not finite
+#pragma unroll
+        for (int ch = 0; ch < kChunks; ++ch) {
+            const int f = ch * 128 + lane * 4;
+            const bool live = f < D;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) k[ch][i] = v[ch][i] = 0.f;
+            if (live) {
+                const bool low = f < half;
+                const int j = low ? f : f - half;
+                float mine[4], other[4];
+                ld4(kx + f, mine);
+                ld4(kx + (low ? f + half : j), other);
+                ld4(vx + f, v[ch]);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const double c = cs[j + i], s = low ? -cs[half + j + i] : cs[half + j + i];
+                    k[ch][i] = as_stored(qkv, fma((double)mine[i], c, (double)other[i] * s));
+                }
+            }
+            gk[ch] = group_of(k[ch], live);
+            gv[ch] = group_of(v[ch], live);
+            bad |= live && (__hisnan(gk[ch].S) || __hisnan(gv[ch].S));
+        }
+        bad = __any_sync(0xffffffffu, bad);
+        const size_t block = ((size_t)page * nkv + u) * kv4_block_bytes(page_size, D);
+        const int slot = pos % page_size;
+#pragma unroll
+        for (int ch = 0; ch < kChunks; ++ch) {
+            const int f = ch * 128 + lane * 4;
+            if (f >= D) break;
+            const size_t codes = block + (size_t)slot * half + f / 2;
+            const size_t pair = block + (size_t)page_size * half + ((size_t)slot * (D / kGroup) + f / kGroup) * 4;
+            const Group nan = {__ushort_as_bfloat16(0x7fff), __ushort_as_bfloat16(0x7fff)}, zero = {__ushort_as_bfloat16(0), __ushort_as_bfloat16(0)};
+            put_group(k[ch], bad ? nan : gk[ch], k_pages + codes, k_pages + pair, (lane & 7) == 0);
+            put_group(v[ch], __hisnan(gv[ch].S) ? zero : gv[ch], v_pages + codes, v_pages + pair, (lane & 7) == 0);
+        }
+    }
+}
+
+// One value of a word (eight features) per thread: k and v of (token, kv head).
+__global__ void __launch_bounds__(kThreads)
+kv4_read_kernel(const uint8_t* __restrict__ k_pages, const uint8_t* __restrict__ v_pages, const int* __restrict__ positions,
+                const int* __restrict__ token_req, const int* __restrict__ block_table, int table_stride, __nv_bfloat16* __restrict__ k_out,
+                __nv_bfloat16* __restrict__ v_out, int n_tokens, int page_size, int nkv, int D) {
+    ns_pdl_launch_dependents();
+    ns_pdl_wait();
+    const int words = D / 8;
+    const long long total = (long long)n_tokens * nkv * words;
+    for (long long i = (long long)blockIdx.x * kThreads + threadIdx.x; i < total; i += (long long)gridDim.x * kThreads) {
+        const int w = (int)(i % words);
+        const long long th = i / words;
+        const int h = (int)(th % nkv), n = (int)(th / nkv);
+        const int req = token_req[n];
+        uint32_t k[4] = {0u, 0u, 0u, 0u}, v[4] = {0u, 0u, 0u, 0u};
+        if (req >= 0) {
+            const int pos = positions[n], slot = pos % page_size;
+            const int page = block_table[(size_t)req * table_stride + pos / page_size];
+            const size_t block = ((size_t)page * nkv + h) * kv4_block_bytes(page_size, D);
+            const size_t codes = block + ((size_t)slot * words + w) * 4;
+            const size_t pair = block + (size_t)page_size * (D / 2) + ((size_t)slot * (D / kGroup) + w / 4) * 4;
+            uint32_t S2, B2;
+            kv4_pair(*reinterpret_cast<const uint32_t*>(k_pages + pair), S2, B2);
+            kv4_word(*reinterpret_cast<const uint32_t*>(k_pages + codes), S2, B2, k);
+            kv4_pair(*reinterpret_cast<const uint32_t*>(v_pages + pair), S2, B2);
+            kv4_word(*reinterpret_cast<const uint32_t*>(v_pages + codes), S2, B2, v);
+        }
+        // from (0, 4) (1, 5) (2, 6) (3, 7) to features in order
+        auto in_order = [](const uint32_t (&p)[4]) {
+            return make_uint4(__byte_perm(p[0], p[1], 0x5410), __byte_perm(p[2], p[3], 0x5410), __byte_perm(p[0], p[1], 0x7632), __byte_perm(p[2], p[3], 0x7632));
+        };
+        *reinterpret_cast<uint4*>(k_out + i * 8) = in_order(k);
+        *reinterpret_cast<uint4*>(v_out + i * 8) = in_order(v);
+    }
+}
+
+int check_geometry(const char* who, int D, int nkv, int page_size) {
+    if (D < kGroup || D % kGroup || D > 256 || nkv < 1 || page_size < 1)
+        NS_FAIL(NS_ERR_UNSUPPORTED, "%s: heads of %d (multiples of 32 up to 256), %d kv heads, pages of %d", who, D, nkv, page_size);
+    return NS_OK;
+}
+
+}  // namespace
+
+// qkv [n_tokens, ld] in the activations' type; q rotated into q_out [n_tokens, ldq] (which may be qkv itself), k and v into the cache.  `pairs`:
+// features j and j + D / 2 with j < pairs are rotated by positions[n] * inv_freq[j] (0: none).
+NS_API int ns_kv4_store(const void* qkv, long long ld, void* q_out, long long ldq, const int* positions, const int* token_req, const int* block_table,
+                        int table_stride, const float* inv_freq, int pairs, void* k_pages, void* v_pages, int page_size, int nq, int nkv, int D,
+                        int n_tokens, int sms, int dtype, cudaStream_t stream) {
+    if (n_tokens <= 0) return NS_OK;
+    int rc = check_geometry("ns_kv4_store", D, nkv, page_size);
+    if (rc) return rc;
+    const int size = dtype == NS_BF16 ? 2 : 4;
+    if (nq < 1 || pairs < 0 || pairs > D / 2 || ld * size % 16 || ldq * size % 16 || ((uintptr_t)qkv | (uintptr_t)q_out) % 16 || ((uintptr_t)k_pages | (uintptr_t)v_pages) % 4)
+        NS_FAIL(NS_ERR_ARGUMENT, "ns_kv4_store: rows on 16-byte boundaries, at most %d rotated pairs (%d)", D / 2, pairs);
+    // a token's heads over several blocks while there are fewer tokens than SMs
+    const int most = (nq + nkv + kThreads / 32 - 1) / (kThreads / 32);
+    int parts = (2 * sms + n_tokens - 1) / n_tokens;
+    parts = parts < 1 ? 1 : parts > most ? most : parts;
+    dim3 grid(n_tokens, parts);
+#define NS_KV4_STORE(T, CHUNKS)                                                                                                       \
+    NS_LAUNCH((kv4_store_kernel<T, CHUNKS>), grid, kThreads, 0, stream, (const T*)qkv, ld, (T*)q_out, ldq, positions, token_req,    \
+              block_table, table_stride, inv_freq, pairs, (uint8_t*)k_pages, (uint8_t*)v_pages, page_size, nq, nkv, D)
+    if (dtype == NS_BF16 && D <= 128) NS_KV4_STORE(__nv_bfloat16, 1);
+    else if (dtype == NS_BF16) NS_KV4_STORE(__nv_bfloat16, 2);
+    else if (dtype == NS_F32 && D <= 128) NS_KV4_STORE(float, 1);
+    else if (dtype == NS_F32) NS_KV4_STORE(float, 2);
+    else NS_FAIL(NS_ERR_UNSUPPORTED, "ns_kv4_store: float32 and bfloat16, not type %d", dtype);
+#undef NS_KV4_STORE
+    NS_CHECK_LAUNCH("ns_kv4_store");
+    return NS_OK;
+}
+
+// k_out, v_out [n_tokens, nkv, D]: what the cache holds at positions[n] of request token_req[n] (zeros where that is negative).
+NS_API int ns_kv4_read(const void* k_pages, const void* v_pages, const int* positions, const int* token_req, const int* block_table, int table_stride,
+                       void* k_out, void* v_out, int n_tokens, int page_size, int nkv, int D, int sms, cudaStream_t stream) {
+    if (n_tokens <= 0) return NS_OK;
+    int rc = check_geometry("ns_kv4_read", D, nkv, page_size);
+    if (rc) return rc;
+    const long long items = (long long)n_tokens * nkv * (D / 8), blocks = (items + kThreads - 1) / kThreads;
+    const int grid = (int)(blocks < 16ll * sms ? blocks : 16ll * sms);
+    NS_LAUNCH(kv4_read_kernel, grid, kThreads, 0, stream, (const uint8_t*)k_pages, (const uint8_t*)v_pages, positions, token_req, block_table, table_stride,
+              (__nv_bfloat16*)k_out, (__nv_bfloat16*)v_out, n_tokens, page_size, nkv, D);
+    NS_CHECK_LAUNCH("ns_kv4_read");
+    return NS_OK;
+}

@@ -1,0 +1,110 @@
+// Rows in 8-bit integers with a float scale each: s = max |x| / 127 rounded to float, q = x / s to the nearest integer, ties to even.
+//
+// The quotient that is rounded is the exact one: a first guess from the reciprocal is off by one at most, and the remainder
+// x - q s, which one fused multiply-add gives without error (its bits are no finer than half of s's last and it is at most about s / 2),
+// says whether the guess stays.  The maximum is taken over the bit patterns of |x|, in whose order infinities and NaN come last.
+//
+// Bound by memory: a row is read once (its pieces stay in registers where the block holds them) and written once in a byte per element.
+#include "common.cuh"
+
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kHeld = 4;  // pieces of 8 elements that a thread keeps: rows of up to 8,192
+
+__device__ __forceinline__ int nearest(float x, float s, float inv) {
+    float r = rintf(x * inv);
+    const float e = fmaf(-r, s, x), half = 0.5f * s;
+    const bool odd = ((int)r) & 1;
+    if (e > half || (e == half && odd)) r += 1.f;
+    else if (e < -half || (e == -half && odd)) r -= 1.f;
+    return (int)r;
+}
+
+template <typename T>
+__device__ __forceinline__ void load_piece(const T* row, int k, int K, bool wide, float (&v)[8]) {
+    if (wide && k + 8 <= K) {
+        ld8(row + k, v);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = k + i < K ? ns_ld(row, k + i) : 0.f;
+    }
+}
+
+__device__ __forceinline__ void store_piece(int8_t* out, int k, int K, const float (&v)[8], float s, float inv) {
+    uint32_t w[2] = {0u, 0u};
+    if (inv != 0.f) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) w[i >> 2] |= ((uint32_t)nearest(v[i], s, inv) & 255u) << (8 * (i & 3));
+    }
+    if (k + 8 <= K) {
+        *reinterpret_cast<uint2*>(out + k) = make_uint2(w[0], w[1]);
+    } else {
+        for (int i = 0; k + i < K; ++i) out[k + i] = (int8_t)(w[i >> 2] >> (8 * (i & 3)));
+    }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kThreads)
+quantize_rows_kernel(const T* __restrict__ x, long long ldx, int8_t* __restrict__ q, long long ldq, float* __restrict__ scale, int K, int wide) {
+    ns_pdl_launch_dependents();
+    ns_pdl_wait();
+    __shared__ uint32_t tops[kThreads / 32];
+    const T* row = x + (size_t)blockIdx.x * ldx;
+    float v[kHeld][8];
+    uint32_t top = 0u;
+    for (int k = threadIdx.x * 8, i = 0; k < K; k += kThreads * 8, ++i) {
+        float t[8];
+        load_piece(row, k, K, wide, t);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) top = max(top, __float_as_uint(t[j]) & 0x7fffffffu);
+#pragma unroll
+        for (int u = 0; u < kHeld; ++u)
+            if (u == i)
+#pragma unroll
+                for (int j = 0; j < 8; ++j) v[u][j] = t[j];
+    }
+    top = __reduce_max_sync(0xffffffffu, top);
+    if ((threadIdx.x & 31) == 0) tops[threadIdx.x >> 5] = top;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kThreads / 32; ++w) top = max(top, tops[w]);
+    float s = __fdiv_rn(__uint_as_float(top), 127.f), inv = 0.f;
+    if (top >= 0x7f800000u) s = __uint_as_float(0x7fffffffu);  // an infinity or a NaN: the row has no scale
+    else if (s < 7.52316385e-37f) s = 0.f;                     // 2^-120: a row of zeros
+    else inv = __frcp_rn(s);
+    if (threadIdx.x == 0) scale[blockIdx.x] = s;
+    int8_t* out = q + (size_t)blockIdx.x * ldq;
+    for (int k = threadIdx.x * 8, i = 0; k < K; k += kThreads * 8, ++i) {
+        float t[8];
+        if (i < kHeld) {
+#pragma unroll
+            for (int u = 0; u < kHeld; ++u)
+                if (u == i)
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) t[j] = v[u][j];
+        } else {
+            load_piece(row, k, K, wide, t);
+        }
+        store_piece(out, k, K, t, s, inv);
+    }
+}
+
+}  // namespace
+
+// q [rows, ldq] (8-bit integers, rows on 8-byte boundaries) and scale [rows] of x [rows, ldx].  A row that holds an infinity or a NaN gets
+// NaN for its scale and zeros; one whose scale would be below 2^-120 gets zeros and 0.
+NS_API int ns_quantize_rows(const void* x, long long ldx, void* q, long long ldq, float* scale, int rows, int K, int dtype, cudaStream_t stream) {
+    if (rows <= 0) return NS_OK;
+    if (K < 1 || ldq % 8 || (uintptr_t)q % 8) NS_FAIL(NS_ERR_ARGUMENT, "ns_quantize_rows: %d columns, output rows %lld apart (multiples of 8 on an 8-byte boundary)", K, ldq);
+    const int size = dtype == NS_BF16 ? 2 : 4;
+    const int wide = (uintptr_t)x % 16 == 0 && ldx * size % 16 == 0;
+    if (dtype == NS_BF16)
+        NS_LAUNCH((quantize_rows_kernel<__nv_bfloat16>), rows, kThreads, 0, stream, (const __nv_bfloat16*)x, ldx, (int8_t*)q, ldq, scale, K, wide);
+    else if (dtype == NS_F32)
+        NS_LAUNCH((quantize_rows_kernel<float>), rows, kThreads, 0, stream, (const float*)x, ldx, (int8_t*)q, ldq, scale, K, wide);
+    else
+        NS_FAIL(NS_ERR_UNSUPPORTED, "ns_quantize_rows: float32 and bfloat16, not type %d", dtype);
+    NS_CHECK_LAUNCH("ns_quantize_rows");
+    return NS_OK;
+}

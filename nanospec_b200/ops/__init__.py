@@ -43,6 +43,14 @@ def _cuda(*tensors: torch.Tensor | None) -> None:
             raise KernelError("kernel operands must live on a CUDA device; there is no CPU path")
 
 
+def _on_current_device(*tensors: torch.Tensor | None) -> None:
+    """Operands of one launch: all on the current CUDA device, whose current stream the kernels go to."""
+    _cuda(*tensors)
+    for t in tensors:
+        if t is not None and t.device.index != torch.cuda.current_device():
+            raise KernelError(f"an operand lies on {t.device}, the current device is cuda:{torch.cuda.current_device()}")
+
+
 def _ptr(t: torch.Tensor | None) -> int | None:
     return None if t is None else t.data_ptr()
 
@@ -1931,3 +1939,7 @@ def head_prepare_store(proj: torch.Tensor, out: torch.Tensor, ctx, lane, nq: int
     if n_taps > 1:
         lib.call("ns_conv_tail", proj.data_ptr(), proj.stride(0), state.data_ptr(), state_floats, 0, ctx.qo_indptr.data_ptr(),
                  ctx.state_slot.data_ptr(), cols, n_taps, ctx.n_requests, dtype_code(proj.dtype), _stream())
+
+
+from .int8 import I8_MAX_K, RowsI8, linear_i8, quantize_rows  # noqa: E402,F401
+from .kv4 import KV4_GROUP, attention_kv4, kv4_block_bytes, kv4_pages, kv4_read, kv4_store  # noqa: E402,F401

@@ -1,0 +1,82 @@
+"""Products in 8-bit integers: rows quantised with a float32 scale each (tokens of activations, output channels of weights) and
+their matrix product with an exact integer sum (csrc/quantize_rows.cu, csrc/gemm_i8.cu)."""
+
+from __future__ import annotations
+
+from dataclasses import dataclass
+
+import torch
+
+from . import _on_current_device, _ptr, _stream, dtype_code, lib
+from .lib import KernelError
+
+I8_MAX_K = 131072  # 127 * 127 * K stays within 32 bits
+
+
+@dataclass
+class RowsI8:
+    """A matrix in 8-bit integers: `q` [R, K] int8 (rows on 16-byte boundaries) and `scale` [R] float32; row r stands for q[r] * scale[r]."""
+
+    q: torch.Tensor
+    scale: torch.Tensor
+
+    @property
+    def shape(self) -> torch.Size:
+        return self.q.shape
+
+    def values(self) -> torch.Tensor:
+        """float32, for inspection."""
+        return self.q.float() * self.scale[:, None]
+
+
+def _aligned_rows(q: torch.Tensor) -> bool:
+    return q.stride(1) == 1 and q.stride(0) % 16 == 0 and q.data_ptr() % 16 == 0
+
+
+def _check_rows(r: RowsI8, name: str) -> None:
+    if r.q.dtype != torch.int8 or r.q.dim() != 2 or r.scale.dtype != torch.float32 or r.scale.shape != (r.q.shape[0],) or not r.scale.is_contiguous():
+        raise KernelError(f"linear_i8: {name} must be int8 [R, K] with one contiguous float32 scale per row")
+    if r.q.shape[0] and not _aligned_rows(r.q):
+        raise KernelError(f"linear_i8: the rows of {name} must start on 16-byte boundaries with unit inner stride (quantize_rows makes them so)")
+
+
+def quantize_rows(x: torch.Tensor) -> RowsI8:
+    """x [R, K] (float32 or bfloat16, unit inner stride) in 8-bit integers: scale[r] = float32(max |x[r]| / 127) and q[r] the integers
+    nearest to x[r] / scale[r] (ties to even).  A row that holds an infinity or a NaN gets NaN for its scale and zeros; a row whose scale
+    would be below 2^-120 gets 0 and zeros.  Weights go through it once, an output channel a row; `linear_i8` takes activations as they are
+    or quantised."""
+    _on_current_device(x)
+    if x.dim() != 2 or x.stride(1) != 1 or not 1 <= x.shape[1] <= I8_MAX_K:
+        raise KernelError(f"quantize_rows: a matrix with unit inner stride and 1 to {I8_MAX_K} columns is needed, not {tuple(x.shape)} with strides {x.stride()}")
+    rows, K = x.shape
+    code = dtype_code(x.dtype)
+    q = torch.empty((rows, -(-K // 16) * 16), dtype=torch.int8, device=x.device)[:, :K]
+    scale = torch.empty(rows, dtype=torch.float32, device=x.device)
+    lib.call("ns_quantize_rows", x.data_ptr(), x.stride(0), q.data_ptr(), q.stride(0), scale.data_ptr(), rows, K, code, _stream())
+    return RowsI8(q, scale)
+
+
+def linear_i8(x: torch.Tensor | RowsI8, w: RowsI8, out: torch.Tensor, bias: torch.Tensor | None = None) -> torch.Tensor:
+    """out[n, f] = (sum_k xq[n, k] wq[f, k]) * xs[n] * ws[f] (+ bias[f], float32), the sum exact in 32-bit integers.  `x` [N, K] is quantised by
+    rows on the way (`quantize_rows`) unless it comes so, for several products of the same activations; `out` [N, F] is float32 or bfloat16
+    with unit inner stride."""
+    held = x.q if isinstance(x, RowsI8) else x
+    _on_current_device(held, w.q, w.scale, out, bias)
+    _check_rows(w, "w")
+    N, (F, K) = held.shape[0], w.q.shape
+    if held.dim() != 2 or held.shape[1] != K or not 1 <= K <= I8_MAX_K:
+        raise KernelError(f"linear_i8: x {tuple(held.shape)} and w {tuple(w.q.shape)} do not agree, or K is beyond {I8_MAX_K}")
+    if out.shape != (N, F) or (F and out.stride(1) != 1):
+        raise KernelError(f"linear_i8: out must be [{N}, {F}] with unit inner stride, not {tuple(out.shape)} with strides {out.stride()}")
+    if bias is not None and (bias.dtype != torch.float32 or bias.shape != (F,) or not bias.is_contiguous()):
+        raise KernelError("linear_i8: the bias is one contiguous float32 number per output feature")
+    code = dtype_code(out.dtype)
+    if isinstance(x, RowsI8):
+        _check_rows(x, "x")
+        _on_current_device(x.scale)
+    if N == 0 or F == 0:
+        return out
+    rows = x if isinstance(x, RowsI8) else quantize_rows(x)
+    lib.call("ns_gemm_i8", rows.q.data_ptr(), rows.q.stride(0), rows.scale.data_ptr(), w.q.data_ptr(), w.q.stride(0), w.scale.data_ptr(), _ptr(bias),
+             out.data_ptr(), out.stride(0), N, F, K, code, _stream())
+    return out

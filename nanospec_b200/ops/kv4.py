@@ -1,0 +1,105 @@
+"""A paged cache of keys and values in 4 bits: the store (with the rotation), reading back, and attention over it.  A lane's `k` and `v`
+are then uint8 [pages, kv heads, page_size * head_dim * 5 / 8] (`kv4_pages`); csrc/kv4.cuh says what the bytes are and stand for."""
+
+from __future__ import annotations
+
+import math
+
+import torch
+
+from . import _i32, _on_current_device, _ptr, _stream, dtype_code, lib, sm_count
+from .lib import KernelError
+
+KV4_GROUP = 32  # features that share a pair of numbers
+KV4_MAX_HEAD = 256
+
+
+def kv4_block_bytes(page_size: int, head_dim: int) -> int:
+    """Bytes of a page of one kv head (of keys, and as many of values): half a byte a feature and 4 bytes a group of 32."""
+    if head_dim % KV4_GROUP or not KV4_GROUP <= head_dim <= KV4_MAX_HEAD or page_size < 1:
+        raise KernelError(f"a 4-bit cache takes heads in multiples of {KV4_GROUP} up to {KV4_MAX_HEAD} and pages of one token at least, not {head_dim} and {page_size}")
+    return page_size * head_dim * 5 // 8
+
+
+def kv4_pages(pages: int, kv_heads: int, page_size: int, head_dim: int, device: torch.device | str = "cuda") -> torch.Tensor:
+    """Pages of keys, or of values, of a lane: every feature zero."""
+    return torch.zeros((pages, kv_heads, kv4_block_bytes(page_size, head_dim)), dtype=torch.uint8, device=device)
+
+
+def _check_lane(who: str, lane, nkv: int, head_dim: int) -> None:
+    size = kv4_block_bytes(lane.page_size, head_dim)
+    for t in (lane.k, lane.v):
+        if t is None or t.dtype != torch.uint8 or t.dim() != 3 or t.shape[1:] != (nkv, size) or not t.is_contiguous() or t.data_ptr() % 16:
+            raise KernelError(f"{who}: the lane's pages must be contiguous uint8 [pages, {nkv}, {size}] on 16-byte boundaries (kv4_pages makes them)")
+    if lane.block_table is None or lane.block_table.dtype != torch.int32 or lane.block_table.dim() != 2 or lane.block_table.stride(1) != 1:
+        raise KernelError(f"{who}: block_table must be int32 [requests, pages] with unit inner stride")
+
+
+def _check_step(who: str, positions: torch.Tensor, token_req: torch.Tensor, n: int) -> None:
+    _i32(positions, "positions"), _i32(token_req, "token_req")
+    if positions.numel() != n or token_req.numel() != n:
+        raise KernelError(f"{who}: one position and one request per token ({n})")
+
+
+def kv4_store(qkv: torch.Tensor, ctx, lane, nq: int, nkv: int, head_dim: int, inv_freq: torch.Tensor | None = None,
+              q_out: torch.Tensor | None = None) -> torch.Tensor:
+    """Rotates q and k of the packed [q | k | v] rows (pairs j and j + head_dim / 2 by position * inv_freq[j]; None: as they are), writes k
+    and v in 4 bits at each token's position, and q to `q_out` ([N, nq * head_dim]; None: in place).  The rotated k is rounded to the
+    activations' type before it is quantised, as a cache in that type would hold it.  Rows of padding (token_req < 0) are left as they
+    are.  Returns where q went."""
+    _on_current_device(qkv, ctx.positions, ctx.token_req, lane.block_table, lane.k, lane.v, inv_freq, q_out)
+    _check_lane("kv4_store", lane, nkv, head_dim)
+    code, size = dtype_code(qkv.dtype), qkv.element_size()
+    n = qkv.shape[0]
+    _check_step("kv4_store", ctx.positions, ctx.token_req, n)
+    if qkv.dim() != 2 or qkv.shape[1] != (nq + 2 * nkv) * head_dim or nq < 1:
+        raise KernelError(f"kv4_store: qkv must be [N, {(nq + 2 * nkv) * head_dim}], not {tuple(qkv.shape)}")
+    target = qkv if q_out is None else q_out
+    if q_out is not None and (q_out.dtype != qkv.dtype or q_out.shape != (n, nq * head_dim)):
+        raise KernelError("kv4_store: q_out must be [N, nq * head_dim] in the type of qkv")
+    for t in (qkv, target):
+        if n and (t.stride(1) != 1 or t.stride(0) * size % 16 or t.data_ptr() % 16):
+            raise KernelError("kv4_store: rows must start on 16-byte boundaries with unit inner stride")
+    if inv_freq is not None and (inv_freq.dtype != torch.float32 or not inv_freq.is_contiguous() or inv_freq.numel() > head_dim // 2):
+        raise KernelError(f"kv4_store: inv_freq must be contiguous float32, at most {head_dim // 2} numbers")
+    lib.call("ns_kv4_store", qkv.data_ptr(), qkv.stride(0), target.data_ptr(), target.stride(0), ctx.positions.data_ptr(), ctx.token_req.data_ptr(),
+             lane.block_table.data_ptr(), lane.block_table.stride(0), _ptr(inv_freq), 0 if inv_freq is None else inv_freq.numel(), lane.k.data_ptr(),
+             lane.v.data_ptr(), lane.page_size, nq, nkv, head_dim, n, sm_count(), code, _stream())
+    return target
+
+
+def kv4_read(lane, positions: torch.Tensor, token_req: torch.Tensor, nkv: int, head_dim: int) -> tuple[torch.Tensor, torch.Tensor]:
+    """What the cache holds at positions[n] of request token_req[n]: keys and values [N, nkv, head_dim] in bfloat16, as `attention_kv4` sees them
+    (zeros where token_req is negative)."""
+    _on_current_device(lane.k, lane.v, lane.block_table, positions, token_req)
+    _check_lane("kv4_read", lane, nkv, head_dim)
+    n = positions.numel()
+    _check_step("kv4_read", positions, token_req, n)
+    k, v = (torch.empty((n, nkv, head_dim), dtype=torch.bfloat16, device=lane.k.device) for _ in range(2))
+    lib.call("ns_kv4_read", lane.k.data_ptr(), lane.v.data_ptr(), positions.data_ptr(), token_req.data_ptr(), lane.block_table.data_ptr(),
+             lane.block_table.stride(0), k.data_ptr(), v.data_ptr(), n, lane.page_size, nkv, head_dim, sm_count(), _stream())
+    return k, v
+
+
+def attention_kv4(qkv: torch.Tensor, lane, ctx, out: torch.Tensor, nq: int, nkv: int, head_dim: int, scale: float | None = None, window: int = 0,
+                  sink: torch.Tensor | None = None) -> torch.Tensor:
+    """Attention of the step's queries (the first nq * head_dim columns of `qkv`, rotated) over a lane in 4 bits: every token sees the positions
+    up to its own (with `window` the last so many of them), which `kv4_store` has filled.  `sink` (float32 [nq]): the softmax's denominator also
+    holds exp(sink[h]).  `scale` is head_dim ** -0.5 when None.  float32 and bfloat16; rows of padding (token_req < 0) are left as they are."""
+    _on_current_device(qkv, out, lane.k, lane.v, lane.block_table, ctx.positions, ctx.token_req, sink)
+    _check_lane("attention_kv4", lane, nkv, head_dim)
+    n = out.shape[0]
+    code = dtype_code(qkv.dtype)
+    _check_step("attention_kv4", ctx.positions, ctx.token_req, n)
+    if nq < 1 or nq % nkv or window < 0:
+        raise KernelError(f"attention_kv4: {nq} query heads over {nkv}, a window of {window}")
+    if qkv.dim() != 2 or qkv.shape[0] != n or qkv.shape[1] < nq * head_dim or out.shape != (n, nq * head_dim) or out.dtype != qkv.dtype \
+            or (n and (qkv.stride(1) != 1 or out.stride(1) != 1)):
+        raise KernelError(f"attention_kv4: q [N, >= {nq * head_dim}] and out [N, {nq * head_dim}] in one type with unit inner strides are needed")
+    if sink is not None and (sink.dtype != torch.float32 or sink.numel() != nq or not sink.is_contiguous()):
+        raise KernelError("attention_kv4: the sink is one contiguous float32 number per query head")
+    scale = 1.0 / math.sqrt(head_dim) if scale is None else float(scale)
+    lib.call("ns_attention_kv4", qkv.data_ptr(), qkv.stride(0), lane.k.data_ptr(), lane.v.data_ptr(), lane.block_table.data_ptr(), lane.block_table.stride(0),
+             ctx.token_req.data_ptr(), ctx.positions.data_ptr(), None, n, out.data_ptr(), out.stride(0), nq, nkv, head_dim, lane.page_size, scale, int(window),
+             _ptr(sink), code, _stream())
+    return out
