@@ -47,8 +47,8 @@ __device__ __forceinline__ void store_piece(int8_t* out, int k, int K, const flo
 template <typename T>
 __global__ void __launch_bounds__(kThreads)
 quantize_rows_kernel(const T* __restrict__ x, long long ldx, int8_t* __restrict__ q, long long ldq, float* __restrict__ scale, int K, int wide) {
-    ns_pdl_launch_dependents();
     ns_pdl_wait();
+    ns_pdl_launch_dependents();  // in this order: the product asks for its weights without a wait of its own, and a kernel before this one may have written them
     __shared__ uint32_t tops[kThreads / 32];
     const T* row = x + (size_t)blockIdx.x * ldx;
     float v[kHeld][8];

@@ -107,6 +107,15 @@ __device__ __forceinline__ void umma_bf16_ts(uint32_t tmem_d, uint32_t tmem_a, u
         ::"r"(tmem_d), "r"(tmem_a), "l"(desc_b), "r"(idesc), "r"(accumulate)
         : "memory");
 }
+// 8-bit integers, 32-bit sums: 32 of the contracted dimension
+__device__ __forceinline__ void umma_i8(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}"
+        ::"r"(tmem_d), "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
 __device__ __forceinline__ void tmem_ld8(uint32_t taddr, uint32_t (&r)[8]) {
     asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
@@ -249,6 +258,14 @@ __device__ __forceinline__ void umma_bf16_pair(uint32_t tmem_d, uint64_t desc_a,
         ::"r"(tmem_d), "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(accumulate)
         : "memory");
 }
+__device__ __forceinline__ void umma_i8_pair(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t}"
+        ::"r"(tmem_d), "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
 // arrives at the barrier of this address in both blocks once the leader's products are complete
 __device__ __forceinline__ void umma_commit_pair(uint32_t bar) {
     asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
@@ -272,7 +289,7 @@ inline NsEncodeTiledFn ns_encode_fn() {
     return fn;
 }
 
-// rows x cols matrix of bfloat16 or float with row stride ld (elements); boxes of box_rows x 128 bytes, 128-byte
+// rows x cols matrix of bytes, bfloat16 or float with row stride ld (elements); boxes of box_rows x 128 bytes, 128-byte
 // swizzle, zero fill outside the matrix.  A map depends on the address, the sizes and the box only, never on the
 // contents, and weights and scratch buffers keep their addresses from step to step: every map is encoded once and
 // kept (per host thread and per source file that asks; the table is emptied when it reaches 8,192 entries), so
@@ -295,9 +312,9 @@ struct NsMapKeyHash {
     }
 };
 
-template <int kBytes>  // of an element: 2 (bfloat16) or 4 (float)
+template <int kBytes>  // of an element: 1, 2 (bfloat16) or 4 (float)
 inline int ns_make_map(CUtensorMap* map, const void* ptr, unsigned long long rows, int cols, long long ld, int box_rows, const char* who) {
-    static_assert(kBytes == 2 || kBytes == 4, "bfloat16 or float");
+    static_assert(kBytes == 1 || kBytes == 2 || kBytes == 4, "bytes, bfloat16 or float");
     static thread_local std::unordered_map<NsMapKey, CUtensorMap, NsMapKeyHash> known;
     const NsMapKey key{ptr, rows, ld, cols, box_rows};
     const auto hit = known.find(key);
@@ -313,7 +330,7 @@ inline int ns_make_map(CUtensorMap* map, const void* ptr, unsigned long long row
     const cuuint64_t strides[1] = {(cuuint64_t)ld * kBytes};
     const cuuint32_t box[2] = {128u / kBytes, (cuuint32_t)box_rows};
     const cuuint32_t estr[2] = {1, 1};
-    const CUresult r = fn(map, kBytes == 2 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 2, const_cast<void*>(ptr), dims,
+    const CUresult r = fn(map, kBytes == 1 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : kBytes == 2 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 2, const_cast<void*>(ptr), dims,
                           strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                           CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (r != CUDA_SUCCESS) NS_FAIL(NS_ERR_CUDA, "%s: cuTensorMapEncodeTiled failed with code %d", who, (int)r);

@@ -7,7 +7,7 @@ from dataclasses import dataclass
 
 import torch
 
-from . import _on_current_device, _ptr, _stream, dtype_code, lib
+from . import _on_current_device, _ptr, _stream, _tc, dtype_code, lib, sm_count
 from .lib import KernelError
 
 I8_MAX_K = 131072  # 127 * 127 * K stays within 32 bits
@@ -56,7 +56,26 @@ def quantize_rows(x: torch.Tensor) -> RowsI8:
     return RowsI8(q, scale)
 
 
-def linear_i8(x: torch.Tensor | RowsI8, w: RowsI8, out: torch.Tensor, bias: torch.Tensor | None = None) -> torch.Tensor:
+def i8_tiles(M: int, N: int, K: int, sms: int) -> tuple[int, int, int]:
+    """(tokens of a tile, features of a tile, blocks or pairs that divide k) of the product."""
+    k_blocks = -(-K // 128)
+    if M > 128:
+        tiles = -(-M // 256) * -(-N // 256)
+        splits = 1
+        while splits < 4 and tiles * splits * 2 <= sms // 2 and splits * 2 <= k_blocks:
+            splits *= 2
+        return 256, 256, splits
+    tile = 16 if M <= 16 else 32 if M <= 32 else 64 if M <= 64 else 128
+    tiles = -(-N // 128)
+    resident = sms * (2 if tile <= 64 else 1)
+    splits = 1
+    while splits < 8 and tiles * splits * 2 <= resident and splits * 2 <= k_blocks:
+        splits *= 2
+    return tile, 128, splits
+
+
+def linear_i8(x: torch.Tensor | RowsI8, w: RowsI8, out: torch.Tensor, bias: torch.Tensor | None = None,
+              tiles: tuple[int, int, int] | None = None) -> torch.Tensor:
     """out[n, f] = (sum_k xq[n, k] wq[f, k]) * xs[n] * ws[f] (+ bias[f], float32), the sum exact in 32-bit integers.  `x` [N, K] is quantised by
     rows on the way (`quantize_rows`) unless it comes so, for several products of the same activations; `out` [N, F] is float32 or bfloat16
     with unit inner stride."""
@@ -77,6 +96,7 @@ def linear_i8(x: torch.Tensor | RowsI8, w: RowsI8, out: torch.Tensor, bias: torc
     if N == 0 or F == 0:
         return out
     rows = x if isinstance(x, RowsI8) else quantize_rows(x)
+    sms = sm_count()
     lib.call("ns_gemm_i8", rows.q.data_ptr(), rows.q.stride(0), rows.scale.data_ptr(), w.q.data_ptr(), w.q.stride(0), w.scale.data_ptr(), _ptr(bias),
-             out.data_ptr(), out.stride(0), N, F, K, code, _stream())
+             out.data_ptr(), out.stride(0), N, F, K, code, *(tiles or i8_tiles(N, F, K, sms)), int(rows is not x), sms, _tc(out.device).error.data_ptr(), _stream())
     return out
