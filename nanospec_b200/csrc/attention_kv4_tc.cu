@@ -1,0 +1,440 @@
+// Attention of single tokens, and of a few tokens of a request, over the 4-bit cache (kv4.cuh) in bfloat16 on the tensor cores (m16n8k16).
+//
+// A (query head, token) pair is a column, eight to an n-block: the cached keys and values are the left operands, so that a group of up to
+// eight query heads fills the instruction, and the scores' and the outputs' columns are the same lanes'.
+//   scores^T [keys x columns] = K [keys x features] q^T.  The contracted order is free as long as q has the same: a lane takes a quarter of a
+//     key's features in one load, which lie in one or two groups, and pairs feature p with p + 4 of every word, as the codes lie.
+//   out^T [features x columns] += V^T [features x keys] weights^T.  A lane takes an eighth of four keys' features; the codes of two keys are
+//     brought side by side (two byte permutations for eight features), and the same shift, mask and fma make two values.  The weights turn from
+//     the scores' layout into the right operand's by one 8 x 8 transposition of 16-bit numbers in registers.
+// Rows of the score tile are dealt to keys (key_of_row) such that both sides' reads of shared memory spread over the banks.
+//
+// Every warp is on its own: it takes every (warps of the cluster)-th tile of 32 keys, brings it with bulk copies (a lane each for the codes and
+// pairs of keys and values of a page) into its own ring, and keeps its own maximum, sum and output; the block's warps, then the cluster's blocks are
+// joined at the end in a fixed order.  The running maximum moves only when a score exceeds it by more than 2^8 (weights are then at most 256,
+// far from any limit of float or bfloat16); the common tile costs a vote.
+//
+// The weights meet the values as bfloat16, as in the attention over a bfloat16 cache; sums, maximum and outputs are float.
+#include "kv4.cuh"
+#include "mma_utils.cuh"
+#include "tcgen05_utils.cuh"
+
+namespace {
+
+constexpr int kTile = 32, kWarps = 8, kThreads = 32 * kWarps, kStages = 2;
+constexpr float kLog2e = 1.4426950408889634f, kSlack = 8.f;
+constexpr int kErrKeys = 71;
+
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
+}
+__device__ __forceinline__ uint32_t transpose8(uint32_t x) {
+    uint32_t y;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
+template <int N>
+__device__ __forceinline__ void lds(uint32_t (&v)[N], const unsigned char* p) {
+    if constexpr (N == 1) v[0] = *reinterpret_cast<const uint32_t*>(p);
+    else if constexpr (N == 2) {
+        const uint2 u = *reinterpret_cast<const uint2*>(p);
+        v[0] = u.x; v[1] = u.y;
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; i += 4) {
+            const uint4 u = *reinterpret_cast<const uint4*>(p + 4 * i);
+            v[i] = u.x; v[i + 1] = u.y; v[i + 2] = u.z; v[i + 3] = u.w;
+        }
+    }
+}
+
+template <int D, int NB>
+struct Shape {
+    static constexpr int kCols = 8 * NB, kWords = D / 32, kVWords = D / 64, kBlocks = D / 16;  // words of a lane per key; m-blocks of features
+    static constexpr int kCodes = kTile * D / 2, kPairs = kTile * D / 8, kStage = 2 * (kCodes + kPairs);
+    static constexpr int kRing = kStages * kStage;
+    static_assert(kRing >= kCols * D * 4, "a warp's output is staged where its ring was");
+    static constexpr int kQBytes = NB * kWords * 512;  // q's operands, 16 bytes a lane
+    static constexpr size_t kSmem = (size_t)kWarps * kRing + kQBytes;
+};
+
+// tokens: `items` [n, 2] = (first row, tokens), rows `rows` [n] of one token each, or row blockIdx.z
+template <int D, int NB>
+__global__ void __launch_bounds__(kThreads, D <= 128 ? 2 : 1)
+attention_kv4_tc_kernel(const __nv_bfloat16* __restrict__ q, long long ldq, const uint8_t* __restrict__ k_pages, const uint8_t* __restrict__ v_pages,
+                        const int* __restrict__ block_table, int table_stride, const int* __restrict__ token_req, const int* __restrict__ positions,
+                        const int* __restrict__ rows, const int* __restrict__ items, __nv_bfloat16* __restrict__ out, long long ldo, int nq, int nkv,
+                        int page_size, float scale, int window, const float* __restrict__ sink, int head_tiles, int splits, int* __restrict__ error_flag) {
+    using S = Shape<D, NB>;
+    extern __shared__ __align__(128) unsigned char smem[];
+    __shared__ __align__(8) unsigned long long bars[kWarps][kStages];
+    __shared__ float m_s[kWarps][S::kCols], l_s[kWarps][S::kCols], mb_s[S::kCols], lb_s[S::kCols];
+    const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31, t = lane & 3, r = lane >> 2;
+    unsigned char* ring = smem + warp * S::kRing;
+    uint4* q_s = reinterpret_cast<uint4*>(smem + (size_t)kWarps * S::kRing);
+    const uint32_t bar0 = smem_u32(&bars[warp][0]);
+
+    ns_pdl_launch_dependents();
+    if (lane == 0) {
+        for (int s = 0; s < kStages; ++s) mbar_init(bar0 + 8u * s, 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        fence_async_smem();
+    }
+    __syncwarp();
+    ns_pdl_wait();
+
+    const int z = blockIdx.z;
+    const int n0 = items ? items[2 * z] : rows ? rows[z] : z, count = items ? items[2 * z + 1] : 1;
+    const int req = token_req[n0];
+    if (req < 0) return;  // a row of padding (all blocks of its cluster leave)
+    const int G = nq / nkv, hk = blockIdx.y / head_tiles, ht = blockIdx.y % head_tiles;
+    const int per = min(G, S::kCols), h0 = hk * G + ht * per, heads = min(per, hk * G + G - h0);  // heads of a token here
+    const int cols = count * heads;
+    const int pos0 = positions[n0], end = pos0 + count;  // keys below `end` are seen by some column
+    const int start = window > 0 ? max(0, pos0 - window + 1) : 0;
+    const int tile0 = start / kTile, tiles = (end + kTile - 1) / kTile - tile0;
+    const int* bt = block_table + (size_t)req * table_stride;
+    const int step = splits * kWarps, first = (int)blockIdx.x * kWarps + warp;
+
+    // a tile's pages: a lane for each page and each of (codes, pairs) x (keys, values)
+    const int in_page = min(kTile, page_size), pages = kTile / in_page;
+    const size_t block_bytes = kv4_block_bytes(page_size, D);
+    const int part = lane & 3, which = lane >> 2;
+    const uint32_t part_bytes = (uint32_t)in_page * ((part & 1) ? D / 8 : D / 2);
+    auto request = [&](int i) {  // tile `i` of this request's into stage (its turn) % kStages
+        const int key0 = (tile0 + i) * kTile, stage = ((i - first) / step) % kStages;
+        const uint32_t bar = bar0 + 8u * stage;
+        const int key = key0 + which * in_page;
+        const bool live = which < pages && key < end && key + in_page > start;
+        const unsigned all = __ballot_sync(0xffffffffu, live && part == 0);
+        if (lane == 0) mbar_expect_tx(bar, (uint32_t)__popc(all) * (uint32_t)in_page * (D / 2 + D / 8) * 2u);
+        __syncwarp();
+        if (live) {
+            const uint8_t* from = (part & 2 ? v_pages : k_pages) + ((size_t)bt[key / page_size] * nkv + hk) * block_bytes;
+            const int slot = key % page_size;
+            from += (part & 1) ? (size_t)page_size * (D / 2) + (size_t)slot * (D / 8) : (size_t)slot * (D / 2);
+            const uint32_t to = smem_u32(ring) + stage * S::kStage + (part & 2 ? S::kCodes + S::kPairs : 0) +
+                                (part & 1 ? S::kCodes + which * in_page * (D / 8) : which * in_page * (D / 2));
+            bulk_load(to, from, part_bytes, bar);
+        }
+    };
+#pragma unroll
+    for (int s = 0; s < kStages; ++s)
+        if (first + s * step < tiles) request(first + s * step);
+
+    // q as right operand: column r of each n-block, word w of the lane's quarter: pairs (p, p + 4)
+    for (int i = warp; i < NB * S::kWords; i += kWarps) {
+        const int nb = i / S::kWords, w = i - nb * S::kWords, c = nb * 8 + r;
+        uint32_t v[4] = {0u, 0u, 0u, 0u};
+        if (c < cols) {
+            const __nv_bfloat16* x = q + (size_t)(n0 + c / heads) * ldq + (size_t)(h0 + c % heads) * D + 8 * (t * S::kWords + w);
+#pragma unroll
+            for (int p = 0; p < 4; ++p) {
+                const __nv_bfloat162 two = __halves2bfloat162(x[p], x[p + 4]);
+                v[p] = *reinterpret_cast<const uint32_t*>(&two);
+            }
+        }
+        q_s[i * 32 + lane] = make_uint4(v[0], v[1], v[2], v[3]);
+    }
+    __syncthreads();
+    uint32_t qf[NB == 1 ? S::kWords : 1][4];
+    if constexpr (NB == 1) {
+#pragma unroll
+        for (int w = 0; w < S::kWords; ++w) {
+            const uint4 u = q_s[w * 32 + lane];
+            qf[w][0] = u.x; qf[w][1] = u.y; qf[w][2] = u.z; qf[w][3] = u.w;
+        }
+    }
+    // the last key that each of this lane's columns sees (columns beyond the last: of the last)
+    int limit[NB][2];
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) limit[nb][j] = pos0 + min(nb * 8 + 2 * t + j, cols - 1) / heads;
+
+    float m[NB][2], l[NB][2], o[NB][S::kBlocks][4];
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) {
+#pragma unroll
+        for (int j = 0; j < 2; ++j) { m[nb][j] = -INFINITY; l[nb][j] = 0.f; }
+#pragma unroll
+        for (int b = 0; b < S::kBlocks; ++b)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) o[nb][b][j] = 0.f;
+    }
+    const float sl = scale * kLog2e;
+    const int row_key = (r & 1) ? 4 + ((r >> 1) ^ 1) : r >> 1;  // key of row r (and, 8 further, of row r + 8)
+    int turn = 0;
+    for (int i = first; i < tiles; i += step, ++turn) {
+        const int stage = turn % kStages;
+        if (!mbar_wait_warp(bar0 + 8u * stage, (uint32_t)(turn / kStages) & 1u)) {
+            if (lane == 0) atomicExch(error_flag, kErrKeys);
+            for (int s = 1; s < kStages; ++s)  // copies in flight, again within a limit
+                if (i + s * step < tiles) mbar_wait_warp(bar0 + 8u * ((turn + s) % kStages), (uint32_t)((turn + s) / kStages) & 1u);
+            break;
+        }
+        const unsigned char *kc = ring + stage * S::kStage, *kp = kc + S::kCodes, *vc = kp + S::kPairs, *vp = vc + S::kCodes;
+        const int key0 = (tile0 + i) * kTile;
+        float s[NB][2][4];  // [half of the tile][(row r, columns 2t, 2t + 1), (row r + 8, ...)]
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+            const int ka = half * 16 + row_key;
+            uint32_t ca[S::kWords], cb[S::kWords];
+            lds(ca, kc + ka * (D / 2) + t * (D / 8));
+            lds(cb, kc + (ka + 8) * (D / 2) + t * (D / 8));
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) s[nb][half][j] = 0.f;
+            uint32_t Sa = 0u, Ba = 0u, Sb = 0u, Bb = 0u;
+#pragma unroll
+            for (int w = 0; w < S::kWords; ++w) {
+                if (w % 4 == 0) {  // (a lane's words begin at a group, or lie in one)
+                    const int g = (t * S::kWords + w) / 4;
+                    kv4_pair(*reinterpret_cast<const uint32_t*>(kp + ka * (D / 8) + 4 * g), Sa, Ba);
+                    kv4_pair(*reinterpret_cast<const uint32_t*>(kp + (ka + 8) * (D / 8) + 4 * g), Sb, Bb);
+                }
+                uint32_t va[4], vb[4];
+                kv4_word(ca[w], Sa, Ba, va);
+                kv4_word(cb[w], Sb, Bb, vb);
+                const uint32_t a0[4] = {va[0], vb[0], va[1], vb[1]}, a1[4] = {va[2], vb[2], va[3], vb[3]};
+#pragma unroll
+                for (int nb = 0; nb < NB; ++nb) {
+                    if constexpr (NB == 1) {
+                        ns_mma_bf16(s[nb][half], a0, qf[w][0], qf[w][1]);
+                        ns_mma_bf16(s[nb][half], a1, qf[w][2], qf[w][3]);
+                    } else {
+                        const uint4 u = q_s[(nb * S::kWords + w) * 32 + lane];
+                        ns_mma_bf16(s[nb][half], a0, u.x, u.y);
+                        ns_mma_bf16(s[nb][half], a1, u.z, u.w);
+                    }
+                }
+            }
+        }
+        // scores in base 2; keys that a column does not see
+        const bool whole = key0 >= start && key0 + kTile <= end;                          // every key is there
+        const bool plain = key0 + kTile - 1 <= pos0 && (window <= 0 || key0 > end - 1 - window);  // ... and seen by every column
+        bool over = false;
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+            for (int half = 0; half < 2; ++half)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    float v = s[nb][half][j] * sl;
+                    if (!plain) {
+                        const int key = key0 + half * 16 + row_key + (j & 2 ? 8 : 0), last = limit[nb][j & 1];
+                        if (key > last || (window > 0 && key <= last - window)) v = -INFINITY;
+                    }
+                    s[nb][half][j] = v;
+                    over |= v > m[nb][j & 1] + kSlack;
+                }
+        if (__any_sync(0xffffffffu, over)) {
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    float top = fmaxf(fmaxf(s[nb][0][j], s[nb][0][j + 2]), fmaxf(s[nb][1][j], s[nb][1][j + 2]));
+                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
+                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
+                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
+                    const float now = fmaxf(m[nb][j], top), keep = now == -INFINITY ? 1.f : ns_exp2(m[nb][j] - now);
+                    m[nb][j] = now;
+                    l[nb][j] *= keep;
+#pragma unroll
+                    for (int b = 0; b < S::kBlocks; ++b) { o[nb][b][j] *= keep; o[nb][b][j + 2] *= keep; }
+                }
+        }
+        uint32_t pb[NB][2][2];  // the weights as right operand, [half][keys 2t, 2t + 1; 2t + 8, 2t + 9]
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) {
+            const float m0 = m[nb][0] == -INFINITY ? 0.f : m[nb][0], m1 = m[nb][1] == -INFINITY ? 0.f : m[nb][1];
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                const float p0 = ns_exp2(s[nb][half][0] - m0), p1 = ns_exp2(s[nb][half][1] - m1), p2 = ns_exp2(s[nb][half][2] - m0),
+                            p3 = ns_exp2(s[nb][half][3] - m1);
+                l[nb][0] += p0 + p2;
+                l[nb][1] += p1 + p3;
+                pb[nb][half][0] = transpose8(ns_pack_bf16(p0, p1));
+                pb[nb][half][1] = transpose8(ns_pack_bf16(p2, p3));
+            }
+        }
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+            // keys of rows 2t, 2t + 1, 2t + 8, 2t + 9
+            const int keys[4] = {half * 16 + t, half * 16 + 4 + (t ^ 1), half * 16 + 8 + t, half * 16 + 12 + (t ^ 1)};
+            uint32_t c[4][S::kVWords], pair[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                lds(c[k], vc + keys[k] * (D / 2) + r * (D / 16));
+                pair[k] = *reinterpret_cast<const uint32_t*>(vp + keys[k] * (D / 8) + 4 * (r * S::kVWords / 4));
+                // what is not there (or nobody's yet) counts as zeros: a weight of zero must not meet a NaN
+                if (!whole && (key0 + keys[k] < start || key0 + keys[k] >= end)) pair[k] = 0u;
+            }
+            const uint32_t S01 = __byte_perm(pair[0], pair[1], 0x5410), B01 = __byte_perm(pair[0], pair[1], 0x7632);
+            const uint32_t S89 = __byte_perm(pair[2], pair[3], 0x5410), B89 = __byte_perm(pair[2], pair[3], 0x7632);
+#pragma unroll
+            for (int w = 0; w < S::kVWords; ++w) {
+                // features 0-3 of two keys side by side, then 4-7
+                uint32_t x01[4], y01[4], x89[4], y89[4];
+                kv4_word(__byte_perm(c[0][w], c[1][w], 0x5410), S01, B01, x01);
+                kv4_word(__byte_perm(c[0][w], c[1][w], 0x7632), S01, B01, y01);
+                kv4_word(__byte_perm(c[2][w], c[3][w], 0x5410), S89, B89, x89);
+                kv4_word(__byte_perm(c[2][w], c[3][w], 0x7632), S89, B89, y89);
+#pragma unroll
+                for (int p = 0; p < 4; ++p) {
+                    const uint32_t a[4] = {x01[p], y01[p], x89[p], y89[p]};
+#pragma unroll
+                    for (int nb = 0; nb < NB; ++nb) ns_mma_bf16(o[nb][w * 4 + p], a, pb[nb][half][0], pb[nb][half][1]);
+                }
+            }
+        }
+        __syncwarp();  // every lane has read the tile
+        if (i + kStages * step < tiles) request(i + kStages * step);
+    }
+
+    // ---- the block's warps -----------------------------------------------------------------------------------------------------------
+    float* mine = reinterpret_cast<float*>(ring);  // [column][feature]
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) {
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            l[nb][j] += __shfl_xor_sync(0xffffffffu, l[nb][j], 4);
+            l[nb][j] += __shfl_xor_sync(0xffffffffu, l[nb][j], 8);
+            l[nb][j] += __shfl_xor_sync(0xffffffffu, l[nb][j], 16);
+            if (r == 0) {
+                m_s[warp][nb * 8 + 2 * t + j] = m[nb][j];
+                l_s[warp][nb * 8 + 2 * t + j] = l[nb][j];
+            }
+        }
+#pragma unroll
+        for (int b = 0; b < S::kBlocks; ++b) {
+            const int f = r * (D / 8) + (b / 4) * 8 + (b & 3), c = nb * 8 + 2 * t;
+            mine[c * D + f] = o[nb][b][0];
+            mine[(c + 1) * D + f] = o[nb][b][1];
+            mine[c * D + f + 4] = o[nb][b][2];
+            mine[(c + 1) * D + f + 4] = o[nb][b][3];
+        }
+    }
+    __syncthreads();
+    // a warp's part: 2^(its maximum - the block's); one that saw no key adds nothing, one whose scores are all NaN makes the column NaN
+    auto share = [](float m_part, float l_part, float top) { return m_part == -INFINITY ? 0.f * l_part : ns_exp2(m_part - top); };
+    float* block_o = reinterpret_cast<float*>(smem);  // (warp 0's: every thread reads its own elements before it writes them)
+    for (int e = threadIdx.x; e < cols * D; e += kThreads) {
+        const int c = e / D;
+        float top = -INFINITY, acc = 0.f, sum = 0.f;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) top = fmaxf(top, m_s[w][c]);
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) {
+            const float f = share(m_s[w][c], l_s[w][c], top);
+            acc += f * reinterpret_cast<const float*>(smem + w * S::kRing)[e];
+            sum += f * l_s[w][c];
+        }
+        block_o[e] = acc;
+        if (e % D == 0) { mb_s[c] = top; lb_s[c] = sum; }
+    }
+    __syncthreads();
+    // ---- the cluster's blocks: each writes a share of the outputs ----------------------------------------------------------------------
+    if (splits > 1) cluster_sync();
+    const int total = cols * D / 2, share_n = (total + splits - 1) / splits;
+    for (int e = (int)blockIdx.x * share_n + threadIdx.x; e < min(total, ((int)blockIdx.x + 1) * share_n); e += kThreads) {
+        const int c = 2 * e / D, f = 2 * e - c * D, h = h0 + c % heads;
+        const float sink2 = sink ? sink[h] * kLog2e : -INFINITY;
+        float top = sink2, a0 = 0.f, a1 = 0.f, sum = 0.f;
+        if (splits == 1) {
+            top = fmaxf(top, mb_s[c]);
+            const float w = share(mb_s[c], lb_s[c], top);
+            sum = w * lb_s[c];
+            a0 = w * block_o[2 * e];
+            a1 = w * block_o[2 * e + 1];
+        } else {
+            float ms[16];
+#pragma unroll
+            for (int b = 0; b < 16; ++b)
+                if (b < splits) top = fmaxf(top, ms[b] = ld_cluster_f32(smem_u32(&mb_s[c]), b));
+#pragma unroll
+            for (int b = 0; b < 16; ++b)
+                if (b < splits) {
+                    const float ls = ld_cluster_f32(smem_u32(&lb_s[c]), b), w = share(ms[b], ls, top);
+                    sum += w * ls;
+                    a0 += w * ld_cluster_f32(smem_u32(block_o + 2 * e), b);
+                    a1 += w * ld_cluster_f32(smem_u32(block_o + 2 * e + 1), b);
+                }
+        }
+        if (sink) sum += ns_exp2(sink2 - top);
+        __nv_bfloat16* to = out + (size_t)(n0 + c / heads) * ldo + (size_t)h * D + f;
+        to[0] = __float2bfloat16_rn(a0 / sum);
+        to[1] = __float2bfloat16_rn(a1 / sum);
+    }
+    if (splits > 1) {
+        __syncthreads();
+        cluster_sync();  // nobody's shared memory goes while another block reads it
+    }
+}
+
+template <int D, int NB>
+int launch(const void* q, long long ldq, const void* k, const void* v, const int* table, int table_stride, const int* token_req, const int* positions,
+           const int* rows, const int* items, int n, void* out, long long ldo, int nq, int nkv, int page_size, float scale, int window, const float* sink,
+           int splits, int* error_flag, cudaStream_t stream) {
+    using S = Shape<D, NB>;
+    static std::atomic<unsigned long long> allowed{0}, wide{0};
+    auto* kernel = attention_kv4_tc_kernel<D, NB>;
+    NS_CUDA(ns_allow_smem((const void*)kernel, (int)S::kSmem, allowed));
+    if (splits > 8) {
+        int dev = 0;
+        NS_CUDA(cudaGetDevice(&dev));
+        const unsigned long long bit = dev < 64 ? 1ull << dev : 0ull;
+        if (!(wide.load() & bit)) {
+            NS_CUDA(cudaFuncSetAttribute((const void*)kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+            wide.fetch_or(bit);
+        }
+    }
+    const int head_tiles = (nq / nkv + S::kCols - 1) / S::kCols;
+    if ((long long)nkv * head_tiles > 65535 || n > 65535) NS_FAIL(NS_ERR_UNSUPPORTED, "ns_attention_kv4_tc: %d tokens, %d heads exceed the grid", n, nq);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(splits, nkv * head_tiles, n);
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = S::kSmem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[2];
+    int n_attr = 0;
+    if (ns_take_pdl()) {
+        attr[n_attr].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[n_attr++].val.programmaticStreamSerializationAllowed = 1;
+    }
+    if (splits > 1) {
+        attr[n_attr].id = cudaLaunchAttributeClusterDimension;
+        attr[n_attr].val.clusterDim.x = splits;
+        attr[n_attr].val.clusterDim.y = 1;
+        attr[n_attr++].val.clusterDim.z = 1;
+    }
+    cfg.attrs = attr;
+    cfg.numAttrs = n_attr;
+    (void)cudaLaunchKernelEx(&cfg, kernel, (const __nv_bfloat16*)q, ldq, (const uint8_t*)k, (const uint8_t*)v, table, table_stride, token_req, positions, rows, items,
+                             (__nv_bfloat16*)out, ldo, nq, nkv, page_size, scale, window, sink, head_tiles, splits, error_flag);
+    NS_CHECK_LAUNCH("ns_attention_kv4_tc");
+    return NS_OK;
+}
+
+}  // namespace
+
+// bfloat16 q [tokens, ldq] and out [tokens, ldo]; heads of 64, 128 or 256; pages of 8, 16 or a multiple of 32 tokens.  Which tokens: `items` [n, 2] =
+// (first row, tokens of one request, of which the heads that share a kv head fill at most 8 * n_blocks columns), or one token each: rows [n], or all n.
+// splits: blocks of a cluster that share a request's keys (1, 2, 4, 8 or 16).
+NS_API int ns_attention_kv4_tc(const void* q, long long ldq, const void* k, const void* v, const int* table, int table_stride, const int* token_req,
+                               const int* positions, const int* rows, const int* items, int n, void* out, long long ldo, int nq, int nkv, int D, int page_size,
+                               float scale, int window, const float* sink, int n_blocks, int splits, int* error_flag, cudaStream_t stream) {
+    if (n <= 0) return NS_OK;
+    if (nkv < 1 || nq < 1 || nq % nkv || window < 0 || !(page_size == 8 || page_size == 16 || (page_size > 0 && page_size % 32 == 0)))
+        NS_FAIL(NS_ERR_UNSUPPORTED, "ns_attention_kv4_tc: %d heads over %d, pages of %d, a window of %d", nq, nkv, page_size, window);
+    if (splits < 1 || splits > 16 || (splits & (splits - 1)) || !error_flag || ((uintptr_t)k | (uintptr_t)v) % 16)
+        NS_FAIL(NS_ERR_ARGUMENT, "ns_attention_kv4_tc: %d blocks to a request, pages on 16-byte boundaries", splits);
+#define NS_KV4_CASE(DD, NBB)                                                                                                                           \
+    if (D == DD && n_blocks == NBB)                                                                                                                    \
+        return launch<DD, NBB>(q, ldq, k, v, table, table_stride, token_req, positions, rows, items, n, out, ldo, nq, nkv, page_size, scale, window, \
+                               sink, splits, error_flag, stream);
+    NS_KV4_CASE(64, 1) NS_KV4_CASE(64, 2) NS_KV4_CASE(128, 1) NS_KV4_CASE(128, 2) NS_KV4_CASE(256, 1) NS_KV4_CASE(256, 2)
+#undef NS_KV4_CASE
+    NS_FAIL(NS_ERR_UNSUPPORTED, "ns_attention_kv4_tc: heads of %d, %d n-blocks", D, n_blocks);
+}

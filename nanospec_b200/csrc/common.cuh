@@ -8,6 +8,8 @@
 #include <stdint.h>
 #include <stdio.h>
 
+#include <atomic>
+
 #define NS_API extern "C" __attribute__((visibility("default")))
 
 enum NsDtype { NS_F32 = 0, NS_BF16 = 1 };
@@ -39,6 +41,18 @@ extern thread_local char ns_error_text[512];
         cudaError_t e_ = (call);                                                            \
         if (e_ != cudaSuccess) NS_FAIL(NS_ERR_CUDA, "%s: %s", #call, cudaGetErrorString(e_)); \
     } while (0)
+
+// Lets `kernel` have `bytes` of dynamic shared memory: asked for once on every device (`done`: one bit each, of the kernel's own).
+inline cudaError_t ns_allow_smem(const void* kernel, int bytes, std::atomic<unsigned long long>& done) {
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    const unsigned long long bit = dev < 64 ? 1ull << dev : 0ull;
+    if (done.load(std::memory_order_relaxed) & bit) return cudaSuccess;
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_relaxed);
+    return e;
+}
 
 // ---- element access: everything is computed in float -----------------------------------
 __device__ __forceinline__ float ns_ld(const float* p, size_t i) { return p[i]; }

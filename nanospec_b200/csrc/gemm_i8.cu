@@ -218,7 +218,8 @@ template <int BN, typename OutT>
 int launch(const void* x, long long ldx, const float* xs, const void* w, long long ldw, const float* ws, const float* bias, void* out, long long ldo,
            int M, int N, int K, int splits, int early, int* error_flag, cudaStream_t stream) {
     using C = Cfg<BN>;
-    NS_CUDA(cudaFuncSetAttribute(gemm_i8_narrow_kernel<BN, OutT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)C::kSmemBytes));
+    static std::atomic<unsigned long long> allowed{0};
+    NS_CUDA(ns_allow_smem((const void*)gemm_i8_narrow_kernel<BN, OutT>, (int)C::kSmemBytes, allowed));
     CUtensorMap mw, mx;
     if (const int rc = ns_make_map<1>(&mw, w, N, K, ldw, BM, "ns_gemm_i8")) return rc;
     if (const int rc = ns_make_map<1>(&mx, x, M, K, ldx, BN, "ns_gemm_i8")) return rc;
@@ -497,7 +498,8 @@ gemm_i8_wide_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
 template <typename OutT>
 int launch(const void* x, long long ldx, const float* xs, const void* w, long long ldw, const float* ws, const float* bias, void* out, long long ldo,
            int M, int N, int K, int tile_n, int splits, int sms, int* error_flag, cudaStream_t stream) {
-    NS_CUDA(cudaFuncSetAttribute(gemm_i8_wide_kernel<OutT>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem));
+    static std::atomic<unsigned long long> allowed{0};
+    NS_CUDA(ns_allow_smem((const void*)gemm_i8_wide_kernel<OutT>, kSmem, allowed));
     CUtensorMap mx, mw;
     if (const int rc = ns_make_map<1>(&mx, x, M, K, ldx, BM, "ns_gemm_i8")) return rc;
     if (const int rc = ns_make_map<1>(&mw, w, N, K, ldw, tile_n / 2, "ns_gemm_i8")) return rc;
@@ -552,4 +554,17 @@ NS_API int ns_gemm_i8(const void* x, long long ldx, const float* xs, const void*
     }
 #undef NS_I8_NARROW
     NS_FAIL(NS_ERR_ARGUMENT, "ns_gemm_i8: tiles of %d tokens", tile);
+}
+
+extern "C" int ns_quantize_rows(const void* x, long long ldx, void* q, long long ldq, float* scale, int rows, int K, int dtype, cudaStream_t stream);
+
+// The product of x [M, ldx] in `x_dtype`, quantised by rows on the way: `scratch`, on a 16-byte boundary, holds M rows of K bytes rounded up to 16 and M floats.
+NS_API int ns_linear_i8(const void* x, long long ldx, int x_dtype, void* scratch, const void* w, long long ldw, const float* ws, const float* bias, void* out,
+                        long long ldo, int M, int N, int K, int dtype, int tile, int features, int splits, int sms, int* error_flag, cudaStream_t stream) {
+    if (M <= 0 || N <= 0) return NS_OK;
+    if (K < 1 || K > 131072) NS_FAIL(NS_ERR_UNSUPPORTED, "ns_linear_i8: K=%d (1 to 131072)", K);
+    const long long ldq = (K + 15) / 16 * 16;
+    float* xs = reinterpret_cast<float*>(static_cast<char*>(scratch) + (size_t)M * ldq);
+    if (const int rc = ns_quantize_rows(x, ldx, scratch, ldq, xs, M, K, x_dtype, stream)) return rc;
+    return ns_gemm_i8(scratch, ldq, xs, w, ldw, ws, bias, out, ldo, M, N, K, dtype, tile, features, splits, 1, sms, error_flag, stream);
 }

@@ -45,10 +45,17 @@ def _cuda(*tensors: torch.Tensor | None) -> None:
 
 def _on_current_device(*tensors: torch.Tensor | None) -> None:
     """Operands of one launch: all on the current CUDA device, whose current stream the kernels go to."""
-    _cuda(*tensors)
+    dev = None
     for t in tensors:
-        if t is not None and t.device.index != torch.cuda.current_device():
-            raise KernelError(f"an operand lies on {t.device}, the current device is cuda:{torch.cuda.current_device()}")
+        if t is None:
+            continue
+        at = t.get_device()  # (-1: not on a CUDA device)
+        if dev is None:
+            _cuda(t)
+            dev = torch.cuda.current_device()
+        if at != dev:
+            _cuda(t)
+            raise KernelError(f"an operand lies on {t.device}, the current device is cuda:{dev}")
 
 
 def _ptr(t: torch.Tensor | None) -> int | None:
@@ -223,6 +230,7 @@ def check_kernel_errors(device: torch.device | None = None) -> None:
                     43: "routed experts: the epilogue waited for the accumulator", 44: "routed experts: copies in flight did not land",
                     61: "8-bit product: the TMA producer waited for a free stage", 62: "8-bit product: the MMA issuer waited",
                     63: "8-bit product: the epilogue waited for the accumulator", 64: "8-bit product: copies in flight did not land",
+                    71: "attention over the 4-bit cache: a warp waited for its keys",
                     31: "wait probe: nobody arrives at its barrier"}.get(code, "?")
             raise KernelError(f"a kernel gave up waiting on an mbarrier (the limit is two seconds) - {what} (code {code}); "
                               "its output is not valid")

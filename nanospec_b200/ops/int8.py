@@ -3,6 +3,7 @@ their matrix product with an exact integer sum (csrc/quantize_rows.cu, csrc/gemm
 
 from __future__ import annotations
 
+import functools
 from dataclasses import dataclass
 
 import torch
@@ -34,9 +35,10 @@ def _aligned_rows(q: torch.Tensor) -> bool:
 
 
 def _check_rows(r: RowsI8, name: str) -> None:
-    if r.q.dtype != torch.int8 or r.q.dim() != 2 or r.scale.dtype != torch.float32 or r.scale.shape != (r.q.shape[0],) or not r.scale.is_contiguous():
+    q, scale = r.q, r.scale
+    if q.dtype != torch.int8 or q.dim() != 2 or scale.dtype != torch.float32 or scale.shape != q.shape[:1] or not scale.is_contiguous():
         raise KernelError(f"linear_i8: {name} must be int8 [R, K] with one contiguous float32 scale per row")
-    if r.q.shape[0] and not _aligned_rows(r.q):
+    if q.shape[0] and not _aligned_rows(q):
         raise KernelError(f"linear_i8: the rows of {name} must start on 16-byte boundaries with unit inner stride (quantize_rows makes them so)")
 
 
@@ -56,6 +58,7 @@ def quantize_rows(x: torch.Tensor) -> RowsI8:
     return RowsI8(q, scale)
 
 
+@functools.lru_cache(maxsize=4096)
 def i8_tiles(M: int, N: int, K: int, sms: int) -> tuple[int, int, int]:
     """(tokens of a tile, features of a tile, blocks or pairs that divide k) of the product."""
     k_blocks = -(-K // 128)
@@ -79,24 +82,26 @@ def linear_i8(x: torch.Tensor | RowsI8, w: RowsI8, out: torch.Tensor, bias: torc
     """out[n, f] = (sum_k xq[n, k] wq[f, k]) * xs[n] * ws[f] (+ bias[f], float32), the sum exact in 32-bit integers.  `x` [N, K] is quantised by
     rows on the way (`quantize_rows`) unless it comes so, for several products of the same activations; `out` [N, F] is float32 or bfloat16
     with unit inner stride."""
-    held = x.q if isinstance(x, RowsI8) else x
-    _on_current_device(held, w.q, w.scale, out, bias)
+    ready = isinstance(x, RowsI8)
+    held, wq = x.q if ready else x, w.q
+    _on_current_device(held, wq, w.scale, out, bias, x.scale if ready else None)
     _check_rows(w, "w")
-    N, (F, K) = held.shape[0], w.q.shape
-    if held.dim() != 2 or held.shape[1] != K or not 1 <= K <= I8_MAX_K:
-        raise KernelError(f"linear_i8: x {tuple(held.shape)} and w {tuple(w.q.shape)} do not agree, or K is beyond {I8_MAX_K}")
-    if out.shape != (N, F) or (F and out.stride(1) != 1):
+    if ready:
+        _check_rows(x, "x")
+    N, (F, K) = held.shape[0], wq.shape
+    if held.dim() != 2 or held.shape[1] != K or not 1 <= K <= I8_MAX_K or (N and held.stride(1) != 1):
+        raise KernelError(f"linear_i8: x {tuple(held.shape)} with unit inner stride and w {tuple(wq.shape)} must agree on K, which is {I8_MAX_K} at most")
+    if out.shape != (N, F) or (N and F and out.stride(1) != 1):
         raise KernelError(f"linear_i8: out must be [{N}, {F}] with unit inner stride, not {tuple(out.shape)} with strides {out.stride()}")
     if bias is not None and (bias.dtype != torch.float32 or bias.shape != (F,) or not bias.is_contiguous()):
         raise KernelError("linear_i8: the bias is one contiguous float32 number per output feature")
-    code = dtype_code(out.dtype)
-    if isinstance(x, RowsI8):
-        _check_rows(x, "x")
-        _on_current_device(x.scale)
-    if N == 0 or F == 0:
-        return out
-    rows = x if isinstance(x, RowsI8) else quantize_rows(x)
-    sms = sm_count()
-    lib.call("ns_gemm_i8", rows.q.data_ptr(), rows.q.stride(0), rows.scale.data_ptr(), w.q.data_ptr(), w.q.stride(0), w.scale.data_ptr(), _ptr(bias),
-             out.data_ptr(), out.stride(0), N, F, K, code, *(tiles or i8_tiles(N, F, K, sms)), int(rows is not x), sms, _tc(out.device).error.data_ptr(), _stream())
+    code, sms = dtype_code(out.dtype), sm_count()
+    tiles = tiles or i8_tiles(N, F, K, sms)
+    if ready:
+        lib.call("ns_gemm_i8", held.data_ptr(), held.stride(0), x.scale.data_ptr(), wq.data_ptr(), wq.stride(0), w.scale.data_ptr(), _ptr(bias),
+                 out.data_ptr(), out.stride(0), N, F, K, code, *tiles, 0, sms, _tc(out.device).error.data_ptr(), _stream())
+    else:
+        scratch = torch.empty(N * (-(-K // 16) * 16 + 4), dtype=torch.int8, device=out.device)
+        lib.call("ns_linear_i8", held.data_ptr(), held.stride(0), dtype_code(held.dtype), scratch.data_ptr(), wq.data_ptr(), wq.stride(0),
+                 w.scale.data_ptr(), _ptr(bias), out.data_ptr(), out.stride(0), N, F, K, code, *tiles, sms, _tc(out.device).error.data_ptr(), _stream())
     return out

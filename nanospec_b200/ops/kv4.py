@@ -7,7 +7,7 @@ import math
 
 import torch
 
-from . import _i32, _on_current_device, _ptr, _stream, dtype_code, lib, sm_count
+from . import _i32, _on_current_device, _ptr, _stream, _tc, dtype_code, lib, sm_count
 from .lib import KernelError
 
 KV4_GROUP = 32  # features that share a pair of numbers
@@ -31,7 +31,8 @@ def _check_lane(who: str, lane, nkv: int, head_dim: int) -> None:
     for t in (lane.k, lane.v):
         if t is None or t.dtype != torch.uint8 or t.dim() != 3 or t.shape[1:] != (nkv, size) or not t.is_contiguous() or t.data_ptr() % 16:
             raise KernelError(f"{who}: the lane's pages must be contiguous uint8 [pages, {nkv}, {size}] on 16-byte boundaries (kv4_pages makes them)")
-    if lane.block_table is None or lane.block_table.dtype != torch.int32 or lane.block_table.dim() != 2 or lane.block_table.stride(1) != 1:
+    table = lane.block_table
+    if table is None or table.dtype != torch.int32 or table.dim() != 2 or table.stride(1) != 1:
         raise KernelError(f"{who}: block_table must be int32 [requests, pages] with unit inner stride")
 
 
@@ -75,17 +76,75 @@ def kv4_read(lane, positions: torch.Tensor, token_req: torch.Tensor, nkv: int, h
     _check_lane("kv4_read", lane, nkv, head_dim)
     n = positions.numel()
     _check_step("kv4_read", positions, token_req, n)
-    k, v = (torch.empty((n, nkv, head_dim), dtype=torch.bfloat16, device=lane.k.device) for _ in range(2))
+    k, v = torch.empty((2, n, nkv, head_dim), dtype=torch.bfloat16, device=lane.k.device).unbind(0)
     lib.call("ns_kv4_read", lane.k.data_ptr(), lane.v.data_ptr(), positions.data_ptr(), token_req.data_ptr(), lane.block_table.data_ptr(),
              lane.block_table.stride(0), k.data_ptr(), v.data_ptr(), n, lane.page_size, nkv, head_dim, sm_count(), _stream())
     return k, v
+
+
+KV4_WARPS, KV4_TILE = 8, 32  # of a block of csrc/attention_kv4_tc.cu, and keys that a warp takes at a time
+
+
+def kv4_tensor_core_ok(dtype: torch.dtype, head_dim: int, page_size: int) -> bool:
+    return dtype == torch.bfloat16 and head_dim in (64, 128, 256) and (page_size in (8, 16) or page_size % 32 == 0)
+
+
+def kv4_splits(blocks: int, longest: int | None, sms: int) -> int:
+    """Blocks of a cluster that share a request's keys: a power of two up to 16 that keeps the grid within two blocks an SM and, when the longest
+    context is known, a tile of keys to every warp."""
+    splits = 1
+    while splits < 16 and blocks * splits * 2 <= 2 * sms and (longest is None or longest > KV4_TILE * KV4_WARPS * splits):
+        splits *= 2
+    return splits
+
+
+def kv4_token_tiles(q_lens: list[int], group: int, most: int) -> tuple[list[tuple[int, int]], int]:
+    """(first row, tokens) of the tiles of every request that brings 2 to `most` tokens, and the n-blocks of 8 columns that they need: a column is a (query
+    head, token) pair, 16 at most to a tile."""
+    longest = max((n for n in q_lens if 2 <= n <= most), default=0)
+    blocks = 1 if longest * group <= 8 else 2
+    per = max(1, 8 * blocks // group)
+    tiles, row = [], 0
+    for n in q_lens:
+        if 2 <= n <= most:
+            tiles += [(row + at, min(per, n - at)) for at in range(0, n, per)]
+        row += n
+    return tiles, blocks
+
+
+def _kv4_plan(ctx, group: int) -> dict:
+    """Once per step and group size: which rows bring one token, and the tiles of the others."""
+    key = ("kv4_plan", group)
+    plan = ctx.extras.get(key)
+    if plan is not None:
+        return plan
+    if ctx.extras.get("graph"):  # every row is a request's one token, and lengths are the device's
+        plan = {"rows": None, "n_rows": None, "longest": None, "tiles": None, "longest_tiles": None}
+    else:
+        if sum(ctx.q_lens) > ctx.positions.numel():
+            raise KernelError(f"attention_kv4: the requests bring {sum(ctx.q_lens)} tokens, the step holds {ctx.positions.numel()}")
+        starts, row = [], 0
+        for n in ctx.q_lens:
+            starts.append(row)
+            row += n
+        rows = [s for s, n in zip(starts, ctx.q_lens) if n == 1]
+        tiles, blocks = kv4_token_tiles(ctx.q_lens, group, 1 << 30)
+        on_device = lambda v: torch.tensor(v, dtype=torch.int32).to(ctx.device, non_blocking=True) if v else None  # noqa: E731
+        plan = {"rows": None if len(rows) == ctx.positions.numel() else on_device(rows), "n_rows": len(rows),
+                "longest": max((kv for kv, n in zip(ctx.kv_lens, ctx.q_lens) if n == 1), default=0),
+                "tiles": on_device(tiles), "n_blocks": blocks, "longest_tiles": max((kv for kv, n in zip(ctx.kv_lens, ctx.q_lens) if n > 1), default=0)}
+    ctx.extras[key] = plan
+    return plan
 
 
 def attention_kv4(qkv: torch.Tensor, lane, ctx, out: torch.Tensor, nq: int, nkv: int, head_dim: int, scale: float | None = None, window: int = 0,
                   sink: torch.Tensor | None = None) -> torch.Tensor:
     """Attention of the step's queries (the first nq * head_dim columns of `qkv`, rotated) over a lane in 4 bits: every token sees the positions
     up to its own (with `window` the last so many of them), which `kv4_store` has filled.  `sink` (float32 [nq]): the softmax's denominator also
-    holds exp(sink[h]).  `scale` is head_dim ** -0.5 when None.  float32 and bfloat16; rows of padding (token_req < 0) are left as they are."""
+    holds exp(sink[h]).  `scale` is head_dim ** -0.5 when None.  float32 and bfloat16; rows of padding (token_req < 0) are left as they are.
+
+    bfloat16 with heads of 64, 128 or 256 and pages of 8, 16 or a multiple of 32 tokens: the tensor cores, softmax weights in bfloat16
+    (csrc/attention_kv4_tc.cu).  Everything else, float32 above all: float throughout (csrc/attention_kv4.cu)."""
     _on_current_device(qkv, out, lane.k, lane.v, lane.block_table, ctx.positions, ctx.token_req, sink)
     _check_lane("attention_kv4", lane, nkv, head_dim)
     n = out.shape[0]
@@ -99,7 +158,24 @@ def attention_kv4(qkv: torch.Tensor, lane, ctx, out: torch.Tensor, nq: int, nkv:
     if sink is not None and (sink.dtype != torch.float32 or sink.numel() != nq or not sink.is_contiguous()):
         raise KernelError("attention_kv4: the sink is one contiguous float32 number per query head")
     scale = 1.0 / math.sqrt(head_dim) if scale is None else float(scale)
-    lib.call("ns_attention_kv4", qkv.data_ptr(), qkv.stride(0), lane.k.data_ptr(), lane.v.data_ptr(), lane.block_table.data_ptr(), lane.block_table.stride(0),
-             ctx.token_req.data_ptr(), ctx.positions.data_ptr(), None, n, out.data_ptr(), out.stride(0), nq, nkv, head_dim, lane.page_size, scale, int(window),
-             _ptr(sink), code, _stream())
+    if not kv4_tensor_core_ok(qkv.dtype, head_dim, lane.page_size):
+        lib.call("ns_attention_kv4", qkv.data_ptr(), qkv.stride(0), lane.k.data_ptr(), lane.v.data_ptr(), lane.block_table.data_ptr(),
+                 lane.block_table.stride(0), ctx.token_req.data_ptr(), ctx.positions.data_ptr(), None, n, out.data_ptr(), out.stride(0), nq, nkv,
+                 head_dim, lane.page_size, scale, int(window), _ptr(sink), code, _stream())
+        return out
+    plan, group, sms = _kv4_plan(ctx, nq // nkv), nq // nkv, sm_count()
+
+    def launch(rows, items, count, longest, blocks):
+        if window and longest is not None:
+            longest = min(longest, window + KV4_TILE)
+        splits = kv4_splits(count * nkv * -(-group // (8 * blocks)), longest, sms)
+        lib.call("ns_attention_kv4_tc", qkv.data_ptr(), qkv.stride(0), lane.k.data_ptr(), lane.v.data_ptr(), lane.block_table.data_ptr(),
+                 lane.block_table.stride(0), ctx.token_req.data_ptr(), ctx.positions.data_ptr(), rows, items, count, out.data_ptr(), out.stride(0), nq,
+                 nkv, head_dim, lane.page_size, scale, int(window), _ptr(sink), blocks, splits, _tc(out.device).error.data_ptr(), _stream())
+
+    n_rows = n if plan["n_rows"] is None else plan["n_rows"]
+    if n_rows:
+        launch(_ptr(plan["rows"]), None, n_rows, plan["longest"], 1 if group <= 8 else 2)
+    if plan["tiles"] is not None:
+        launch(None, plan["tiles"].data_ptr(), plan["tiles"].shape[0], plan["longest_tiles"], plan["n_blocks"])
     return out
