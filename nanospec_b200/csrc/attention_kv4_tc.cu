@@ -9,8 +9,8 @@
 //     the scores' layout into the right operand's by one 8 x 8 transposition of 16-bit numbers in registers.
 // Rows of the score tile are dealt to keys (key_of_row) such that both sides' reads of shared memory spread over the banks.
 //
-// Every warp is on its own: it takes every (warps of the cluster)-th tile of 32 keys, brings it with bulk copies (a lane each for the codes and
-// pairs of keys and values of a page) into its own ring, and keeps its own maximum, sum and output; the block's warps, then the cluster's blocks are
+// Every warp is on its own: it takes every (warps of the cluster)-th tile of 32 keys, brings it in 16-byte pieces into its own ring (bulk copies, a lane each for the codes and pairs of a page, took as
+// long as the tile's arithmetic: their addresses are not a warp's but a lane's), and keeps its own maximum, sum and output; the block's warps, then the cluster's blocks are
 // joined at the end in a fixed order.  The running maximum moves only when a score exceeds it by more than 2^8 (weights are then at most 256,
 // far from any limit of float or bfloat16); the common tile costs a vote.
 //
@@ -21,12 +21,11 @@
 
 namespace {
 
-constexpr int kTile = 32, kWarps = 8, kThreads = 32 * kWarps, kStages = 2;
+constexpr int kTile = 32, kStages = 2;
 constexpr float kLog2e = 1.4426950408889634f, kSlack = 8.f;
-constexpr int kErrKeys = 71;
 
-__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
-    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
+__device__ __forceinline__ void copy16(void* to, const void* from) {
+    asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16;" ::"r"(ns_smem_u32(to)), "l"(from) : "memory");
 }
 __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
     uint32_t y;
@@ -48,8 +47,9 @@ __device__ __forceinline__ void lds(uint32_t (&v)[N], const unsigned char* p) {
     }
 }
 
-template <int D, int NB>
+template <int D, int NB, int kWarps>
 struct Shape {
+    static constexpr int kThreads = 32 * kWarps, kResident = D <= 128 ? 16 / kWarps : 8 / kWarps;  // blocks an SM
     static constexpr int kCols = 8 * NB, kWords = D / 32, kVWords = D / 64, kBlocks = D / 16;  // words of a lane per key; m-blocks of features
     static constexpr int kCodes = kTile * D / 2, kPairs = kTile * D / 8, kStage = 2 * (kCodes + kPairs);
     static constexpr int kRing = kStages * kStage;
@@ -59,28 +59,21 @@ struct Shape {
 };
 
 // tokens: `items` [n, 2] = (first row, tokens), rows `rows` [n] of one token each, or row blockIdx.z
-template <int D, int NB>
-__global__ void __launch_bounds__(kThreads, D <= 128 ? 2 : 1)
+template <int D, int NB, int kWarps>
+__global__ void __launch_bounds__(32 * kWarps, Shape<D, NB, kWarps>::kResident)
 attention_kv4_tc_kernel(const __nv_bfloat16* __restrict__ q, long long ldq, const uint8_t* __restrict__ k_pages, const uint8_t* __restrict__ v_pages,
                         const int* __restrict__ block_table, int table_stride, const int* __restrict__ token_req, const int* __restrict__ positions,
                         const int* __restrict__ rows, const int* __restrict__ items, __nv_bfloat16* __restrict__ out, long long ldo, int nq, int nkv,
-                        int page_size, float scale, int window, const float* __restrict__ sink, int head_tiles, int splits, int* __restrict__ error_flag) {
-    using S = Shape<D, NB>;
+                        int page_size, float scale, int window, const float* __restrict__ sink, int head_tiles, int splits, int page_shift) {
+    using S = Shape<D, NB, kWarps>;
+    constexpr int kThreads = S::kThreads;
     extern __shared__ __align__(128) unsigned char smem[];
-    __shared__ __align__(8) unsigned long long bars[kWarps][kStages];
     __shared__ float m_s[kWarps][S::kCols], l_s[kWarps][S::kCols], mb_s[S::kCols], lb_s[S::kCols];
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31, t = lane & 3, r = lane >> 2;
     unsigned char* ring = smem + warp * S::kRing;
     uint4* q_s = reinterpret_cast<uint4*>(smem + (size_t)kWarps * S::kRing);
-    const uint32_t bar0 = smem_u32(&bars[warp][0]);
 
     ns_pdl_launch_dependents();
-    if (lane == 0) {
-        for (int s = 0; s < kStages; ++s) mbar_init(bar0 + 8u * s, 1);
-        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-        fence_async_smem();
-    }
-    __syncwarp();
     ns_pdl_wait();
 
     const int z = blockIdx.z;
@@ -96,31 +89,46 @@ attention_kv4_tc_kernel(const __nv_bfloat16* __restrict__ q, long long ldq, cons
     const int* bt = block_table + (size_t)req * table_stride;
     const int step = splits * kWarps, first = (int)blockIdx.x * kWarps + warp;
 
-    // a tile's pages: a lane for each page and each of (codes, pairs) x (keys, values)
-    const int in_page = min(kTile, page_size), pages = kTile / in_page;
+    // a tile: 16-byte pieces, codes and pairs of keys and of values, from the pages that it lies in (1, 2 or 4)
+    const int page_log = 31 - __clz(min(kTile, page_size)), pages = kTile >> page_log;  // keys of a page in a tile
     const size_t block_bytes = kv4_block_bytes(page_size, D);
-    const int part = lane & 3, which = lane >> 2;
-    const uint32_t part_bytes = (uint32_t)in_page * ((part & 1) ? D / 8 : D / 2);
-    auto request = [&](int i) {  // tile `i` of this request's into stage (its turn) % kStages
-        const int key0 = (tile0 + i) * kTile, stage = ((i - first) / step) % kStages;
-        const uint32_t bar = bar0 + 8u * stage;
-        const int key = key0 + which * in_page;
-        const bool live = which < pages && key < end && key + in_page > start;
-        const unsigned all = __ballot_sync(0xffffffffu, live && part == 0);
-        if (lane == 0) mbar_expect_tx(bar, (uint32_t)__popc(all) * (uint32_t)in_page * (D / 2 + D / 8) * 2u);
-        __syncwarp();
-        if (live) {
-            const uint8_t* from = (part & 2 ? v_pages : k_pages) + ((size_t)bt[key / page_size] * nkv + hk) * block_bytes;
-            const int slot = key % page_size;
-            from += (part & 1) ? (size_t)page_size * (D / 2) + (size_t)slot * (D / 8) : (size_t)slot * (D / 2);
-            const uint32_t to = smem_u32(ring) + stage * S::kStage + (part & 2 ? S::kCodes + S::kPairs : 0) +
-                                (part & 1 ? S::kCodes + which * in_page * (D / 8) : which * in_page * (D / 2));
-            bulk_load(to, from, part_bytes, bar);
+    // the page that lane `which` answers for (the table is read a tile ahead: its latency would stand before every copy)
+    auto page_of = [&](int i) {
+        const int key = (tile0 + i) * kTile + (lane << page_log);
+        return i < tiles && lane < pages && key < end && key + (1 << page_log) > start ? bt[page_shift >= 0 ? key >> page_shift : key / page_size] : -1;
+    };
+    auto request = [&](int i, int page) {  // tile `i` of this request's into stage (its turn) % kStages
+        unsigned char* to = ring + ((i - first) / step) % kStages * S::kStage + lane * 16;
+        const int key0 = (tile0 + i) * kTile, slot0 = page_shift >= 0 ? key0 & (page_size - 1) : key0 % page_size;
+#pragma unroll
+        for (int c = 0; c < (S::kCodes + 511) / 512; ++c) {  // codes
+            const int at = c * 512 + lane * 16, which = at / (D / 2) >> page_log, mine = __shfl_sync(0xffffffffu, page, which);
+            const size_t from = ((size_t)mine * nkv + hk) * block_bytes + (size_t)slot0 * (D / 2) + (at - (which << page_log) * (D / 2));
+            if (mine >= 0) {
+                copy16(to + c * 512, k_pages + from);
+                copy16(to + S::kCodes + S::kPairs + c * 512, v_pages + from);
+            }
+        }
+#pragma unroll
+        for (int c = 0; c < (S::kPairs + 511) / 512; ++c) {
+            const int at = c * 512 + lane * 16, which = at / (D / 8) >> page_log, mine = __shfl_sync(0xffffffffu, page, which & 31);
+            const size_t from = ((size_t)mine * nkv + hk) * block_bytes + (size_t)page_size * (D / 2) + (size_t)slot0 * (D / 8) + (at - (which << page_log) * (D / 8));
+            if (mine >= 0 && at < S::kPairs) {
+                copy16(to + S::kCodes + c * 512, k_pages + from);
+                copy16(to + 2 * S::kCodes + S::kPairs + c * 512, v_pages + from);
+            }
         }
     };
+    {
+        int page[kStages];
 #pragma unroll
-    for (int s = 0; s < kStages; ++s)
-        if (first + s * step < tiles) request(first + s * step);
+        for (int s = 0; s < kStages; ++s) page[s] = page_of(first + s * step);
+#pragma unroll
+        for (int s = 0; s < kStages; ++s) {
+            if (first + s * step < tiles) request(first + s * step, page[s]);
+            ns_cp_async_commit();
+        }
+    }
 
     // q as right operand: column r of each n-block, word w of the lane's quarter: pairs (p, p + 4)
     for (int i = warp; i < NB * S::kWords; i += kWarps) {
@@ -152,11 +160,11 @@ attention_kv4_tc_kernel(const __nv_bfloat16* __restrict__ q, long long ldq, cons
 #pragma unroll
         for (int j = 0; j < 2; ++j) limit[nb][j] = pos0 + min(nb * 8 + 2 * t + j, cols - 1) / heads;
 
-    float m[NB][2], l[NB][2], o[NB][S::kBlocks][4];
+    float m[NB][2], m_use[NB][2], l[NB][2], o[NB][S::kBlocks][4];  // m_use: m, or 0 while that is -infinity
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) {
 #pragma unroll
-        for (int j = 0; j < 2; ++j) { m[nb][j] = -INFINITY; l[nb][j] = 0.f; }
+        for (int j = 0; j < 2; ++j) { m[nb][j] = -INFINITY; m_use[nb][j] = l[nb][j] = 0.f; }
 #pragma unroll
         for (int b = 0; b < S::kBlocks; ++b)
 #pragma unroll
@@ -167,12 +175,9 @@ attention_kv4_tc_kernel(const __nv_bfloat16* __restrict__ q, long long ldq, cons
     int turn = 0;
     for (int i = first; i < tiles; i += step, ++turn) {
         const int stage = turn % kStages;
-        if (!mbar_wait_warp(bar0 + 8u * stage, (uint32_t)(turn / kStages) & 1u)) {
-            if (lane == 0) atomicExch(error_flag, kErrKeys);
-            for (int s = 1; s < kStages; ++s)  // copies in flight, again within a limit
-                if (i + s * step < tiles) mbar_wait_warp(bar0 + 8u * ((turn + s) % kStages), (uint32_t)((turn + s) / kStages) & 1u);
-            break;
-        }
+        const int next_page = page_of(i + kStages * step);
+        ns_cp_async_wait<kStages - 1>();
+        __syncwarp();  // ... of every lane
         const unsigned char *kc = ring + stage * S::kStage, *kp = kc + S::kCodes, *vc = kp + S::kPairs, *vp = vc + S::kCodes;
         const int key0 = (tile0 + i) * kTile;
         float s[NB][2][4];  // [half of the tile][(row r, columns 2t, 2t + 1), (row r + 8, ...)]
@@ -211,24 +216,35 @@ attention_kv4_tc_kernel(const __nv_bfloat16* __restrict__ q, long long ldq, cons
                 }
             }
         }
-        // scores in base 2; keys that a column does not see
+        // scores in base 2, relative to the running maximum; keys that a column does not see
         const bool whole = key0 >= start && key0 + kTile <= end;                          // every key is there
         const bool plain = key0 + kTile - 1 <= pos0 && (window <= 0 || key0 > end - 1 - window);  // ... and seen by every column
-        bool over = false;
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
             for (int half = 0; half < 2; ++half)
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    float v = s[nb][half][j] * sl;
-                    if (!plain) {
-                        const int key = key0 + half * 16 + row_key + (j & 2 ? 8 : 0), last = limit[nb][j & 1];
-                        if (key > last || (window > 0 && key <= last - window)) v = -INFINITY;
-                    }
+                    const float v = s[nb][half][j] * sl - m_use[nb][j & 1];
                     s[nb][half][j] = v;
-                    over |= v > m[nb][j & 1] + kSlack;
                 }
+        if (!plain) {
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+                for (int half = 0; half < 2; ++half)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const int key = key0 + half * 16 + row_key + (j & 2 ? 8 : 0), last = limit[nb][j & 1];
+                        if (key > last || (window > 0 && key <= last - window)) s[nb][half][j] = -INFINITY;
+                    }
+        }
+        bool over = false;
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+                over |= fmaxf(fmaxf(s[nb][0][j], s[nb][0][j + 2]), fmaxf(s[nb][1][j], s[nb][1][j + 2])) > (m[nb][j] == -INFINITY ? -INFINITY : kSlack);
         if (__any_sync(0xffffffffu, over)) {
 #pragma unroll
             for (int nb = 0; nb < NB; ++nb)
@@ -238,8 +254,13 @@ attention_kv4_tc_kernel(const __nv_bfloat16* __restrict__ q, long long ldq, cons
                     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
                     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
                     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
-                    const float now = fmaxf(m[nb][j], top), keep = now == -INFINITY ? 1.f : ns_exp2(m[nb][j] - now);
+                    // (top is relative to m_use, which is 0 until a key is seen)
+                    const float now = fmaxf(m[nb][j], top + m_use[nb][j]), use = now == -INFINITY ? 0.f : now, keep = ns_exp2(m[nb][j] - use);
+                    const float by = m_use[nb][j] - use;
                     m[nb][j] = now;
+                    m_use[nb][j] = use;
+#pragma unroll
+                    for (int half = 0; half < 2; ++half) { s[nb][half][j] += by; s[nb][half][j + 2] += by; }
                     l[nb][j] *= keep;
 #pragma unroll
                     for (int b = 0; b < S::kBlocks; ++b) { o[nb][b][j] *= keep; o[nb][b][j + 2] *= keep; }
@@ -248,11 +269,9 @@ attention_kv4_tc_kernel(const __nv_bfloat16* __restrict__ q, long long ldq, cons
         uint32_t pb[NB][2][2];  // the weights as right operand, [half][keys 2t, 2t + 1; 2t + 8, 2t + 9]
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) {
-            const float m0 = m[nb][0] == -INFINITY ? 0.f : m[nb][0], m1 = m[nb][1] == -INFINITY ? 0.f : m[nb][1];
 #pragma unroll
             for (int half = 0; half < 2; ++half) {
-                const float p0 = ns_exp2(s[nb][half][0] - m0), p1 = ns_exp2(s[nb][half][1] - m1), p2 = ns_exp2(s[nb][half][2] - m0),
-                            p3 = ns_exp2(s[nb][half][3] - m1);
+                const float p0 = ns_exp2(s[nb][half][0]), p1 = ns_exp2(s[nb][half][1]), p2 = ns_exp2(s[nb][half][2]), p3 = ns_exp2(s[nb][half][3]);
                 l[nb][0] += p0 + p2;
                 l[nb][1] += p1 + p3;
                 pb[nb][half][0] = transpose8(ns_pack_bf16(p0, p1));
@@ -268,8 +287,11 @@ attention_kv4_tc_kernel(const __nv_bfloat16* __restrict__ q, long long ldq, cons
             for (int k = 0; k < 4; ++k) {
                 lds(c[k], vc + keys[k] * (D / 2) + r * (D / 16));
                 pair[k] = *reinterpret_cast<const uint32_t*>(vp + keys[k] * (D / 8) + 4 * (r * S::kVWords / 4));
-                // what is not there (or nobody's yet) counts as zeros: a weight of zero must not meet a NaN
-                if (!whole && (key0 + keys[k] < start || key0 + keys[k] >= end)) pair[k] = 0u;
+            }
+            if (!whole) {  // what is not there (or nobody's yet) counts as zeros: a weight of zero must not meet a NaN
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                    if (key0 + keys[k] < start || key0 + keys[k] >= end) pair[k] = 0u;
             }
             const uint32_t S01 = __byte_perm(pair[0], pair[1], 0x5410), B01 = __byte_perm(pair[0], pair[1], 0x7632);
             const uint32_t S89 = __byte_perm(pair[2], pair[3], 0x5410), B89 = __byte_perm(pair[2], pair[3], 0x7632);
@@ -290,8 +312,10 @@ attention_kv4_tc_kernel(const __nv_bfloat16* __restrict__ q, long long ldq, cons
             }
         }
         __syncwarp();  // every lane has read the tile
-        if (i + kStages * step < tiles) request(i + kStages * step);
+        if (i + kStages * step < tiles) request(i + kStages * step, next_page);
+        ns_cp_async_commit();
     }
+    ns_cp_async_wait<0>();
 
     // ---- the block's warps -----------------------------------------------------------------------------------------------------------
     float* mine = reinterpret_cast<float*>(ring);  // [column][feature]
@@ -373,13 +397,13 @@ attention_kv4_tc_kernel(const __nv_bfloat16* __restrict__ q, long long ldq, cons
     }
 }
 
-template <int D, int NB>
+template <int D, int NB, int kWarps>
 int launch(const void* q, long long ldq, const void* k, const void* v, const int* table, int table_stride, const int* token_req, const int* positions,
            const int* rows, const int* items, int n, void* out, long long ldo, int nq, int nkv, int page_size, float scale, int window, const float* sink,
-           int splits, int* error_flag, cudaStream_t stream) {
-    using S = Shape<D, NB>;
+           int splits, cudaStream_t stream) {
+    using S = Shape<D, NB, kWarps>;
     static std::atomic<unsigned long long> allowed{0}, wide{0};
-    auto* kernel = attention_kv4_tc_kernel<D, NB>;
+    auto* kernel = attention_kv4_tc_kernel<D, NB, kWarps>;
     NS_CUDA(ns_allow_smem((const void*)kernel, (int)S::kSmem, allowed));
     if (splits > 8) {
         int dev = 0;
@@ -394,7 +418,7 @@ int launch(const void* q, long long ldq, const void* k, const void* v, const int
     if ((long long)nkv * head_tiles > 65535 || n > 65535) NS_FAIL(NS_ERR_UNSUPPORTED, "ns_attention_kv4_tc: %d tokens, %d heads exceed the grid", n, nq);
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(splits, nkv * head_tiles, n);
-    cfg.blockDim = dim3(kThreads);
+    cfg.blockDim = dim3(S::kThreads);
     cfg.dynamicSmemBytes = S::kSmem;
     cfg.stream = stream;
     cudaLaunchAttribute attr[2];
@@ -412,7 +436,8 @@ int launch(const void* q, long long ldq, const void* k, const void* v, const int
     cfg.attrs = attr;
     cfg.numAttrs = n_attr;
     (void)cudaLaunchKernelEx(&cfg, kernel, (const __nv_bfloat16*)q, ldq, (const uint8_t*)k, (const uint8_t*)v, table, table_stride, token_req, positions, rows, items,
-                             (__nv_bfloat16*)out, ldo, nq, nkv, page_size, scale, window, sink, head_tiles, splits, error_flag);
+                             (__nv_bfloat16*)out, ldo, nq, nkv, page_size, scale, window, sink, head_tiles, splits,
+                             (page_size & (page_size - 1)) == 0 ? 31 - __builtin_clz(page_size) : -1);
     NS_CHECK_LAUNCH("ns_attention_kv4_tc");
     return NS_OK;
 }
@@ -424,17 +449,18 @@ int launch(const void* q, long long ldq, const void* k, const void* v, const int
 // splits: blocks of a cluster that share a request's keys (1, 2, 4, 8 or 16).
 NS_API int ns_attention_kv4_tc(const void* q, long long ldq, const void* k, const void* v, const int* table, int table_stride, const int* token_req,
                                const int* positions, const int* rows, const int* items, int n, void* out, long long ldo, int nq, int nkv, int D, int page_size,
-                               float scale, int window, const float* sink, int n_blocks, int splits, int* error_flag, cudaStream_t stream) {
+                               float scale, int window, const float* sink, int n_blocks, int warps, int splits, cudaStream_t stream) {
     if (n <= 0) return NS_OK;
     if (nkv < 1 || nq < 1 || nq % nkv || window < 0 || !(page_size == 8 || page_size == 16 || (page_size > 0 && page_size % 32 == 0)))
         NS_FAIL(NS_ERR_UNSUPPORTED, "ns_attention_kv4_tc: %d heads over %d, pages of %d, a window of %d", nq, nkv, page_size, window);
-    if (splits < 1 || splits > 16 || (splits & (splits - 1)) || !error_flag || ((uintptr_t)k | (uintptr_t)v) % 16)
+    if (splits < 1 || splits > 16 || (splits & (splits - 1)) || ((uintptr_t)k | (uintptr_t)v) % 16)
         NS_FAIL(NS_ERR_ARGUMENT, "ns_attention_kv4_tc: %d blocks to a request, pages on 16-byte boundaries", splits);
-#define NS_KV4_CASE(DD, NBB)                                                                                                                           \
-    if (D == DD && n_blocks == NBB)                                                                                                                    \
-        return launch<DD, NBB>(q, ldq, k, v, table, table_stride, token_req, positions, rows, items, n, out, ldo, nq, nkv, page_size, scale, window, \
-                               sink, splits, error_flag, stream);
-    NS_KV4_CASE(64, 1) NS_KV4_CASE(64, 2) NS_KV4_CASE(128, 1) NS_KV4_CASE(128, 2) NS_KV4_CASE(256, 1) NS_KV4_CASE(256, 2)
+#define NS_KV4_CASE(DD, NBB, WW)                                                                                                                        \
+    if (D == DD && n_blocks == NBB && warps == WW)                                                                                                     \
+        return launch<DD, NBB, WW>(q, ldq, k, v, table, table_stride, token_req, positions, rows, items, n, out, ldo, nq, nkv, page_size, scale,     \
+                                   window, sink, splits, stream);
+    NS_KV4_CASE(64, 1, 4) NS_KV4_CASE(64, 2, 4) NS_KV4_CASE(128, 1, 4) NS_KV4_CASE(128, 2, 4) NS_KV4_CASE(256, 1, 4) NS_KV4_CASE(256, 2, 4)
+    NS_KV4_CASE(64, 1, 8) NS_KV4_CASE(64, 2, 8) NS_KV4_CASE(128, 1, 8) NS_KV4_CASE(128, 2, 8) NS_KV4_CASE(256, 1, 8) NS_KV4_CASE(256, 2, 8)
 #undef NS_KV4_CASE
-    NS_FAIL(NS_ERR_UNSUPPORTED, "ns_attention_kv4_tc: heads of %d, %d n-blocks", D, n_blocks);
+    NS_FAIL(NS_ERR_UNSUPPORTED, "ns_attention_kv4_tc: heads of %d, %d n-blocks, %d warps", D, n_blocks, warps);
 }

@@ -230,7 +230,6 @@ def check_kernel_errors(device: torch.device | None = None) -> None:
                     43: "routed experts: the epilogue waited for the accumulator", 44: "routed experts: copies in flight did not land",
                     61: "8-bit product: the TMA producer waited for a free stage", 62: "8-bit product: the MMA issuer waited",
                     63: "8-bit product: the epilogue waited for the accumulator", 64: "8-bit product: copies in flight did not land",
-                    71: "attention over the 4-bit cache: a warp waited for its keys",
                     31: "wait probe: nobody arrives at its barrier"}.get(code, "?")
             raise KernelError(f"a kernel gave up waiting on an mbarrier (the limit is two seconds) - {what} (code {code}); "
                               "its output is not valid")

@@ -7,7 +7,7 @@ import math
 
 import torch
 
-from . import _i32, _on_current_device, _ptr, _stream, _tc, dtype_code, lib, sm_count
+from . import _i32, _on_current_device, _ptr, _stream, dtype_code, lib, sm_count
 from .lib import KernelError
 
 KV4_GROUP = 32  # features that share a pair of numbers
@@ -82,20 +82,20 @@ def kv4_read(lane, positions: torch.Tensor, token_req: torch.Tensor, nkv: int, h
     return k, v
 
 
-KV4_WARPS, KV4_TILE = 8, 32  # of a block of csrc/attention_kv4_tc.cu, and keys that a warp takes at a time
+KV4_TILE = 32  # keys that a warp of csrc/attention_kv4_tc.cu takes at a time
 
 
 def kv4_tensor_core_ok(dtype: torch.dtype, head_dim: int, page_size: int) -> bool:
     return dtype == torch.bfloat16 and head_dim in (64, 128, 256) and (page_size in (8, 16) or page_size % 32 == 0)
 
 
-def kv4_splits(blocks: int, longest: int | None, sms: int) -> int:
-    """Blocks of a cluster that share a request's keys: a power of two up to 16 that keeps the grid within two blocks an SM and, when the longest
-    context is known, a tile of keys to every warp."""
+def kv4_shape(blocks: int, longest: int | None, sms: int) -> tuple[int, int]:
+    """(warps of a block, blocks of a cluster) that share a request's keys."""
+    warps = 4 if blocks >= 2 * sms else 8
     splits = 1
-    while splits < 16 and blocks * splits * 2 <= 2 * sms and (longest is None or longest > KV4_TILE * KV4_WARPS * splits):
+    while splits < 16 and blocks * splits * 2 <= sms * 16 // warps and (longest is None or longest > KV4_TILE * warps * splits):
         splits *= 2
-    return splits
+    return warps, splits
 
 
 def kv4_token_tiles(q_lens: list[int], group: int, most: int) -> tuple[list[tuple[int, int]], int]:
@@ -127,10 +127,15 @@ def _kv4_plan(ctx, group: int) -> dict:
         for n in ctx.q_lens:
             starts.append(row)
             row += n
-        rows = [s for s, n in zip(starts, ctx.q_lens) if n == 1]
+        # the longest first: blocks are scheduled in this order
+        held = {}
+        for s, n, kv in zip(starts, ctx.q_lens, ctx.kv_lens):
+            held.update((s + i, kv) for i in range(n))
+        rows = sorted((s for s, n in zip(starts, ctx.q_lens) if n == 1), key=lambda row: -held[row])
         tiles, blocks = kv4_token_tiles(ctx.q_lens, group, 1 << 30)
+        tiles.sort(key=lambda tile: -held[tile[0]])
         on_device = lambda v: torch.tensor(v, dtype=torch.int32).to(ctx.device, non_blocking=True) if v else None  # noqa: E731
-        plan = {"rows": None if len(rows) == ctx.positions.numel() else on_device(rows), "n_rows": len(rows),
+        plan = {"rows": None if rows == list(range(ctx.positions.numel())) else on_device(rows), "n_rows": len(rows),
                 "longest": max((kv for kv, n in zip(ctx.kv_lens, ctx.q_lens) if n == 1), default=0),
                 "tiles": on_device(tiles), "n_blocks": blocks, "longest_tiles": max((kv for kv, n in zip(ctx.kv_lens, ctx.q_lens) if n > 1), default=0)}
     ctx.extras[key] = plan
@@ -168,10 +173,10 @@ def attention_kv4(qkv: torch.Tensor, lane, ctx, out: torch.Tensor, nq: int, nkv:
     def launch(rows, items, count, longest, blocks):
         if window and longest is not None:
             longest = min(longest, window + KV4_TILE)
-        splits = kv4_splits(count * nkv * -(-group // (8 * blocks)), longest, sms)
+        warps, splits = kv4_shape(count * nkv * -(-group // (8 * blocks)), longest, sms)
         lib.call("ns_attention_kv4_tc", qkv.data_ptr(), qkv.stride(0), lane.k.data_ptr(), lane.v.data_ptr(), lane.block_table.data_ptr(),
                  lane.block_table.stride(0), ctx.token_req.data_ptr(), ctx.positions.data_ptr(), rows, items, count, out.data_ptr(), out.stride(0), nq,
-                 nkv, head_dim, lane.page_size, scale, int(window), _ptr(sink), blocks, splits, _tc(out.device).error.data_ptr(), _stream())
+                 nkv, head_dim, lane.page_size, scale, int(window), _ptr(sink), blocks, warps, splits, _stream())
 
     n_rows = n if plan["n_rows"] is None else plan["n_rows"]
     if n_rows:
