@@ -49,7 +49,7 @@ __device__ __forceinline__ void lds(uint32_t (&v)[N], const unsigned char* p) {
 
 template <int D, int NB, int kWarps>
 struct Shape {
-    static constexpr int kThreads = 32 * kWarps, kResident = D <= 128 ? 16 / kWarps : 8 / kWarps;  // blocks an SM
+    static constexpr int kThreads = 32 * kWarps, kResident = D > 128 ? 8 / kWarps : NB == 2 && kWarps == 4 ? 3 : 16 / kWarps;  // blocks an SM
     static constexpr int kCols = 8 * NB, kWords = D / 32, kVWords = D / 64, kBlocks = D / 16;  // words of a lane per key; m-blocks of features
     static constexpr int kCodes = kTile * D / 2, kPairs = kTile * D / 8, kStage = 2 * (kCodes + kPairs);
     static constexpr int kRing = kStages * kStage;
@@ -59,7 +59,8 @@ struct Shape {
 };
 
 // tokens: `items` [n, 2] = (first row, tokens), rows `rows` [n] of one token each, or row blockIdx.z
-template <int D, int NB, int kWarps>
+// kPages: pages of a tile, 1 or 2 (whole or half tiles in a page), or 0: by page_size
+template <int D, int NB, int kWarps, int kPages>
 __global__ void __launch_bounds__(32 * kWarps, Shape<D, NB, kWarps>::kResident)
 attention_kv4_tc_kernel(const __nv_bfloat16* __restrict__ q, long long ldq, const uint8_t* __restrict__ k_pages, const uint8_t* __restrict__ v_pages,
                         const int* __restrict__ block_table, int table_stride, const int* __restrict__ token_req, const int* __restrict__ positions,
@@ -78,12 +79,12 @@ attention_kv4_tc_kernel(const __nv_bfloat16* __restrict__ q, long long ldq, cons
 
     const int z = blockIdx.z;
     const int n0 = items ? items[2 * z] : rows ? rows[z] : z, count = items ? items[2 * z + 1] : 1;
-    const int req = token_req[n0];
+    const int req = token_req[n0], pos0 = positions[n0];
     if (req < 0) return;  // a row of padding (all blocks of its cluster leave)
     const int G = nq / nkv, hk = blockIdx.y / head_tiles, ht = blockIdx.y % head_tiles;
     const int per = min(G, S::kCols), h0 = hk * G + ht * per, heads = min(per, hk * G + G - h0);  // heads of a token here
     const int cols = count * heads;
-    const int pos0 = positions[n0], end = pos0 + count;  // keys below `end` are seen by some column
+    const int end = pos0 + count;  // keys below `end` are seen by some column
     const int start = window > 0 ? max(0, pos0 - window + 1) : 0;
     const int tile0 = start / kTile, tiles = (end + kTile - 1) / kTile - tile0;
     const int* bt = block_table + (size_t)req * table_stride;
@@ -91,41 +92,52 @@ attention_kv4_tc_kernel(const __nv_bfloat16* __restrict__ q, long long ldq, cons
 
     // a tile: 16-byte pieces, codes and pairs of keys and of values, from the pages that it lies in (1, 2 or 4)
     const int page_log = 31 - __clz(min(kTile, page_size)), pages = kTile >> page_log;  // keys of a page in a tile
-    const size_t block_bytes = kv4_block_bytes(page_size, D);
-    // the page that lane `which` answers for (the table is read a tile ahead: its latency would stand before every copy)
-    auto page_of = [&](int i) {
-        const int key = (tile0 + i) * kTile + (lane << page_log);
-        return i < tiles && lane < pages && key < end && key + (1 << page_log) > start ? bt[page_shift >= 0 ? key >> page_shift : key / page_size] : -1;
+    const unsigned block_bytes = (unsigned)kv4_block_bytes(page_size, D);
+    // Where the blocks of a tile begin, or -1 (the table is read a tile ahead: its latency would stand before every copy): each lane knows the one or two,
+    // or lane i the i-th of more.
+    constexpr int kKnown = kPages == 2 ? 2 : 1;
+    struct Blocks { long long at[kKnown]; };
+    auto blocks_of = [&](int i) {
+        Blocks b;
+#pragma unroll
+        for (int u = 0; u < kKnown; ++u) {
+            const int which = kPages ? u : lane, key = (tile0 + i) * kTile + (which << page_log);
+            const bool live = i < tiles && which < pages && key < end && key + (1 << page_log) > start;
+            b.at[u] = live ? (long long)((unsigned)(bt[page_shift >= 0 ? key >> page_shift : key / page_size] * nkv + hk) * (unsigned long long)block_bytes) : -1;
+        }
+        return b;
     };
-    auto request = [&](int i, int page) {  // tile `i` of this request's into stage (its turn) % kStages
-        unsigned char* to = ring + ((i - first) / step) % kStages * S::kStage + lane * 16;
-        const int key0 = (tile0 + i) * kTile, slot0 = page_shift >= 0 ? key0 & (page_size - 1) : key0 % page_size;
-#pragma unroll
-        for (int c = 0; c < (S::kCodes + 511) / 512; ++c) {  // codes
-            const int at = c * 512 + lane * 16, which = at / (D / 2) >> page_log, mine = __shfl_sync(0xffffffffu, page, which);
-            const size_t from = ((size_t)mine * nkv + hk) * block_bytes + (size_t)slot0 * (D / 2) + (at - (which << page_log) * (D / 2));
-            if (mine >= 0) {
-                copy16(to + c * 512, k_pages + from);
-                copy16(to + S::kCodes + S::kPairs + c * 512, v_pages + from);
+    auto request = [&](int i, int turn, const Blocks& b) {  // tile `i` of this request's, the warp's turn-th, into stage turn % kStages
+        unsigned char* to = ring + turn % kStages * S::kStage + lane * 16;
+        const int key0 = (tile0 + i) * kTile, slot0 = kPages == 2 ? 0 : page_shift >= 0 ? key0 & (page_size - 1) : key0 % page_size;
+        const uint8_t *kb = k_pages + slot0 * (D / 2) + lane * 16, *vb = v_pages + slot0 * (D / 2) + lane * 16;
+        const int to_pairs = page_size * (D / 2) - slot0 * (D / 2 - D / 8);
+        // (the block of a lane's piece, and how far the piece's page lies behind the tile's beginning)
+        auto copy = [&](int o, int row, unsigned char* k_to, unsigned char* v_to, int skip, bool there) {  // o: the lane's byte among those of `row` bytes a token
+            const int which = o / row >> page_log;
+            long long from;
+            if (kPages == 1) from = b.at[0];
+            else if (kPages == 2) from = which ? b.at[kKnown - 1] : b.at[0];
+            else from = __shfl_sync(0xffffffffu, b.at[0], which & 31);
+            from += skip - (which << page_log) * row;
+            if (there && (kPages == 1 || from >= skip - (which << page_log) * row)) {
+                copy16(k_to, kb + from);
+                copy16(v_to, vb + from);
             }
-        }
+        };
 #pragma unroll
-        for (int c = 0; c < (S::kPairs + 511) / 512; ++c) {
-            const int at = c * 512 + lane * 16, which = at / (D / 8) >> page_log, mine = __shfl_sync(0xffffffffu, page, which & 31);
-            const size_t from = ((size_t)mine * nkv + hk) * block_bytes + (size_t)page_size * (D / 2) + (size_t)slot0 * (D / 8) + (at - (which << page_log) * (D / 8));
-            if (mine >= 0 && at < S::kPairs) {
-                copy16(to + S::kCodes + c * 512, k_pages + from);
-                copy16(to + 2 * S::kCodes + S::kPairs + c * 512, v_pages + from);
-            }
-        }
+        for (int c = 0; c < S::kCodes / 512; ++c) copy(c * 512 + lane * 16, D / 2, to + c * 512, to + S::kCodes + S::kPairs + c * 512, c * 512, true);
+#pragma unroll
+        for (int c = 0; c < (S::kPairs + 511) / 512; ++c)  // (every lane takes part in the exchange, those beyond the pairs copy nothing)
+            copy(c * 512 + lane * 16, D / 8, to + S::kCodes + c * 512, to + 2 * S::kCodes + S::kPairs + c * 512, to_pairs + c * 512, c * 512 + lane * 16 < S::kPairs);
     };
     {
-        int page[kStages];
+        Blocks block[kStages];
 #pragma unroll
-        for (int s = 0; s < kStages; ++s) page[s] = page_of(first + s * step);
+        for (int s = 0; s < kStages; ++s) block[s] = blocks_of(first + s * step);
 #pragma unroll
         for (int s = 0; s < kStages; ++s) {
-            if (first + s * step < tiles) request(first + s * step, page[s]);
+            if (first + s * step < tiles) request(first + s * step, s, block[s]);
             ns_cp_async_commit();
         }
     }
@@ -160,11 +172,11 @@ attention_kv4_tc_kernel(const __nv_bfloat16* __restrict__ q, long long ldq, cons
 #pragma unroll
         for (int j = 0; j < 2; ++j) limit[nb][j] = pos0 + min(nb * 8 + 2 * t + j, cols - 1) / heads;
 
-    float m[NB][2], m_use[NB][2], l[NB][2], o[NB][S::kBlocks][4];  // m_use: m, or 0 while that is -infinity
+    float m_use[NB][2], slack[NB][2], l[NB][2], o[NB][S::kBlocks][4];  // the maximum, or 0 while no key was seen (slack: -infinity then)
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) {
 #pragma unroll
-        for (int j = 0; j < 2; ++j) { m[nb][j] = -INFINITY; m_use[nb][j] = l[nb][j] = 0.f; }
+        for (int j = 0; j < 2; ++j) { slack[nb][j] = -INFINITY; m_use[nb][j] = l[nb][j] = 0.f; }
 #pragma unroll
         for (int b = 0; b < S::kBlocks; ++b)
 #pragma unroll
@@ -175,7 +187,7 @@ attention_kv4_tc_kernel(const __nv_bfloat16* __restrict__ q, long long ldq, cons
     int turn = 0;
     for (int i = first; i < tiles; i += step, ++turn) {
         const int stage = turn % kStages;
-        const int next_page = page_of(i + kStages * step);
+        const Blocks next_block = blocks_of(i + kStages * step);
         ns_cp_async_wait<kStages - 1>();
         __syncwarp();  // ... of every lane
         const unsigned char *kc = ring + stage * S::kStage, *kp = kc + S::kCodes, *vc = kp + S::kPairs, *vp = vc + S::kCodes;
@@ -244,7 +256,7 @@ attention_kv4_tc_kernel(const __nv_bfloat16* __restrict__ q, long long ldq, cons
         for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
             for (int j = 0; j < 2; ++j)
-                over |= fmaxf(fmaxf(s[nb][0][j], s[nb][0][j + 2]), fmaxf(s[nb][1][j], s[nb][1][j + 2])) > (m[nb][j] == -INFINITY ? -INFINITY : kSlack);
+                over |= fmaxf(fmaxf(s[nb][0][j], s[nb][0][j + 2]), fmaxf(s[nb][1][j], s[nb][1][j + 2])) > slack[nb][j];
         if (__any_sync(0xffffffffu, over)) {
 #pragma unroll
             for (int nb = 0; nb < NB; ++nb)
@@ -254,11 +266,11 @@ attention_kv4_tc_kernel(const __nv_bfloat16* __restrict__ q, long long ldq, cons
                     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
                     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
                     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
-                    // (top is relative to m_use, which is 0 until a key is seen)
-                    const float now = fmaxf(m[nb][j], top + m_use[nb][j]), use = now == -INFINITY ? 0.f : now, keep = ns_exp2(m[nb][j] - use);
-                    const float by = m_use[nb][j] - use;
-                    m[nb][j] = now;
-                    m_use[nb][j] = use;
+                    // (relative to the maximum so far: what lies below it does not move it)
+                    const bool none = slack[nb][j] == -INFINITY;
+                    const float by = none ? (top == -INFINITY ? 0.f : -top) : fminf(-top, 0.f), keep = none ? 1.f : ns_exp2(by);
+                    if (top != -INFINITY) slack[nb][j] = kSlack;
+                    m_use[nb][j] -= by;
 #pragma unroll
                     for (int half = 0; half < 2; ++half) { s[nb][half][j] += by; s[nb][half][j + 2] += by; }
                     l[nb][j] *= keep;
@@ -312,7 +324,7 @@ attention_kv4_tc_kernel(const __nv_bfloat16* __restrict__ q, long long ldq, cons
             }
         }
         __syncwarp();  // every lane has read the tile
-        if (i + kStages * step < tiles) request(i + kStages * step, next_page);
+        if (i + kStages * step < tiles) request(i + kStages * step, turn, next_block);
         ns_cp_async_commit();
     }
     ns_cp_async_wait<0>();
@@ -327,7 +339,7 @@ attention_kv4_tc_kernel(const __nv_bfloat16* __restrict__ q, long long ldq, cons
             l[nb][j] += __shfl_xor_sync(0xffffffffu, l[nb][j], 8);
             l[nb][j] += __shfl_xor_sync(0xffffffffu, l[nb][j], 16);
             if (r == 0) {
-                m_s[warp][nb * 8 + 2 * t + j] = m[nb][j];
+                m_s[warp][nb * 8 + 2 * t + j] = slack[nb][j] == -INFINITY ? -INFINITY : m_use[nb][j];
                 l_s[warp][nb * 8 + 2 * t + j] = l[nb][j];
             }
         }
@@ -397,13 +409,13 @@ attention_kv4_tc_kernel(const __nv_bfloat16* __restrict__ q, long long ldq, cons
     }
 }
 
-template <int D, int NB, int kWarps>
+template <int D, int NB, int kWarps, int kPages>
 int launch(const void* q, long long ldq, const void* k, const void* v, const int* table, int table_stride, const int* token_req, const int* positions,
            const int* rows, const int* items, int n, void* out, long long ldo, int nq, int nkv, int page_size, float scale, int window, const float* sink,
            int splits, cudaStream_t stream) {
     using S = Shape<D, NB, kWarps>;
     static std::atomic<unsigned long long> allowed{0}, wide{0};
-    auto* kernel = attention_kv4_tc_kernel<D, NB, kWarps>;
+    auto* kernel = attention_kv4_tc_kernel<D, NB, kWarps, kPages>;
     NS_CUDA(ns_allow_smem((const void*)kernel, (int)S::kSmem, allowed));
     if (splits > 8) {
         int dev = 0;
@@ -457,7 +469,7 @@ NS_API int ns_attention_kv4_tc(const void* q, long long ldq, const void* k, cons
         NS_FAIL(NS_ERR_ARGUMENT, "ns_attention_kv4_tc: %d blocks to a request, pages on 16-byte boundaries", splits);
 #define NS_KV4_CASE(DD, NBB, WW)                                                                                                                        \
     if (D == DD && n_blocks == NBB && warps == WW)                                                                                                     \
-        return launch<DD, NBB, WW>(q, ldq, k, v, table, table_stride, token_req, positions, rows, items, n, out, ldo, nq, nkv, page_size, scale,     \
+        return (page_size == 16 ? launch<DD, NBB, WW, 2> : page_size < 16 ? launch<DD, NBB, WW, 0> : launch<DD, NBB, WW, 1>)(q, ldq, k, v, table, table_stride, token_req, positions, rows, items, n, out, ldo, nq, nkv, page_size, scale,     \
                                    window, sink, splits, stream);
     NS_KV4_CASE(64, 1, 4) NS_KV4_CASE(64, 2, 4) NS_KV4_CASE(128, 1, 4) NS_KV4_CASE(128, 2, 4) NS_KV4_CASE(256, 1, 4) NS_KV4_CASE(256, 2, 4)
     NS_KV4_CASE(64, 1, 8) NS_KV4_CASE(64, 2, 8) NS_KV4_CASE(128, 1, 8) NS_KV4_CASE(128, 2, 8) NS_KV4_CASE(256, 1, 8) NS_KV4_CASE(256, 2, 8)

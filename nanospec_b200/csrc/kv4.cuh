@@ -30,7 +30,9 @@ __device__ __forceinline__ uint32_t kv4_fma(uint32_t w, uint32_t S2, uint32_t B2
 }
 // the eight codes of a word as values: out[p] = features (p, p + 4) of the word
 __device__ __forceinline__ void kv4_word(uint32_t w, uint32_t S2, uint32_t B2, uint32_t (&out)[4]) {
-    out[0] = kv4_fma(w << 3, S2, B2);
+    uint32_t up;  // w << 3, in the multiplier's pipe: the logic pipe, at half of the issue rate, is what bounds a kernel that does little else than unpack
+    asm("mad.lo.u32 %0, %1, 8, 0;" : "=r"(up) : "r"(w));
+    out[0] = kv4_fma(up, S2, B2);
     out[1] = kv4_fma(w >> 1, S2, B2);
     out[2] = kv4_fma(w >> 5, S2, B2);
     out[3] = kv4_fma(w >> 9, S2, B2);
