@@ -190,25 +190,18 @@ kv4_read_kernel(const uint8_t* __restrict__ k_pages, const uint8_t* __restrict__
         const long long th = i / words;
         const int h = (int)(th % nkv), n = (int)(th / nkv);
         const int req = token_req[n];
-        uint32_t k[4] = {0u, 0u, 0u, 0u}, v[4] = {0u, 0u, 0u, 0u};
+        uint4 k = make_uint4(0u, 0u, 0u, 0u), v = k;
         if (req >= 0) {
             const int pos = positions[n], slot = pos % page_size;
             const int page = block_table[(size_t)req * table_stride + pos / page_size];
             const size_t block = ((size_t)page * nkv + h) * kv4_block_bytes(page_size, D);
             const size_t codes = block + ((size_t)slot * words + w) * 4;
             const size_t pair = block + (size_t)page_size * (D / 2) + ((size_t)slot * (D / kGroup) + w / 4) * 4;
-            uint32_t S2, B2;
-            kv4_pair(*reinterpret_cast<const uint32_t*>(k_pages + pair), S2, B2);
-            kv4_word(*reinterpret_cast<const uint32_t*>(k_pages + codes), S2, B2, k);
-            kv4_pair(*reinterpret_cast<const uint32_t*>(v_pages + pair), S2, B2);
-            kv4_word(*reinterpret_cast<const uint32_t*>(v_pages + codes), S2, B2, v);
+            k = kv4_in_order(*reinterpret_cast<const uint32_t*>(k_pages + codes), *reinterpret_cast<const uint32_t*>(k_pages + pair));
+            v = kv4_in_order(*reinterpret_cast<const uint32_t*>(v_pages + codes), *reinterpret_cast<const uint32_t*>(v_pages + pair));
         }
-        // from (0, 4) (1, 5) (2, 6) (3, 7) to features in order
-        auto in_order = [](const uint32_t (&p)[4]) {
-            return make_uint4(__byte_perm(p[0], p[1], 0x5410), __byte_perm(p[2], p[3], 0x5410), __byte_perm(p[0], p[1], 0x7632), __byte_perm(p[2], p[3], 0x7632));
-        };
-        *reinterpret_cast<uint4*>(k_out + i * 8) = in_order(k);
-        *reinterpret_cast<uint4*>(v_out + i * 8) = in_order(v);
+        *reinterpret_cast<uint4*>(k_out + i * 8) = k;
+        *reinterpret_cast<uint4*>(v_out + i * 8) = v;
     }
 }
 
@@ -260,5 +253,58 @@ NS_API int ns_kv4_read(const void* k_pages, const void* v_pages, const int* posi
     NS_LAUNCH(kv4_read_kernel, grid, kThreads, 0, stream, (const uint8_t*)k_pages, (const uint8_t*)v_pages, positions, token_req, block_table, table_stride,
               (__nv_bfloat16*)k_out, (__nv_bfloat16*)v_out, n_tokens, page_size, nkv, D);
     NS_CHECK_LAUNCH("ns_kv4_read");
+    return NS_OK;
+}
+
+// ---- whole portions in bfloat16 -----------------------------------------------------------------------------------------------------
+// 64 tokens of a request and a kv head to a block: what their bytes stand for, as pages of 64 tokens of a bfloat16 cache, [item, head, token, D].  Tokens that the
+// request does not hold (any more) are zeros.  Bound by memory: 5 D / 4 bytes read and 4 D written for a token.
+namespace {
+constexpr int kUnfoldTokens = 64;
+
+__global__ void __launch_bounds__(kThreads)
+kv4_unfold_kernel(const uint8_t* __restrict__ k_pages, const uint8_t* __restrict__ v_pages, const int* __restrict__ block_table, int table_stride,
+                  const int* __restrict__ items, const int* __restrict__ kv_len, __nv_bfloat16* __restrict__ k_out, __nv_bfloat16* __restrict__ v_out,
+                  int page_size, int nkv, int head0, int D) {
+    ns_pdl_wait();
+    ns_pdl_launch_dependents();
+    __shared__ long long base[kUnfoldTokens];  // where a token's block begins, less its slot's codes; -1: not held
+    const int req = items[2 * blockIdx.x], pos0 = items[2 * blockIdx.x + 1] * kUnfoldTokens, words = D / 8;
+    const int h = blockIdx.y, held = kv_len[req];
+    if (threadIdx.x < kUnfoldTokens) {
+        const int pos = pos0 + threadIdx.x;
+        long long at = -1;
+        const int page = pos < held ? block_table[(size_t)req * table_stride + pos / page_size] : -1;
+        if (page >= 0) at = (long long)(((size_t)page * nkv + head0 + h) * kv4_block_bytes(page_size, D));
+        base[threadIdx.x] = at;
+    }
+    __syncthreads();
+    const size_t out0 = ((size_t)blockIdx.x * gridDim.y + h) * kUnfoldTokens * D;
+    for (int i = threadIdx.x; i < kUnfoldTokens * words; i += kThreads) {
+        const int token = i / words, w = i - token * words;
+        const long long at = base[token];
+        uint4 k = make_uint4(0u, 0u, 0u, 0u), v = k;
+        if (at >= 0) {
+            const int slot = (pos0 + token) % page_size;
+            const size_t codes = (size_t)at + ((size_t)slot * words + w) * 4, pair = (size_t)at + (size_t)page_size * (D / 2) + ((size_t)slot * (D / kGroup) + w / 4) * 4;
+            k = kv4_in_order(*reinterpret_cast<const uint32_t*>(k_pages + codes), *reinterpret_cast<const uint32_t*>(k_pages + pair));
+            v = kv4_in_order(*reinterpret_cast<const uint32_t*>(v_pages + codes), *reinterpret_cast<const uint32_t*>(v_pages + pair));
+        }
+        *reinterpret_cast<uint4*>(k_out + out0 + (size_t)i * 8) = k;
+        *reinterpret_cast<uint4*>(v_out + out0 + (size_t)i * 8) = v;
+    }
+}
+}  // namespace
+
+// items [n, 2] = (request, block of 64 positions); k_out, v_out [n, heads, 64, D]: kv heads head0 .. head0 + heads - 1 of nkv.
+NS_API int ns_kv4_unfold(const void* k_pages, const void* v_pages, const int* block_table, int table_stride, const int* items, int n, const int* kv_len,
+                         void* k_out, void* v_out, int page_size, int nkv, int head0, int heads, int D, cudaStream_t stream) {
+    if (n <= 0 || heads <= 0) return NS_OK;
+    int rc = check_geometry("ns_kv4_unfold", D, nkv, page_size);
+    if (rc) return rc;
+    if (head0 < 0 || head0 + heads > nkv || heads > 65535) NS_FAIL(NS_ERR_ARGUMENT, "ns_kv4_unfold: heads %d to %d of %d", head0, head0 + heads, nkv);
+    NS_LAUNCH(kv4_unfold_kernel, dim3(n, heads), kThreads, 0, stream, (const uint8_t*)k_pages, (const uint8_t*)v_pages, block_table, table_stride, items, kv_len,
+              (__nv_bfloat16*)k_out, (__nv_bfloat16*)v_out, page_size, nkv, head0, D);
+    NS_CHECK_LAUNCH("ns_kv4_unfold");
     return NS_OK;
 }

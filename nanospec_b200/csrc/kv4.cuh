@@ -42,6 +42,13 @@ __device__ __forceinline__ void kv4_pair(uint32_t pair, uint32_t& S2, uint32_t& 
     S2 = __byte_perm(pair, pair, 0x1010);
     B2 = __byte_perm(pair, pair, 0x3232);
 }
+// a word's eight values in the features' order
+__device__ __forceinline__ uint4 kv4_in_order(uint32_t w, uint32_t pair) {
+    uint32_t S2, B2, p[4];
+    kv4_pair(pair, S2, B2);
+    kv4_word(w, S2, B2, p);
+    return make_uint4(__byte_perm(p[0], p[1], 0x5410), __byte_perm(p[2], p[3], 0x5410), __byte_perm(p[0], p[1], 0x7632), __byte_perm(p[2], p[3], 0x7632));
+}
 __device__ __forceinline__ float2 kv4_floats(uint32_t v) { return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u)); }
 
 }  // namespace

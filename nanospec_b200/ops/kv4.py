@@ -4,10 +4,11 @@ are then uint8 [pages, kv heads, page_size * head_dim * 5 / 8] (`kv4_pages`); cs
 from __future__ import annotations
 
 import math
+from dataclasses import dataclass
 
 import torch
 
-from . import _i32, _on_current_device, _ptr, _stream, dtype_code, lib, sm_count
+from . import BF16, TILE_Q, TILE_Q_TCGEN05, _i32, _on_current_device, _ptr, _stream, attention_prefill, dtype_code, lib, sm_count
 from .lib import KernelError
 
 KV4_GROUP = 32  # features that share a pair of numbers
@@ -98,48 +99,118 @@ def kv4_shape(blocks: int, longest: int | None, sms: int) -> tuple[int, int]:
     return warps, splits
 
 
-def kv4_token_tiles(q_lens: list[int], group: int, most: int) -> tuple[list[tuple[int, int]], int]:
-    """(first row, tokens) of the tiles of every request that brings 2 to `most` tokens, and the n-blocks of 8 columns that they need: a column is a (query
-    head, token) pair, 16 at most to a tile."""
-    longest = max((n for n in q_lens if 2 <= n <= most), default=0)
-    blocks = 1 if longest * group <= 8 else 2
+def kv4_token_tiles(requests: list[tuple[int, int, int]], group: int) -> tuple[list[tuple[int, int]], int]:
+    """(first row, tokens) of the tiles of requests of (first row, tokens, ...), in their order, and the n-blocks of 8 columns that the tiles need: a column
+    is a (query head, token) pair, 16 at most to a tile."""
+    blocks = 1 if max(n for _, n, *_ in requests) * group <= 8 else 2
     per = max(1, 8 * blocks // group)
-    tiles, row = [], 0
-    for n in q_lens:
-        if 2 <= n <= most:
-            tiles += [(row + at, min(per, n - at)) for at in range(0, n, per)]
-        row += n
-    return tiles, blocks
+    return [(row + at, min(per, n - at)) for row, n, *_ in requests for at in range(0, n, per)], blocks
 
 
-def _kv4_plan(ctx, group: int) -> dict:
-    """Once per step and group size: which rows bring one token, and the tiles of the others."""
-    key = ("kv4_plan", group)
+KV4_UNFOLD_COLUMNS = 64       # portions of more (query head, token) pairs to a kv head than this meet their keys and values in bfloat16
+KV4_UNFOLD_MAX = 1 << 30      # bytes of keys and values in bfloat16 at a time: more requests, or kv heads, go one after another
+KV4_UNFOLD_PAGE = 64          # tokens of a page of theirs
+
+
+def kv4_unfold_pays(tokens: int, group: int) -> bool:
+    """Whether a request's portion is better served by bringing its keys and values into bfloat16 once, for the attention over such a cache."""
+    return tokens * group > KV4_UNFOLD_COLUMNS
+
+
+def kv4_unfold_runs(chunks: list[int], nkv: int, head_dim: int, limit: int) -> list[tuple[int, int, int, int]]:
+    """(first request, requests, first kv head, kv heads) of the runs that keep `chunks` of 64 positions a request within `limit` bytes: whole
+    requests together while they fit, one request's heads in parts where they do not."""
+    one = KV4_UNFOLD_PAGE * head_dim * 4  # of a kv head
+    runs, first, held = [], 0, 0
+    for i, n in enumerate(chunks):
+        if held and (held + n) * nkv * one > limit:
+            runs.append((first, i - first, 0, nkv))
+            first, held = i, 0
+        if n * nkv * one > limit:
+            heads = max(1, min(nkv, limit // (n * one)))
+            runs += [(i, 1, h, min(heads, nkv - h)) for h in range(0, nkv, heads)]
+            first, held = i + 1, 0
+        else:
+            held += n
+    if held:
+        runs.append((first, len(chunks) - first, 0, nkv))
+    return runs
+
+
+def _kv4_plan(ctx, group: int, nkv: int, head_dim: int, window: int, tensor_core: bool, unfold: bool) -> dict:
+    """Once per step and kind of layer: which rows run by themselves, the tiles of a few tokens, and the portions that are unfolded.  `tensor_core`: rows and
+    tiles are those of csrc/attention_kv4_tc.cu; else rows alone, of csrc/attention_kv4.cu."""
+    key = ("kv4_plan", group, nkv, head_dim, window, tensor_core, unfold)
     plan = ctx.extras.get(key)
     if plan is not None:
         return plan
+    total = ctx.positions.numel()
+    on_device = lambda v: torch.tensor(v, dtype=torch.int32).to(ctx.device, non_blocking=True) if v else None  # noqa: E731
     if ctx.extras.get("graph"):  # every row is a request's one token, and lengths are the device's
-        plan = {"rows": None, "n_rows": None, "longest": None, "tiles": None, "longest_tiles": None}
+        plan = {"rows": None, "n_rows": total, "longest": None, "tiles": None, "portions": []}
     else:
-        if sum(ctx.q_lens) > ctx.positions.numel():
-            raise KernelError(f"attention_kv4: the requests bring {sum(ctx.q_lens)} tokens, the step holds {ctx.positions.numel()}")
+        if sum(ctx.q_lens) > total:
+            raise KernelError(f"attention_kv4: the requests bring {sum(ctx.q_lens)} tokens, the step holds {total}")
         starts, row = [], 0
         for n in ctx.q_lens:
             starts.append(row)
             row += n
-        # the longest first: blocks are scheduled in this order
-        held = {}
-        for s, n, kv in zip(starts, ctx.q_lens, ctx.kv_lens):
-            held.update((s + i, kv) for i in range(n))
-        rows = sorted((s for s, n in zip(starts, ctx.q_lens) if n == 1), key=lambda row: -held[row])
-        tiles, blocks = kv4_token_tiles(ctx.q_lens, group, 1 << 30)
-        tiles.sort(key=lambda tile: -held[tile[0]])
-        on_device = lambda v: torch.tensor(v, dtype=torch.int32).to(ctx.device, non_blocking=True) if v else None  # noqa: E731
-        plan = {"rows": None if rows == list(range(ctx.positions.numel())) else on_device(rows), "n_rows": len(rows),
-                "longest": max((kv for kv, n in zip(ctx.kv_lens, ctx.q_lens) if n == 1), default=0),
-                "tiles": on_device(tiles), "n_blocks": blocks, "longest_tiles": max((kv for kv, n in zip(ctx.kv_lens, ctx.q_lens) if n > 1), default=0)}
+        requests = list(zip(starts, ctx.q_lens, ctx.kv_lens))
+        long = [i for i, n in enumerate(ctx.q_lens) if n > 1 and unfold and (kv4_unfold_pays(n, group) or not tensor_core)]
+        rest = [(s, n, kv) for i, (s, n, kv) in enumerate(requests) if i not in set(long)]
+        rest.sort(key=lambda r: -r[2])  # the longest first: blocks are scheduled in this order
+        rows = [s + i for s, n, _ in rest for i in range(n) if n == 1 or not tensor_core]
+        plan = {"rows": None if rows == list(range(total)) else on_device(rows), "n_rows": len(rows),
+                "longest": max((kv for _, n, kv in rest if n == 1 or not tensor_core), default=0), "tiles": None, "portions": []}
+        few = [r for r in rest if r[1] > 1]
+        if tensor_core and few:
+            tiles, blocks = kv4_token_tiles(few, group)
+            plan.update(tiles=on_device(tiles), n_blocks=blocks, longest_tiles=few[0][2])
+        for first, count, head, heads in kv4_unfold_runs([-(-ctx.kv_lens[i] // KV4_UNFOLD_PAGE) - _first_chunk(ctx, i, window) for i in long], nkv, head_dim,
+                                                         KV4_UNFOLD_MAX):
+            plan["portions"].append(_kv4_portion(ctx, long[first: first + count], window, head, heads, on_device))
     ctx.extras[key] = plan
     return plan
+
+
+def _first_chunk(ctx, i: int, window: int) -> int:
+    return max(0, ctx.kv_lens[i] - ctx.q_lens[i] - window + 1) // KV4_UNFOLD_PAGE if window else 0
+
+
+def _kv4_portion(ctx, requests: list[int], window: int, head: int, heads: int, on_device) -> dict:
+    """What the unfolding and the attention of `requests` need: chunks of 64 positions, a block table of theirs, tiles of queries."""
+    items, table = [], [[0] * max(-(-ctx.kv_lens[i] // KV4_UNFOLD_PAGE) for i in requests) for _ in ctx.q_lens]
+    for i in requests:
+        for c in range(_first_chunk(ctx, i, window), -(-ctx.kv_lens[i] // KV4_UNFOLD_PAGE)):
+            table[i][c] = len(items)
+            items.append((i, c))
+
+    def tiles(step):  # those that see the most keys come first: blocks are scheduled in this order
+        found = [(i, at) for i in requests for at in range(0, ctx.q_lens[i], step)]
+        found.sort(key=lambda t: -(ctx.kv_lens[t[0]] - ctx.q_lens[t[0]] + min(t[1] + step, ctx.q_lens[t[0]])))
+        return on_device(found)
+
+    return {"items": on_device(items), "n": len(items), "table": on_device(table), "tiles": tiles(TILE_Q), "tiles_tc": tiles(TILE_Q_TCGEN05), "head": head, "heads": heads}
+
+
+@dataclass
+class _Unfolded:
+    """A lane in bfloat16 that holds what a step's portions see of one in 4 bits."""
+
+    k: torch.Tensor
+    v: torch.Tensor
+    block_table: torch.Tensor
+    page_size: int = KV4_UNFOLD_PAGE
+
+
+def _attend_unfolded(qkv, lane, ctx, out, nkv: int, group: int, head_dim: int, scale: float, window: int, sink, portion: dict) -> None:
+    head, heads, n = portion["head"], portion["heads"], portion["n"]
+    k, v = torch.empty((2, n, heads, KV4_UNFOLD_PAGE, head_dim), dtype=torch.bfloat16, device=out.device).unbind(0)
+    lib.call("ns_kv4_unfold", lane.k.data_ptr(), lane.v.data_ptr(), lane.block_table.data_ptr(), lane.block_table.stride(0), portion["items"].data_ptr(), n,
+             ctx.kv_len.data_ptr(), k.data_ptr(), v.data_ptr(), lane.page_size, nkv, head, heads, head_dim, _stream())
+    at, width = head * group * head_dim, heads * group * head_dim
+    attention_prefill(qkv[:, at: at + width], _Unfolded(k, v, portion["table"]), ctx, out[:, at: at + width], heads * group, heads, head_dim, scale, window,
+                      portion["tiles"], portion["tiles_tc"], sink=None if sink is None else sink[head * group: (head + heads) * group])
 
 
 def attention_kv4(qkv: torch.Tensor, lane, ctx, out: torch.Tensor, nq: int, nkv: int, head_dim: int, scale: float | None = None, window: int = 0,
@@ -148,8 +219,10 @@ def attention_kv4(qkv: torch.Tensor, lane, ctx, out: torch.Tensor, nq: int, nkv:
     up to its own (with `window` the last so many of them), which `kv4_store` has filled.  `sink` (float32 [nq]): the softmax's denominator also
     holds exp(sink[h]).  `scale` is head_dim ** -0.5 when None.  float32 and bfloat16; rows of padding (token_req < 0) are left as they are.
 
-    bfloat16 with heads of 64, 128 or 256 and pages of 8, 16 or a multiple of 32 tokens: the tensor cores, softmax weights in bfloat16
-    (csrc/attention_kv4_tc.cu).  Everything else, float32 above all: float throughout (csrc/attention_kv4.cu)."""
+    bfloat16, softmax weights in bfloat16: single tokens and a few of a request on the tensor cores from the cache's bytes (csrc/attention_kv4_tc.cu: heads
+    of 64, 128 or 256, pages of 8, 16 or a multiple of 32 tokens); longer portions of prompts unfold the keys and values that they see into bfloat16 once
+    and take the attention over such a cache (heads up to 128, rows of q on 16-byte boundaries).  Everything else, float32 above all: float
+    throughout (csrc/attention_kv4.cu)."""
     _on_current_device(qkv, out, lane.k, lane.v, lane.block_table, ctx.positions, ctx.token_req, sink)
     _check_lane("attention_kv4", lane, nkv, head_dim)
     n = out.shape[0]
@@ -163,24 +236,28 @@ def attention_kv4(qkv: torch.Tensor, lane, ctx, out: torch.Tensor, nq: int, nkv:
     if sink is not None and (sink.dtype != torch.float32 or sink.numel() != nq or not sink.is_contiguous()):
         raise KernelError("attention_kv4: the sink is one contiguous float32 number per query head")
     scale = 1.0 / math.sqrt(head_dim) if scale is None else float(scale)
-    if not kv4_tensor_core_ok(qkv.dtype, head_dim, lane.page_size):
+    group, sms, window = nq // nkv, sm_count(), int(window)
+    tensor_core = kv4_tensor_core_ok(qkv.dtype, head_dim, lane.page_size)
+    unfold = code == BF16 and head_dim <= 128 and qkv.stride(0) % 8 == 0 and out.stride(0) % 2 == 0 and qkv.data_ptr() % 16 == 0 and out.data_ptr() % 4 == 0
+    plan = _kv4_plan(ctx, group, nkv, head_dim, window, tensor_core, unfold)
+    if plan["n_rows"] and not tensor_core:
         lib.call("ns_attention_kv4", qkv.data_ptr(), qkv.stride(0), lane.k.data_ptr(), lane.v.data_ptr(), lane.block_table.data_ptr(),
-                 lane.block_table.stride(0), ctx.token_req.data_ptr(), ctx.positions.data_ptr(), None, n, out.data_ptr(), out.stride(0), nq, nkv,
-                 head_dim, lane.page_size, scale, int(window), _ptr(sink), code, _stream())
-        return out
-    plan, group, sms = _kv4_plan(ctx, nq // nkv), nq // nkv, sm_count()
-
-    def launch(rows, items, count, longest, blocks):
-        if window and longest is not None:
-            longest = min(longest, window + KV4_TILE)
-        warps, splits = kv4_shape(count * nkv * -(-group // (8 * blocks)), longest, sms)
-        lib.call("ns_attention_kv4_tc", qkv.data_ptr(), qkv.stride(0), lane.k.data_ptr(), lane.v.data_ptr(), lane.block_table.data_ptr(),
-                 lane.block_table.stride(0), ctx.token_req.data_ptr(), ctx.positions.data_ptr(), rows, items, count, out.data_ptr(), out.stride(0), nq,
-                 nkv, head_dim, lane.page_size, scale, int(window), _ptr(sink), blocks, warps, splits, _stream())
-
-    n_rows = n if plan["n_rows"] is None else plan["n_rows"]
-    if n_rows:
-        launch(_ptr(plan["rows"]), None, n_rows, plan["longest"], 1 if group <= 8 else 2)
+                 lane.block_table.stride(0), ctx.token_req.data_ptr(), ctx.positions.data_ptr(), _ptr(plan["rows"]), plan["n_rows"], out.data_ptr(),
+                 out.stride(0), nq, nkv, head_dim, lane.page_size, scale, window, _ptr(sink), code, _stream())
+    elif plan["n_rows"]:
+        _attend_tokens(qkv, lane, ctx, out, nq, nkv, head_dim, scale, window, sink, sms, plan["rows"], None, plan["n_rows"], plan["longest"], 1 if group <= 8 else 2)
     if plan["tiles"] is not None:
-        launch(None, plan["tiles"].data_ptr(), plan["tiles"].shape[0], plan["longest_tiles"], plan["n_blocks"])
+        _attend_tokens(qkv, lane, ctx, out, nq, nkv, head_dim, scale, window, sink, sms, None, plan["tiles"], plan["tiles"].shape[0], plan["longest_tiles"],
+                       plan["n_blocks"])
+    for portion in plan["portions"]:
+        _attend_unfolded(qkv, lane, ctx, out, nkv, group, head_dim, scale, window, sink, portion)
     return out
+
+
+def _attend_tokens(qkv, lane, ctx, out, nq, nkv, head_dim, scale, window, sink, sms, rows, items, count, longest, blocks) -> None:
+    if window and longest is not None:
+        longest = min(longest, window + KV4_TILE)
+    warps, splits = kv4_shape(count * nkv * -(-(nq // nkv) // (8 * blocks)), longest, sms)
+    lib.call("ns_attention_kv4_tc", qkv.data_ptr(), qkv.stride(0), lane.k.data_ptr(), lane.v.data_ptr(), lane.block_table.data_ptr(),
+             lane.block_table.stride(0), ctx.token_req.data_ptr(), ctx.positions.data_ptr(), _ptr(rows), _ptr(items), count, out.data_ptr(), out.stride(0), nq,
+             nkv, head_dim, lane.page_size, scale, window, _ptr(sink), blocks, warps, splits, _stream())
