@@ -107,14 +107,28 @@ def kv4_token_tiles(requests: list[tuple[int, int, int]], group: int) -> tuple[l
     return [(row + at, min(per, n - at)) for row, n, *_ in requests for at in range(0, n, per)], blocks
 
 
-KV4_UNFOLD_COLUMNS = 64       # portions of more (query head, token) pairs to a kv head than this meet their keys and values in bfloat16
 KV4_UNFOLD_MAX = 1 << 30      # bytes of keys and values in bfloat16 at a time: more requests, or kv heads, go one after another
 KV4_UNFOLD_PAGE = 64          # tokens of a page of theirs
 
 
-def kv4_unfold_pays(tokens: int, group: int) -> bool:
-    """Whether a request's portion is better served by bringing its keys and values into bfloat16 once, for the attention over such a cache."""
-    return tokens * group > KV4_UNFOLD_COLUMNS
+def kv4_unfolded(requests: list[tuple[int, int]], group: int, nkv: int, head_dim: int, window: int, sms: int, tensor_core: bool) -> list[int]:
+    """Which of the requests of (tokens brought, positions held after the step) meet their keys and values in bfloat16, unfolded once for all of the portion's
+    tokens.  From the bytes the keys are unpacked again for every 16 (query head, token) pairs: about 17,000 keys of a head of 128 a us; unfolded they cost 3.3
+    MB a us, and a block of 256 tokens of a head takes 11 ns a key, one block an SM.  Us on a B200, from the bytes / unfolded, heads of 128, 4 to each of
+    8 kv heads: one request on 30,000 positions, 64 tokens 202 / 328, 96 378 / 330; 8 on 3,000, 24 tokens 74 / 104, 48 137 / 104; 32 on 1,000, 32
+    tokens 141 / 152, 48 203 / 154; 8 on 500, 24 tokens 27 / 34, 48 45 / 35.  Without the tensor cores a token goes by itself, 2,000 keys a us."""
+    scale = head_dim / 128
+    cost = []  # (request, from the bytes, unfolding and blocks together, one block)
+    for i, (n, kv) in enumerate(requests):
+        if n < 2:
+            continue
+        seen = min(kv, window + n) if window else kv
+        packed = -(-n * group // 16) * seen * nkv * scale / 17000 if tensor_core else n * -(-group // 8) * seen * nkv * scale / 2000
+        cost.append((i, packed, seen * nkv * head_dim * 4 / 3.3e6 + nkv * group * -(-n // 256) * seen * 0.011 / sms, seen * 0.011))
+    chosen = [c for c in cost if c[1] > c[2]]
+    if not chosen or sum(c[1] for c in chosen) < 10 + max(sum(c[2] for c in chosen), max(c[3] for c in chosen)):
+        return []
+    return [c[0] for c in chosen]
 
 
 def kv4_unfold_runs(chunks: list[int], nkv: int, head_dim: int, limit: int) -> list[tuple[int, int, int, int]]:
@@ -156,7 +170,7 @@ def _kv4_plan(ctx, group: int, nkv: int, head_dim: int, window: int, tensor_core
             starts.append(row)
             row += n
         requests = list(zip(starts, ctx.q_lens, ctx.kv_lens))
-        long = [i for i, n in enumerate(ctx.q_lens) if n > 1 and unfold and (kv4_unfold_pays(n, group) or not tensor_core)]
+        long = kv4_unfolded(list(zip(ctx.q_lens, ctx.kv_lens)), group, nkv, head_dim, window, sm_count(), tensor_core) if unfold else []
         rest = [(s, n, kv) for i, (s, n, kv) in enumerate(requests) if i not in set(long)]
         rest.sort(key=lambda r: -r[2])  # the longest first: blocks are scheduled in this order
         rows = [s + i for s, n, _ in rest for i in range(n) if n == 1 or not tensor_core]
@@ -241,9 +255,15 @@ def attention_kv4(qkv: torch.Tensor, lane, ctx, out: torch.Tensor, nq: int, nkv:
     unfold = code == BF16 and head_dim <= 128 and qkv.stride(0) % 8 == 0 and out.stride(0) % 2 == 0 and qkv.data_ptr() % 16 == 0 and out.data_ptr() % 4 == 0
     plan = _kv4_plan(ctx, group, nkv, head_dim, window, tensor_core, unfold)
     if plan["n_rows"] and not tensor_core:
+        longest, splits = plan["longest"], 1
+        if window and longest is not None:
+            longest = min(longest, window)
+        blocks = plan["n_rows"] * nkv * -(-group // 8)
+        while splits < 8 and blocks * splits * 2 <= 2 * sms and (longest is None or longest > 256 * splits):  # a tile of 32 keys to each of eight warps
+            splits *= 2
         lib.call("ns_attention_kv4", qkv.data_ptr(), qkv.stride(0), lane.k.data_ptr(), lane.v.data_ptr(), lane.block_table.data_ptr(),
                  lane.block_table.stride(0), ctx.token_req.data_ptr(), ctx.positions.data_ptr(), _ptr(plan["rows"]), plan["n_rows"], out.data_ptr(),
-                 out.stride(0), nq, nkv, head_dim, lane.page_size, scale, window, _ptr(sink), code, _stream())
+                 out.stride(0), nq, nkv, head_dim, lane.page_size, scale, window, _ptr(sink), splits, code, _stream())
     elif plan["n_rows"]:
         _attend_tokens(qkv, lane, ctx, out, nq, nkv, head_dim, scale, window, sink, sms, plan["rows"], None, plan["n_rows"], plan["longest"], 1 if group <= 8 else 2)
     if plan["tiles"] is not None:
