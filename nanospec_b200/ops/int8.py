@@ -58,23 +58,37 @@ def quantize_rows(x: torch.Tensor) -> RowsI8:
     return RowsI8(q, scale)
 
 
+# us that a pair of SMs takes for 128 of k of a tile of 256 tokens x so many features
+I8_WIDE_US = {64: 0.172, 128: 0.209, 192: 0.256, 256: 0.336}
+
+
 @functools.lru_cache(maxsize=4096)
 def i8_tiles(M: int, N: int, K: int, sms: int) -> tuple[int, int, int]:
-    """(tokens of a tile, features of a tile, blocks or pairs that divide k) of the product."""
-    k_blocks = -(-K // 128)
-    if M > 128:
-        tiles = -(-M // 256) * -(-N // 256)
-        splits = 1
-        while splits < 4 and tiles * splits * 2 <= sms // 2 and splits * 2 <= k_blocks:
+    """(tokens of a tile, features of a tile, blocks or pairs that divide k) of the product.
+
+    Up to 64 tokens, and up to 128 while the tiles of 128 features fit the SMs: one tile of tokens, k divided over up to eight blocks until every SM
+    has one, and beyond that while a block keeps eight of its 128-wide pieces (us on a B200, 32 x 4096 x 4096, one, two, four and eight blocks: 16.4, 14.3, 12.3,
+    14.3; 8 x 14336 x 4096: 32.8, 24.6, 22.5, 20.5; 77 x 2051 x 1003: eight 10.2, four 12.3; 128 x 4096 x 28672: 53 so, 43 in wide tiles).
+    More tokens: the wide tiles of least cost, `I8_WIDE_US` for every piece of k and round over the pairs of SMs; two pairs to a tile only while all
+    clusters of four blocks run at once (32 of them), for about 4 us (512 x 14336 x 4096: 256 features and two pairs 36.9, one 49.2; 200 x 4096 x 4096: 64
+    features 16.4, 256 20.5; four pairs took 47 where two took 31: clusters of eight such blocks do not all find a place)."""
+    k_blocks, tiles = -(-K // 128), -(-N // 128)
+    if M <= 64 or (M <= 128 and tiles <= sms):
+        tile = 16 if M <= 16 else 32 if M <= 32 else 64 if M <= 64 else 128
+        resident, splits = sms * (2 if tile <= 64 else 1), 1
+        while splits < 8 and splits * 2 <= k_blocks and (tiles * splits * 2 <= sms or (tiles * splits * 2 <= resident and k_blocks >= 16 * splits)):
             splits *= 2
-        return 256, 256, splits
-    tile = 16 if M <= 16 else 32 if M <= 32 else 64 if M <= 64 else 128
-    tiles = -(-N // 128)
-    resident = sms * (2 if tile <= 64 else 1)
-    splits = 1
-    while splits < 8 and tiles * splits * 2 <= resident and splits * 2 <= k_blocks:
-        splits *= 2
-    return tile, 128, splits
+        return tile, 128, splits
+    best = None
+    for features, us in I8_WIDE_US.items():
+        tiles = -(-M // 256) * -(-N // features)
+        for splits in (1, 2):
+            if splits > 1 and (tiles > 32 or k_blocks < 16):
+                continue
+            cost = -(-tiles // (sms // 2)) * -(-k_blocks // splits) * us + (4 if splits > 1 else 0)
+            if best is None or cost < best[0]:
+                best = (cost, features, splits)
+    return 256, *best[1:]
 
 
 def linear_i8(x: torch.Tensor | RowsI8, w: RowsI8, out: torch.Tensor, bias: torch.Tensor | None = None,
