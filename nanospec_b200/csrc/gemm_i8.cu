@@ -18,6 +18,8 @@ enum I8Error { kErrProducerWait = 61, kErrMmaWait = 62, kErrEpilogueWait = 63, k
 // D = 32-bit integers, A = B = signed 8-bit integers, both K-major
 __host__ __device__ constexpr uint32_t i8_desc(int m, int n) { return (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24); }
 
+// (spelled out, so that every tile rounds alike: an output's bits do not depend on which one it fell into)
+__device__ __forceinline__ float scaled(int sum, float x_scale, float w_scale) { return __fmul_rn(__int2float_rn(sum), __fmul_rn(x_scale, w_scale)); }
 __device__ __forceinline__ void put(float* p, float v) { *p = v; }
 __device__ __forceinline__ void put(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
 
@@ -191,8 +193,8 @@ gemm_i8_narrow_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_co
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const bool live = f + i < N;
-                y[i] = __int2float_rn(part[i]) * (scale * (live ? __ldg(ws + f + i) : 0.f));
-                if (bias && live) y[i] += __ldg(bias + f + i);
+                y[i] = scaled(part[i], scale, live ? __ldg(ws + f + i) : 0.f);
+                if (bias && live) y[i] = __fadd_rn(y[i], __ldg(bias + f + i));
             }
             if (f + 4 <= N && (reinterpret_cast<uintptr_t>(to) & (4 * sizeof(OutT) - 1)) == 0) {
                 if constexpr (sizeof(OutT) == 4) {
@@ -248,7 +250,7 @@ int launch(const void* x, long long ldx, const float* xs, const void* w, long lo
 }  // namespace narrow
 
 // ---- many tokens -------------------------------------------------------------------------------------------------------------
-// A cluster is `splits` pairs of blocks.  Of a pair, each block holds 128 tokens of A and of the accumulator, and half of the rows of B; the
+// A cluster is `splits` (1 or 2) pairs of blocks.  Of a pair, each block holds 128 tokens of A and of the accumulator, and half of the rows of B; the
 // pair's first block (the leader) issues.  Warps: 0 loads (each block its own operands; the bytes count on the leader's barrier), 1 issues (the
 // leader's), 2-9 the epilogue: four warps for each half of the columns.
 namespace wide {
@@ -256,7 +258,7 @@ constexpr int kTok = 256, kFeat = 256, kStages = 6, kThreads = 64 + 256;
 constexpr int kABytes = BM * BK, kStageBytes = 2 * BM * BK;
 constexpr int kPitch = 80, kBarBytes = 256;             // bytes of a staged row: 64 of outputs, so that eight rows fall in different banks
 constexpr int kSmem = kStages * kStageBytes + kBarBytes + 8 * 32 * kPitch + 1024;
-static_assert(kSmem <= 232448, "shared memory of a block");
+static_assert(kSmem <= 232448 && BM * kFeat / 2 * 4 <= kStages * kStageBytes, "shared memory of a block");
 
 __device__ __forceinline__ uint32_t at_rank(uint32_t local, uint32_t rank) {
     uint32_t r;
@@ -284,8 +286,8 @@ __device__ __forceinline__ void emit(const uint32_t (&r)[32], unsigned char* st,
             float y[kPer];
 #pragma unroll
             for (int i = 0; i < kPer; ++i) {
-                y[i] = __int2float_rn((int)r[c1 + c + i]) * (row_scale * __shfl_sync(0xffffffffu, mine_ws, c1 + c + i));
-                if (bias) y[i] += __shfl_sync(0xffffffffu, mine_b, c1 + c + i);
+                y[i] = scaled((int)r[c1 + c + i], row_scale, __shfl_sync(0xffffffffu, mine_ws, c1 + c + i));
+                if (bias) y[i] = __fadd_rn(y[i], __shfl_sync(0xffffffffu, mine_b, c1 + c + i));
             }
             unsigned char* p = st + lane * kPitch + c * sizeof(OutT);
             if constexpr (sizeof(OutT) == 4) *reinterpret_cast<float4*>(p) = make_float4(y[0], y[1], y[2], y[3]);
@@ -424,7 +426,7 @@ gemm_i8_wide_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
                     break;
                 }
         }
-    } else {
+    } else if (splits == 1) {
         const int q = warp & 3, half = (warp - 2) >> 2;  // q: the TMEM lane quarter this warp may read
         unsigned char* st = out_s + (warp - 2) * 32 * kPitch;
         const int row_in = q * 32, half_n = tile_n / 2;
@@ -448,51 +450,56 @@ gemm_i8_wide_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_cons
                     __syncwarp();
                     if (lane == 0) mbar_arrive_cluster(at_rank(acc_free(b), leader));
                 }
-                if (splits == 1) {
-                    if (row0 < M && col0 + c0 < N) emit(r, st, row_scale, ws, bias, out, ldo, row0, col0 + c0, M, N, aligned);
-                } else {
-                    int* stage = reinterpret_cast<int*>(smem);  // [tile_n][128]: the ring is free, the one tile is multiplied
+                if (row0 < M && col0 + c0 < N) emit(r, st, row_scale, ws, bias, out, ldo, row0, col0 + c0, M, N, aligned);
+            }
+        }
+    }
+    if (splits > 1) {
+        // Two pairs, one tile: each finishes half of its columns.  The columns that are the other pair's go to shared memory (the ring is free: the
+        // tile is multiplied), its own stay in tensor memory until the other pair's part of them can be read.
+        const int q = warp & 3, group = (warp - 2) >> 2, half_n = tile_n / 2;
+        const int row_in = q * 32, row0 = tok_of(cluster) + row_in, col0 = feat_of(cluster);
+        const uint32_t taddr = tmem_base + ((uint32_t)row_in << 16);
+        uint32_t* part = reinterpret_cast<uint32_t*>(smem) + row_in + lane;  // [column][128 rows]: a warp's 32 rows lie side by side, here and from another block
+        if (warp >= 2) {
+            if (!mbar_wait_warp(acc_full(0), 0)) {
+                if (lane == 0) { failed = 1; atomicExch(error_flag, kErrEpilogueWait); }
+            } else {
+                tc_fence_after();
+                for (int c = group * 32; c < half_n; c += 64) {
+                    uint32_t r[32];
+                    tmem_ld32(taddr + (1 - split) * half_n + c, r);
+                    tmem_ld_wait();
 #pragma unroll
-                    for (int j = 0; j < 32; ++j) stage[(c0 + j) * BM + row_in + lane] = (int)r[j];
+                    for (int j = 0; j < 32; ++j) part[(c + j) * BM] = r[j];
                 }
+            }
+        }
+        __syncthreads();
+        cluster_sync();
+        if (warp >= 2 && !failed && row0 < M) {
+            unsigned char* st = out_s + (warp - 2) * 32 * kPitch;
+            const float row_scale = row0 + lane < M ? __ldg(xs + row0 + lane) : 0.f;
+            for (int c = group * 32; c < half_n; c += 64) {
+                const int col = col0 + split * half_n + c;
+                if (col >= N) break;
+                uint32_t r[32];
+                tmem_ld32(taddr + split * half_n + c, r);
+                tmem_ld_wait();
+#pragma unroll
+                for (int j = 0; j < 32; ++j) r[j] += __float_as_uint(ld_cluster_f32(smem_u32(part + (c + j) * BM), rank ^ 2u));
+                emit(r, st, row_scale, ws, bias, out, ldo, row0, col, M, N, aligned);
             }
         }
     }
     __syncwarp();
     tc_fence_before();
     __syncthreads();
-    cluster_sync();  // no block's shared or tensor memory is being written any more
+    cluster_sync();  // no block's shared or tensor memory is in use any more
     if (warp == 1) {
         tc_fence_after();
         tmem_dealloc_pair(tmem_base, 512);
     }
-    if (splits == 1) return;
-    // Every pair of the cluster adds up its share of the tile's columns: each block for its own 128 tokens, from the blocks of its side.
-    if (warp >= 2 && !failed && cluster < tiles) {
-        const int q = warp & 3;
-        unsigned char* st = out_s + (warp - 2) * 32 * kPitch;
-        const int row0 = tok_of(cluster) + q * 32, col0 = feat_of(cluster);
-        const float row_scale = row0 + lane < M ? __ldg(xs + row0 + lane) : 0.f;
-        const int runs = tile_n / 32, mine = (warp - 2) >> 2;  // runs of 32 columns: every 2 * splits-th
-        for (int run = split * 2 + mine; run < runs; run += 2 * splits) {
-            if (row0 >= M || col0 + run * 32 >= N) continue;
-            uint32_t r[32];
-#pragma unroll
-            for (int j = 0; j < 32; ++j) r[j] = 0u;
-            for (int s = 0; s < splits; ++s) {
-                const uint32_t from = at_rank(base + 4u * (uint32_t)((run * 32) * BM + q * 32 + lane), 2u * s + side);
-#pragma unroll
-                for (int j = 0; j < 32; ++j) {
-                    uint32_t v;
-                    asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(from + 4u * (uint32_t)(j * BM)) : "memory");
-                    r[j] += v;
-                }
-            }
-            emit(r, st, row_scale, ws, bias, out, ldo, row0, col0 + run * 32, M, N, aligned);
-        }
-    }
-    __syncthreads();
-    cluster_sync();  // nobody's shared memory goes while another block reads it
 }
 
 template <typename OutT>
@@ -530,7 +537,7 @@ int launch(const void* x, long long ldx, const float* xs, const void* w, long lo
 
 // x [M, ldx], w [N, ldw] 8-bit integers whose rows start on 16-byte boundaries; xs [M], ws [N] (and bias [N] or null) float; out [M, ldo].
 // tile 16, 32, 64 or 128: that many tokens to a block, `splits` (1, 2, 4, 8, at most the blocks of 128 k) blocks to a tile; tile 256: 256 tokens and
-// `features` (a multiple of 64 up to 256) to a pair, `splits` (1, 2, 4) pairs to a tile.  `early`: the kernel before this one in the stream did not write w.
+// `features` (a multiple of 64 up to 256) to a pair, `splits` (1 or 2) pairs to a tile.  `early`: the kernel before this one in the stream did not write w.
 NS_API int ns_gemm_i8(const void* x, long long ldx, const float* xs, const void* w, long long ldw, const float* ws, const float* bias, void* out,
                       long long ldo, int M, int N, int K, int dtype, int tile, int features, int splits, int early, int sms, int* error_flag, cudaStream_t stream) {
     if (M <= 0 || N <= 0) return NS_OK;
@@ -538,7 +545,7 @@ NS_API int ns_gemm_i8(const void* x, long long ldx, const float* xs, const void*
     if (ldx % 16 || ldw % 16 || ((uintptr_t)x | (uintptr_t)w) % 16) NS_FAIL(NS_ERR_UNSUPPORTED, "ns_gemm_i8: rows must start on 16-byte boundaries");
     if (dtype != NS_BF16 && dtype != NS_F32) NS_FAIL(NS_ERR_UNSUPPORTED, "ns_gemm_i8: float32 and bfloat16 outputs, not type %d", dtype);
     const int k_blocks = (K + BK - 1) / BK;
-    if (!error_flag || splits < 1 || splits > (tile == 256 ? 4 : 8) || (splits & (splits - 1)) || splits > k_blocks ||
+    if (!error_flag || splits < 1 || splits > (tile == 256 ? 2 : 8) || (splits & (splits - 1)) || splits > k_blocks ||
         (tile == 256 && (features < 64 || features > 256 || features % 64)))
         NS_FAIL(NS_ERR_ARGUMENT, "ns_gemm_i8: tiles of %d x %d, %d blocks to a tile with %d blocks of k", tile, features, splits, k_blocks);
     if (tile < 256 && (M + tile - 1) / tile > 65535) NS_FAIL(NS_ERR_UNSUPPORTED, "ns_gemm_i8: too many rows (%d)", M);
