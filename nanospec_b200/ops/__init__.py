@@ -50,11 +50,11 @@ def _on_current_device(*tensors: torch.Tensor | None) -> None:
         if t is None:
             continue
         at = t.get_device()  # (-1: not on a CUDA device)
-        if dev is None:
+        if at < 0:
             _cuda(t)
+        if dev is None:
             dev = torch.cuda.current_device()
         if at != dev:
-            _cuda(t)
             raise KernelError(f"an operand lies on {t.device}, the current device is cuda:{dev}")
 
 

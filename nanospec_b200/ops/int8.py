@@ -30,16 +30,15 @@ class RowsI8:
         return self.q.float() * self.scale[:, None]
 
 
-def _aligned_rows(q: torch.Tensor) -> bool:
-    return q.stride(1) == 1 and q.stride(0) % 16 == 0 and q.data_ptr() % 16 == 0
-
-
-def _check_rows(r: RowsI8, name: str) -> None:
+def _check_rows(r: RowsI8, name: str) -> int:
+    """Elements from one row to the next."""
     q, scale = r.q, r.scale
     if q.dtype != torch.int8 or q.dim() != 2 or scale.dtype != torch.float32 or scale.shape != q.shape[:1] or not scale.is_contiguous():
         raise KernelError(f"linear_i8: {name} must be int8 [R, K] with one contiguous float32 scale per row")
-    if q.shape[0] and not _aligned_rows(q):
+    step, inner = q.stride()
+    if q.numel() and (inner != 1 or step % 16 or q.data_ptr() % 16):
         raise KernelError(f"linear_i8: the rows of {name} must start on 16-byte boundaries with unit inner stride (quantize_rows makes them so)")
+    return step
 
 
 def quantize_rows(x: torch.Tensor) -> RowsI8:
@@ -97,25 +96,27 @@ def linear_i8(x: torch.Tensor | RowsI8, w: RowsI8, out: torch.Tensor, bias: torc
     rows on the way (`quantize_rows`) unless it comes so, for several products of the same activations; `out` [N, F] is float32 or bfloat16
     with unit inner stride."""
     ready = isinstance(x, RowsI8)
-    held, wq = x.q if ready else x, w.q
-    _on_current_device(held, wq, w.scale, out, bias, x.scale if ready else None)
-    _check_rows(w, "w")
+    held, wq, ws = x.q if ready else x, w.q, w.scale
+    _on_current_device(held, wq, ws, out, bias, x.scale if ready else None)
+    ldw = _check_rows(w, "w")
     if ready:
         _check_rows(x, "x")
-    N, (F, K) = held.shape[0], wq.shape
-    if held.dim() != 2 or held.shape[1] != K or not 1 <= K <= I8_MAX_K or (N and held.stride(1) != 1):
-        raise KernelError(f"linear_i8: x {tuple(held.shape)} with unit inner stride and w {tuple(wq.shape)} must agree on K, which is {I8_MAX_K} at most")
-    if out.shape != (N, F) or (N and F and out.stride(1) != 1):
+    F, K = wq.shape
+    shape, (ldo, inner) = held.shape, out.stride() if out.dim() == 2 else (0, 0)
+    if len(shape) != 2 or shape[1] != K or not 1 <= K <= I8_MAX_K or (shape[0] and held.stride(1) != 1):
+        raise KernelError(f"linear_i8: x {tuple(shape)} with unit inner stride and w {tuple(wq.shape)} must agree on K, which is {I8_MAX_K} at most")
+    N = shape[0]
+    if out.shape != (N, F) or (N and F and inner != 1):
         raise KernelError(f"linear_i8: out must be [{N}, {F}] with unit inner stride, not {tuple(out.shape)} with strides {out.stride()}")
     if bias is not None and (bias.dtype != torch.float32 or bias.shape != (F,) or not bias.is_contiguous()):
         raise KernelError("linear_i8: the bias is one contiguous float32 number per output feature")
-    code, sms = dtype_code(out.dtype), sm_count()
-    tiles = tiles or i8_tiles(N, F, K, sms)
+    code, sms, dev = dtype_code(out.dtype), sm_count(), out.device
+    tile, features, splits = tiles or i8_tiles(N, F, K, sms)
     if ready:
-        lib.call("ns_gemm_i8", held.data_ptr(), held.stride(0), x.scale.data_ptr(), wq.data_ptr(), wq.stride(0), w.scale.data_ptr(), _ptr(bias),
-                 out.data_ptr(), out.stride(0), N, F, K, code, *tiles, 0, sms, _tc(out.device).error.data_ptr(), _stream())
+        lib.call("ns_gemm_i8", held.data_ptr(), held.stride(0), x.scale.data_ptr(), wq.data_ptr(), ldw, ws.data_ptr(), _ptr(bias), out.data_ptr(), ldo, N, F, K,
+                 code, tile, features, splits, 0, sms, _tc(dev).error.data_ptr(), _stream())
     else:
-        scratch = torch.empty(N * (-(-K // 16) * 16 + 4), dtype=torch.int8, device=out.device)
-        lib.call("ns_linear_i8", held.data_ptr(), held.stride(0), dtype_code(held.dtype), scratch.data_ptr(), wq.data_ptr(), wq.stride(0),
-                 w.scale.data_ptr(), _ptr(bias), out.data_ptr(), out.stride(0), N, F, K, code, *tiles, sms, _tc(out.device).error.data_ptr(), _stream())
+        scratch = torch.empty(N * (-(-K // 16) * 16 + 4), dtype=torch.int8, device=dev)
+        lib.call("ns_linear_i8", held.data_ptr(), held.stride(0), dtype_code(held.dtype), scratch.data_ptr(), wq.data_ptr(), ldw, ws.data_ptr(), _ptr(bias),
+                 out.data_ptr(), ldo, N, F, K, code, tile, features, splits, sms, _tc(dev).error.data_ptr(), _stream())
     return out

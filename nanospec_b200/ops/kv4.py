@@ -28,11 +28,11 @@ def kv4_pages(pages: int, kv_heads: int, page_size: int, head_dim: int, device: 
 
 
 def _check_lane(who: str, lane, nkv: int, head_dim: int) -> None:
+    k, v, table = lane.k, lane.v, lane.block_table
     size = kv4_block_bytes(lane.page_size, head_dim)
-    for t in (lane.k, lane.v):
-        if t is None or t.dtype != torch.uint8 or t.dim() != 3 or t.shape[1:] != (nkv, size) or not t.is_contiguous() or t.data_ptr() % 16:
-            raise KernelError(f"{who}: the lane's pages must be contiguous uint8 [pages, {nkv}, {size}] on 16-byte boundaries (kv4_pages makes them)")
-    table = lane.block_table
+    if k is None or v is None or k.dtype != torch.uint8 or v.dtype != torch.uint8 or k.shape != v.shape or k.dim() != 3 or k.shape[1:] != (nkv, size) \
+            or not k.is_contiguous() or not v.is_contiguous() or (k.data_ptr() | v.data_ptr()) % 16:
+        raise KernelError(f"{who}: the lane's pages must be contiguous uint8 [pages, {nkv}, {size}] on 16-byte boundaries (kv4_pages makes them)")
     if table is None or table.dtype != torch.int32 or table.dim() != 2 or table.stride(1) != 1:
         raise KernelError(f"{who}: block_table must be int32 [requests, pages] with unit inner stride")
 
@@ -59,12 +59,12 @@ def kv4_store(qkv: torch.Tensor, ctx, lane, nq: int, nkv: int, head_dim: int, in
     target = qkv if q_out is None else q_out
     if q_out is not None and (q_out.dtype != qkv.dtype or q_out.shape != (n, nq * head_dim)):
         raise KernelError("kv4_store: q_out must be [N, nq * head_dim] in the type of qkv")
-    for t in (qkv, target):
-        if n and (t.stride(1) != 1 or t.stride(0) * size % 16 or t.data_ptr() % 16):
-            raise KernelError("kv4_store: rows must start on 16-byte boundaries with unit inner stride")
+    (ld, inner), (ldq, inner_q) = qkv.stride(), target.stride()
+    if n and (inner != 1 or inner_q != 1 or (ld | ldq) * size % 16 or (qkv.data_ptr() | target.data_ptr()) % 16):
+        raise KernelError("kv4_store: rows must start on 16-byte boundaries with unit inner stride")
     if inv_freq is not None and (inv_freq.dtype != torch.float32 or not inv_freq.is_contiguous() or inv_freq.numel() > head_dim // 2):
         raise KernelError(f"kv4_store: inv_freq must be contiguous float32, at most {head_dim // 2} numbers")
-    lib.call("ns_kv4_store", qkv.data_ptr(), qkv.stride(0), target.data_ptr(), target.stride(0), ctx.positions.data_ptr(), ctx.token_req.data_ptr(),
+    lib.call("ns_kv4_store", qkv.data_ptr(), ld, target.data_ptr(), ldq, ctx.positions.data_ptr(), ctx.token_req.data_ptr(),
              lane.block_table.data_ptr(), lane.block_table.stride(0), _ptr(inv_freq), 0 if inv_freq is None else inv_freq.numel(), lane.k.data_ptr(),
              lane.v.data_ptr(), lane.page_size, nq, nkv, head_dim, n, sm_count(), code, _stream())
     return target
