@@ -1,9 +1,10 @@
 // Store into the 4-bit cache, with the rotation of q and k, and reading values back (the format: kv4.cuh).
 //
-// What the cache holds is the definition's to the last bit: angles, their sines and the rotation of k run in double and are rounded once to
-// the activations' type, S and B are rounded once from double, and codes are decided by the exact remainder.  One rounding that fell on
-// the other side of a border would move a feature by a whole code, or a group by its S.  q, which is rounded to the activations' type and not
-// quantised, is rotated in float.
+// What the cache holds is the definition's to the last bit: k rotated exactly and rounded once to the activations' type, S and B rounded once, codes decided by
+// exact remainders.  One rounding that fell on the other side of a border would move a feature by a whole code, or a group by its S.  Computed in double
+// throughout, a prompt is bound by its instructions (3,745 tokens of the 8B shape 53 us, 96 MB); so everything is first done in float, with a bound of
+// its error, and again in double where a border between two roundings lies within the bound - one element in some thousands.  float32 activations, which have
+// no bits to spare in float, are rotated in double.  q, which is rounded to the activations' type and not quantised, is rotated in float.
 #include "kv4.cuh"
 
 namespace {
@@ -12,14 +13,28 @@ constexpr int kThreads = 256;
 
 // a double to the nearest bfloat16, ties to even, in one rounding: to float towards zero with the last bit marking that something was
 // dropped (float has more than two bits beyond bfloat16's), then to bfloat16
-__device__ __forceinline__ float odd_float(double d) {
+__device__ __forceinline__ __nv_bfloat16 nearest_bf16(double d) {
     const float f = __double2float_rz(d);
-    return (double)f == d ? f : __uint_as_float(__float_as_uint(f) | 1u);
+    return __float2bfloat16_rn((double)f == d ? f : __uint_as_float(__float_as_uint(f) | 1u));
 }
-__device__ __forceinline__ __nv_bfloat16 nearest_bf16(double d) { return __float2bfloat16_rn(odd_float(d)); }
+// Whether a float that is off by no more than a few of its last bits may lie on the other side of the middle between two bfloat16 numbers.
+__device__ __forceinline__ bool near_middle(float f) { return (__float_as_uint(f) & 0xffffu) - 0x7ff8u <= 16u; }
 
-__device__ __forceinline__ float as_stored(const float*, double d) { return __double2float_rn(d); }
-__device__ __forceinline__ float as_stored(const __nv_bfloat16*, double d) { return __bfloat162float(nearest_bf16(d)); }
+// The angle position * frequency less whole turns, as a sum of two floats.
+__device__ __forceinline__ void turned_angle(int pos, float freq, float& hi, float& lo) {
+    const double a = (double)pos * (double)freq, n = rint(a * 0.15915494309189535);
+    const double r = fma(-n, 2.4492935982947064e-16, fma(-n, 6.283185307179586, a));
+    hi = (float)r;
+    lo = (float)(r - (double)hi);
+}
+// Its cosine and sine to about three half steps: of the larger float, turned on by the smaller one.
+__device__ __forceinline__ void cos_sin(int pos, float freq, float& c, float& s) {
+    float hi, lo, c0, s0;
+    turned_angle(pos, freq, hi, lo);
+    sincosf(hi, &s0, &c0);
+    c = fmaf(-s0, lo, c0);
+    s = fmaf(c0, lo, s0);
+}
 
 __device__ __forceinline__ void ld4(const float* p, float (&v)[4]) {
     const float4 a = *reinterpret_cast<const float4*>(p);
@@ -30,14 +45,11 @@ __device__ __forceinline__ void ld4(const __nv_bfloat16* p, float (&v)[4]) {
     const float2 a = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&u.x)), b = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&u.y));
     v[0] = a.x; v[1] = a.y; v[2] = b.x; v[3] = b.y;
 }
-__device__ __forceinline__ void st4(float* p, const float (&v)[4]) { *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]); }
-__device__ __forceinline__ void st4(__nv_bfloat16* p, const float (&v)[4]) {
-    const __nv_bfloat162 a = __floats2bfloat162_rn(v[0], v[1]), b = __floats2bfloat162_rn(v[2], v[3]);
-    *reinterpret_cast<uint2*>(p) = make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
-}
+
+constexpr float kMagic = 12582912.f;  // 1.5 * 2^23: added to it, a small number is rounded to an integer, which the last bits hold
 
 // the code of x in a group: the integer nearest to 16 (x - B) / S - 16, ties to even, within 0 .. 15
-__device__ __forceinline__ uint32_t code_of(float x, float S, float B, float inv) {
+__device__ __noinline__ uint32_t code_of(float x, float S, float B, float inv) {
     // d + rest = x - B without error
     const float d = __fsub_rn(x, B), back = __fsub_rn(d, x);
     const float rest = __fadd_rn(__fsub_rn(x, __fsub_rn(d, back)), __fsub_rn(-B, back));
@@ -52,21 +64,44 @@ __device__ __forceinline__ uint32_t code_of(float x, float S, float B, float inv
 
 struct Group { __nv_bfloat16 S, B; };
 
-// S and B of a group that lies over 8 neighbouring lanes, four features each; S is NaN where the group is not finite
-__device__ __forceinline__ Group group_of(const float (&x)[4], bool live) {
-    float lo = fminf(fminf(x[0], x[1]), fminf(x[2], x[3])), hi = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
-    // (x - x is NaN for infinities and NaN, whose presence the minimum and maximum would hide)
-    bool bad = live && !((x[0] - x[0]) + (x[1] - x[1]) + (x[2] - x[2]) + (x[3] - x[3]) == 0.f);
-#pragma unroll
-    for (int o = 1; o < 8; o <<= 1) {
-        lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-        hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
-        bad |= (bool)__shfl_xor_sync(0xffffffffu, (int)bad, o);
-    }
+__device__ __noinline__ Group exact_group(float lo, float hi) {
     const double spread = ((double)hi - (double)lo) * 16.0 / 15.0;
     Group g;
     g.S = spread < 7.888609052210118e-31 /* 2^-100 */ ? __float2bfloat16_rn(0.f) : nearest_bf16(spread);
     g.B = nearest_bf16((double)lo - (double)__bfloat162float(g.S));
+    return g;
+}
+
+// smallest and largest of a group, which lies over 8 neighbouring lanes
+__device__ __forceinline__ void bounds(const float*, float& lo, float& hi) {
+#pragma unroll
+    for (int o = 1; o < 8; o <<= 1) {
+        lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+        hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+    }
+}
+__device__ __forceinline__ void bounds(const __nv_bfloat16*, float& lo, float& hi) {  // (bfloat16 numbers, both in one register)
+    __nv_bfloat162 b = __floats2bfloat162_rn(lo, -hi);
+#pragma unroll
+    for (int o = 1; o < 8; o <<= 1) b = __hmin2(b, __shfl_xor_sync(0xffffffffu, b, o));
+    lo = __low2float(b);
+    hi = -__high2float(b);
+}
+
+// S and B of a group, four features in each of 8 neighbouring lanes; S is NaN where the group is not finite
+template <typename T>
+__device__ __forceinline__ Group group_of(const T* type, const float (&x)[4], bool live) {
+    float lo = fminf(fminf(x[0], x[1]), fminf(x[2], x[3])), hi = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
+    // (x - x is NaN for infinities and NaN, whose presence the minimum and maximum would hide)
+    const bool mine = live && !((x[0] - x[0]) + (x[1] - x[1]) + (x[2] - x[2]) + (x[3] - x[3]) == 0.f);
+    const bool bad = (__ballot_sync(0xffffffffu, mine) >> (threadIdx.x & 24u)) & 0xffu;
+    bounds(type, lo, hi);
+    const float spread = (hi - lo) * (16.f / 15.f);  // off by three half steps
+    Group g;
+    g.S = __float2bfloat16_rn(spread);
+    const float base = lo - __bfloat162float(g.S);
+    g.B = __float2bfloat16_rn(base);
+    if (near_middle(spread) || near_middle(base) || spread < 1.5777218e-30f /* 2^-99 */) g = exact_group(lo, hi);
     const float s = __bfloat162float(g.S), b = __bfloat162float(g.B);
     if (bad || !((s - s) + (b - b) == 0.f)) g.S = g.B = __ushort_as_bfloat16(0x7fff);
     return g;
@@ -77,31 +112,67 @@ __device__ __forceinline__ void put_group(const float (&x)[4], Group g, uint8_t*
     const float S = __bfloat162float(g.S), B = __bfloat162float(g.B);
     uint32_t c = 0u;
     if (S > 0.f) {
-        const float inv = __fdiv_rn(16.f, S);
+        const float inv = __fdividef(16.f, S), step = S * 0.0625f, half = 0.5f * step;
+        uint32_t t[4];
+        bool again = false;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) c |= code_of(x[i], S, B, inv) << (4 * i);
+        for (int i = 0; i < 4; ++i) {
+            const float d = __fsub_rn(x[i], B), sum = __fmaf_rn(d, inv, kMagic), k = __fsub_rn(sum, kMagic);
+            again |= fabsf(__fmaf_rn(-k, step, d)) >= half;
+            t[i] = __float_as_uint(fminf(fmaxf(sum, kMagic + 16.f), kMagic + 31.f)) & 15u;  // 16 .. 31: code + 16
+        }
+        if (again) {
+            const float near = __fdiv_rn(16.f, S);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) t[i] = code_of(x[i], S, B, near);
+        }
+        c = t[0] | t[1] << 4 | t[2] << 8 | t[3] << 12;
     }
     *reinterpret_cast<uint16_t*>(codes) = (uint16_t)c;
     if (first) *reinterpret_cast<__nv_bfloat162*>(pair) = __halves2bfloat162(g.S, g.B);
 }
 
-// One block (or `gridDim.y` blocks, which share its heads) per token; a warp takes a head of q, or a kv head's key and value.
-// A lane holds four neighbouring features of every 128, eight lanes a group.
+// A feature of k rotated, rounded to the type once: a c - b s for the first of its pair (`low`, b the other one), a c + b s for the second.
+__device__ __noinline__ float exact_rotation(float a, float b, int pos, float freq, bool low) {
+    double s, c;
+    sincos((double)pos * (double)freq, &s, &c);
+    return __bfloat162float(nearest_bf16(fma((double)a, c, (double)b * (low ? -s : s))));
+}
+__device__ __forceinline__ float rotated(const float*, float a, float b, double c, double s, int, float, bool low) {
+    return __double2float_rn(fma((double)a, c, (double)b * (low ? -s : s)));
+}
+__device__ __forceinline__ float rotated(const __nv_bfloat16*, float a, float b, float c, float s, int pos, float freq, bool low) {
+    const float r = fmaf(a, c, b * (low ? -s : s));
+    // cosine and sine are off by less than 1.25 * 2^-23, the product, the sum and the bounds themselves by half a step each: 1.4 * 2^-22 in all
+    const float off = (fabsf(a) + fabsf(b)) * 4.7683716e-7f;  // 2^-21
+    const __nv_bfloat162 both = __floats2bfloat162_rn(r - off, r + off);
+    const uint32_t u = *reinterpret_cast<const uint32_t*>(&both);
+    return (u & 0xffffu) == u >> 16 ? __low2float(both) : exact_rotation(a, b, pos, freq, low);
+}
+__device__ __forceinline__ void angles(int pos, float freq, float& c, float& s) { cos_sin(pos, freq, c, s); }
+__device__ __forceinline__ void angles(int pos, float freq, double& c, double& s) { sincos((double)pos * (double)freq, &s, &c); }
+
+// what a token's cosines and sines are held in
+template <typename T> struct Angle { using type = float; };
+template <> struct Angle<float> { using type = double; };
+
+// One block (or `gridDim.y` blocks, which share its heads) per token.  For keys and values a lane holds four neighbouring features of every 128, eight lanes a group.
 template <typename T, int kChunks>
 __global__ void __launch_bounds__(kThreads)
 kv4_store_kernel(const T* __restrict__ qkv, long long ld, T* __restrict__ q_out, long long ldq, const int* __restrict__ positions,
                  const int* __restrict__ token_req, const int* __restrict__ block_table, int table_stride, const float* __restrict__ inv_freq,
                  int pairs, uint8_t* __restrict__ k_pages, uint8_t* __restrict__ v_pages, int page_size, int nq, int nkv, int D) {
     ns_pdl_launch_dependents();
-    __shared__ double cs[256];  // cos of the token's angles, then their sines
+    using A = typename Angle<T>::type;
+    __shared__ __align__(16) A cs[256];  // cosines of the token's angles, then their sines
     const int n = blockIdx.x, half = D / 2;
     const int req = token_req[n];
     if (req < 0) { ns_pdl_wait(); return; }  // a padding row (it waits all the same: see common.cuh)
     const int pos = positions[n];
     const int page = block_table[(size_t)req * table_stride + pos / page_size];
     for (int j = threadIdx.x; j < half; j += kThreads) {
-        double s = 0.0, c = 1.0;
-        if (j < pairs) sincos((double)pos * (double)inv_freq[j], &s, &c);
+        A s = 0, c = 1;
+        if (j < pairs) angles(pos, inv_freq[j], c, s);
         cs[j] = c;
         cs[half + j] = s;
     }
@@ -110,28 +181,29 @@ kv4_store_kernel(const T* __restrict__ qkv, long long ld, T* __restrict__ q_out,
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = kThreads / 32 * gridDim.y;
     const T* row = qkv + (size_t)n * ld;
     const int first = blockIdx.y * (kThreads / 32) + warp;
-    // heads 0 .. nkv - 1 here are the kv heads, which take longer, then those of q (none without a rotation whose output stays in place)
-    const int units = nkv + (pairs > 0 || q_out != qkv ? nq : 0);
-    for (int u = first; u < units; u += warps) {
-        if (u >= nkv) {
-            const T* x = row + (size_t)(u - nkv) * D;
-            T* y = q_out + (size_t)n * ldq + (size_t)(u - nkv) * D;
-            // (both halves of a pair in one lane: q may be rotated in place)
-            for (int f = lane * 4; f < half; f += 128) {
-                float a[4], b[4], oa[4], ob[4];
-                ld4(x + f, a);
-                ld4(x + half + f, b);
+    // q: eight pairs of a head to a thread (both features of a pair: q may be rotated in place); nothing to do without a rotation whose output stays in place
+    if (pairs > 0 || q_out != qkv) {
+        const int per_head = half / 8;
+        for (int i = blockIdx.y * kThreads + threadIdx.x; i < nq * per_head; i += gridDim.y * kThreads) {
+            const int h = i / per_head, f = (i - h * per_head) * 8;
+            const T* x = row + (size_t)h * D + f;
+            T* y = q_out + (size_t)n * ldq + (size_t)h * D + f;
+            float a[8], b[8], oa[8], ob[8], c[8], s[8];
+            ld8(x, a);
+            ld8(x + half, b);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float c = (float)cs[f + i], s = (float)cs[half + f + i];
-                    oa[i] = __fmaf_rn(a[i], c, -__fmul_rn(b[i], s));
-                    ob[i] = __fmaf_rn(b[i], c, __fmul_rn(a[i], s));
-                }
-                st4(y + f, oa);
-                st4(y + half + f, ob);
+            for (int k = 0; k < 8; ++k) { c[k] = (float)cs[f + k]; s[k] = (float)cs[half + f + k]; }
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                oa[k] = __fmaf_rn(a[k], c[k], -__fmul_rn(b[k], s[k]));
+                ob[k] = __fmaf_rn(b[k], c[k], __fmul_rn(a[k], s[k]));
             }
-            continue;
+            st8(y, oa);
+            st8(y + half, ob);
         }
+    }
+    // a warp to each kv head's key and value
+    for (int u = first; u < nkv; u += warps) {
         const T* kx = row + (size_t)(nq + u) * D;
         const T* vx = kx + (size_t)nkv * D;
         float k[kChunks][4], v[kChunks][4];
@@ -151,13 +223,11 @@ kv4_store_kernel(const T* __restrict__ qkv, long long ld, T* __restrict__ q_out,
                 ld4(kx + (low ? f + half : j), other);
                 ld4(vx + f, v[ch]);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const double c = cs[j + i], s = low ? -cs[half + j + i] : cs[half + j + i];
-                    k[ch][i] = as_stored(qkv, fma((double)mine[i], c, (double)other[i] * s));
-                }
+                for (int i = 0; i < 4; ++i)
+                    k[ch][i] = j + i < pairs ? rotated(qkv, mine[i], other[i], cs[j + i], cs[half + j + i], pos, inv_freq[j + i], low) : mine[i];
             }
-            gk[ch] = group_of(k[ch], live);
-            gv[ch] = group_of(v[ch], live);
+            gk[ch] = group_of(qkv, k[ch], live);
+            gv[ch] = group_of(qkv, v[ch], live);
             bad |= live && (__hisnan(gk[ch].S) || __hisnan(gv[ch].S));
         }
         bad = __any_sync(0xffffffffu, bad);
@@ -183,12 +253,15 @@ kv4_read_kernel(const uint8_t* __restrict__ k_pages, const uint8_t* __restrict__
                 __nv_bfloat16* __restrict__ v_out, int n_tokens, int page_size, int nkv, int D) {
     ns_pdl_launch_dependents();
     ns_pdl_wait();
-    const int words = D / 8;
-    const long long total = (long long)n_tokens * nkv * words;
-    for (long long i = (long long)blockIdx.x * kThreads + threadIdx.x; i < total; i += (long long)gridDim.x * kThreads) {
-        const int w = (int)(i % words);
-        const long long th = i / words;
-        const int h = (int)(th % nkv), n = (int)(th / nkv);
+    const int words = D / 8, per_token = nkv * words;
+    // a block takes tokens in turn (their number, and not that of all words, holds in 32 bits)
+    const int side = max(1, kThreads / per_token), lanes = kThreads / side;  // tokens at a time, threads of each
+    const int part = threadIdx.x / lanes;
+    if (part >= side) return;
+    for (long long n = (long long)blockIdx.x * side + part; n < n_tokens; n += (long long)gridDim.x * side)
+    for (int u = threadIdx.x - part * lanes; u < per_token; u += lanes) {
+        const long long i = n * per_token + u;
+        const int h = u / words, w = u - h * words;
         const int req = token_req[n];
         uint4 k = make_uint4(0u, 0u, 0u, 0u), v = k;
         if (req >= 0) {
@@ -248,8 +321,8 @@ NS_API int ns_kv4_read(const void* k_pages, const void* v_pages, const int* posi
     if (n_tokens <= 0) return NS_OK;
     int rc = check_geometry("ns_kv4_read", D, nkv, page_size);
     if (rc) return rc;
-    const long long items = (long long)n_tokens * nkv * (D / 8), blocks = (items + kThreads - 1) / kThreads;
-    const int grid = (int)(blocks < 16ll * sms ? blocks : 16ll * sms);
+    const int per_token = nkv * (D / 8), side = per_token < kThreads ? kThreads / per_token : 1, blocks = (n_tokens + side - 1) / side;
+    const int grid = blocks < 16 * sms ? blocks : 16 * sms;
     NS_LAUNCH(kv4_read_kernel, grid, kThreads, 0, stream, (const uint8_t*)k_pages, (const uint8_t*)v_pages, positions, token_req, block_table, table_stride,
               (__nv_bfloat16*)k_out, (__nv_bfloat16*)v_out, n_tokens, page_size, nkv, D);
     NS_CHECK_LAUNCH("ns_kv4_read");
@@ -268,7 +341,8 @@ kv4_unfold_kernel(const uint8_t* __restrict__ k_pages, const uint8_t* __restrict
                   int page_size, int nkv, int head0, int D) {
     ns_pdl_wait();
     ns_pdl_launch_dependents();
-    __shared__ long long base[kUnfoldTokens];  // where a token's block begins, less its slot's codes; -1: not held
+    __shared__ long long base[kUnfoldTokens];  // where a token's block begins; -1: not held
+    __shared__ int slots[kUnfoldTokens];
     const int req = items[2 * blockIdx.x], pos0 = items[2 * blockIdx.x + 1] * kUnfoldTokens, words = D / 8;
     const int h = blockIdx.y, held = kv_len[req];
     if (threadIdx.x < kUnfoldTokens) {
@@ -277,15 +351,17 @@ kv4_unfold_kernel(const uint8_t* __restrict__ k_pages, const uint8_t* __restrict
         const int page = pos < held ? block_table[(size_t)req * table_stride + pos / page_size] : -1;
         if (page >= 0) at = (long long)(((size_t)page * nkv + head0 + h) * kv4_block_bytes(page_size, D));
         base[threadIdx.x] = at;
+        slots[threadIdx.x] = pos % page_size;
     }
     __syncthreads();
+    const unsigned by_words = (65536u + words - 1u) / words;
     const size_t out0 = ((size_t)blockIdx.x * gridDim.y + h) * kUnfoldTokens * D;
     for (int i = threadIdx.x; i < kUnfoldTokens * words; i += kThreads) {
-        const int token = i / words, w = i - token * words;
+        const int token = (int)((unsigned)i * by_words >> 16), w = i - token * words;  // i / words: exact below 2^16 / words
         const long long at = base[token];
         uint4 k = make_uint4(0u, 0u, 0u, 0u), v = k;
         if (at >= 0) {
-            const int slot = (pos0 + token) % page_size;
+            const int slot = slots[token];
             const size_t codes = (size_t)at + ((size_t)slot * words + w) * 4, pair = (size_t)at + (size_t)page_size * (D / 2) + ((size_t)slot * (D / kGroup) + w / 4) * 4;
             k = kv4_in_order(*reinterpret_cast<const uint32_t*>(k_pages + codes), *reinterpret_cast<const uint32_t*>(k_pages + pair));
             v = kv4_in_order(*reinterpret_cast<const uint32_t*>(v_pages + codes), *reinterpret_cast<const uint32_t*>(v_pages + pair));

@@ -1,8 +1,9 @@
 // Rows in 8-bit integers with a float scale each: s = max |x| / 127 rounded to float, q = x / s to the nearest integer, ties to even.
 //
-// The quotient that is rounded is the exact one: a first guess from the reciprocal is off by one at most, and the remainder
-// x - q s, which one fused multiply-add gives without error (its bits are no finer than half of s's last and it is at most about s / 2),
-// says whether the guess stays.  The maximum is taken over the bit patterns of |x|, in whose order infinities and NaN come last.
+// The quotient that is rounded is the exact one: a first guess (x times the reciprocal, added to 1.5 * 2^23, whose last bits are then the integer) is off by
+// one at most, and the remainder x - q s, which one fused multiply-add gives without error (its bits are no finer than half of s's last and it is at most
+// about s / 2), says whether the guess stays.  It nearly always does: a piece of eight elements is looked at once more only when a remainder reaches s / 2.
+// The maximum is taken over the bit patterns of |x|, in whose order infinities and NaN come last.
 //
 // Bound by memory: a row is read once (its pieces stay in registers where the block holds them) and written once in a byte per element.
 #include "common.cuh"
@@ -12,7 +13,9 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kHeld = 4;  // pieces of 8 elements that a thread keeps: rows of up to 8,192
 
-__device__ __forceinline__ int nearest(float x, float s, float inv) {
+constexpr float kMagic = 12582912.f;  // 1.5 * 2^23
+
+__device__ __noinline__ int nearest(float x, float s, float inv) {
     float r = rintf(x * inv);
     const float e = fmaf(-r, s, x), half = 0.5f * s;
     const bool odd = ((int)r) & 1;
@@ -34,8 +37,22 @@ __device__ __forceinline__ void load_piece(const T* row, int k, int K, bool wide
 __device__ __forceinline__ void store_piece(int8_t* out, int k, int K, const float (&v)[8], float s, float inv) {
     uint32_t w[2] = {0u, 0u};
     if (inv != 0.f) {
+        const float half = 0.5f * s;
+        uint32_t t[8];
+        bool again = false;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) w[i >> 2] |= ((uint32_t)nearest(v[i], s, inv) & 255u) << (8 * (i & 3));
+        for (int i = 0; i < 8; ++i) {
+            const float sum = __fmaf_rn(v[i], inv, kMagic), r = __fsub_rn(sum, kMagic);
+            again |= fabsf(__fmaf_rn(-r, s, v[i])) >= half;
+            t[i] = __float_as_uint(sum);
+        }
+        if (again) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) t[i] = (uint32_t)nearest(v[i], s, inv);
+        }
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+            w[i] = __byte_perm(__byte_perm(t[4 * i], t[4 * i + 1], 0x0040), __byte_perm(t[4 * i + 2], t[4 * i + 3], 0x0040), 0x5410);
     }
     if (k + 8 <= K) {
         *reinterpret_cast<uint2*>(out + k) = make_uint2(w[0], w[1]);
