@@ -99,16 +99,23 @@ __device__ __forceinline__ Group group_of(const T* type, const float (&x)[4], bo
     const float spread = (hi - lo) * (16.f / 15.f);  // off by three half steps
     Group g;
     g.S = __float2bfloat16_rn(spread);
-    const float base = lo - __bfloat162float(g.S);
+    const float S = __bfloat162float(g.S), base = __fsub_rn(lo, S), back = __fsub_rn(base, lo);
     g.B = __float2bfloat16_rn(base);
-    if (near_middle(spread) || near_middle(base) || spread < 1.5777218e-30f /* 2^-99 */) g = exact_group(lo, hi);
+    // (the difference of two bfloat16 numbers is mostly exact, and often just in the middle)
+    const bool inexact = __fadd_rn(__fsub_rn(lo, __fsub_rn(base, back)), __fsub_rn(-S, back)) != 0.f;
+    if (near_middle(spread) || (inexact && near_middle(base)) || spread < 1.5777218e-30f /* 2^-99 */) g = exact_group(lo, hi);
     const float s = __bfloat162float(g.S), b = __bfloat162float(g.B);
     if (bad || !((s - s) + (b - b) == 0.f)) g.S = g.B = __ushort_as_bfloat16(0x7fff);
     return g;
 }
 
+// Whether d = x - B, half way between two codes, may not be all of x - B: never between bfloat16 numbers, but where x is next to nothing beside B.
+__device__ __forceinline__ bool more_than(const float*, float, float) { return true; }
+__device__ __forceinline__ bool more_than(const __nv_bfloat16*, float x, float step) { return x != 0.f && fabsf(x) < step; }
+
 // four neighbouring codes and, from one lane of the group, its pair (codes of 0 where S is not a positive number)
-__device__ __forceinline__ void put_group(const float (&x)[4], Group g, uint8_t* codes, uint8_t* pair, bool first) {
+template <typename T>
+__device__ __forceinline__ void put_group(const T* type, const float (&x)[4], Group g, uint8_t* codes, uint8_t* pair, bool first) {
     const float S = __bfloat162float(g.S), B = __bfloat162float(g.B);
     uint32_t c = 0u;
     if (S > 0.f) {
@@ -117,8 +124,14 @@ __device__ __forceinline__ void put_group(const float (&x)[4], Group g, uint8_t*
         bool again = false;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const float d = __fsub_rn(x[i], B), sum = __fmaf_rn(d, inv, kMagic), k = __fsub_rn(sum, kMagic);
-            again |= fabsf(__fmaf_rn(-k, step, d)) >= half;
+            const float d = __fsub_rn(x[i], B);
+            float sum = __fmaf_rn(d, inv, kMagic);
+            const float e = __fmaf_rn(__fsub_rn(kMagic, sum), step, d);
+            again |= fabsf(e) > half;
+            if (fabsf(e) == half) {  // half way: to the even one
+                if (__float_as_uint(sum) & 1u) sum += copysignf(1.f, e);
+                again |= more_than(type, x[i], step);
+            }
             t[i] = __float_as_uint(fminf(fmaxf(sum, kMagic + 16.f), kMagic + 31.f)) & 15u;  // 16 .. 31: code + 16
         }
         if (again) {
@@ -133,15 +146,15 @@ __device__ __forceinline__ void put_group(const float (&x)[4], Group g, uint8_t*
 }
 
 // A feature of k rotated, rounded to the type once: a c - b s for the first of its pair (`low`, b the other one), a c + b s for the second.
-__device__ __noinline__ float exact_rotation(float a, float b, int pos, float freq, bool low) {
+__device__ __noinline__ float exact_rotation(float a, float b, int pos, const float* freq, bool low) {
     double s, c;
-    sincos((double)pos * (double)freq, &s, &c);
+    sincos((double)pos * (double)*freq, &s, &c);
     return __bfloat162float(nearest_bf16(fma((double)a, c, (double)b * (low ? -s : s))));
 }
-__device__ __forceinline__ float rotated(const float*, float a, float b, double c, double s, int, float, bool low) {
+__device__ __forceinline__ float rotated(const float*, float a, float b, double c, double s, int, const float*, bool low) {
     return __double2float_rn(fma((double)a, c, (double)b * (low ? -s : s)));
 }
-__device__ __forceinline__ float rotated(const __nv_bfloat16*, float a, float b, float c, float s, int pos, float freq, bool low) {
+__device__ __forceinline__ float rotated(const __nv_bfloat16*, float a, float b, float c, float s, int pos, const float* freq, bool low) {
     const float r = fmaf(a, c, b * (low ? -s : s));
     // cosine and sine are off by less than 1.25 * 2^-23, the product, the sum and the bounds themselves by half a step each: 1.4 * 2^-22 in all
     const float off = (fabsf(a) + fabsf(b)) * 4.7683716e-7f;  // 2^-21
@@ -162,14 +175,47 @@ __global__ void __launch_bounds__(kThreads)
 kv4_store_kernel(const T* __restrict__ qkv, long long ld, T* __restrict__ q_out, long long ldq, const int* __restrict__ positions,
                  const int* __restrict__ token_req, const int* __restrict__ block_table, int table_stride, const float* __restrict__ inv_freq,
                  int pairs, uint8_t* __restrict__ k_pages, uint8_t* __restrict__ v_pages, int page_size, int nq, int nkv, int D) {
-    ns_pdl_launch_dependents();
     using A = typename Angle<T>::type;
     __shared__ __align__(16) A cs[256];  // cosines of the token's angles, then their sines
-    const int n = blockIdx.x, half = D / 2;
-    const int req = token_req[n];
-    if (req < 0) { ns_pdl_wait(); return; }  // a padding row (it waits all the same: see common.cuh)
-    const int pos = positions[n];
-    const int page = block_table[(size_t)req * table_stride + pos / page_size];
+    __shared__ long long block_s;        // where the token's page begins
+    __shared__ int slot_s;
+    ns_pdl_wait();
+    ns_pdl_launch_dependents();
+    const int n = blockIdx.x, half = D / 2, req = token_req[n], pos = positions[n];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = kThreads / 32 * gridDim.y, first = blockIdx.y * (kThreads / 32) + warp;
+    const T* row = qkv + (size_t)n * ld;
+    // What this thread takes first is asked for before the angles are worked out.
+    // q: eight pairs of a head to a thread (both features of a pair: q may be rotated in place); nothing to do without a rotation whose output stays in place
+    const int per_head = half / 8, q_units = pairs > 0 || q_out != qkv ? nq * per_head : 0;
+    int q_unit = blockIdx.y * kThreads + threadIdx.x;
+    float a[8], b[8];
+    auto load_q = [&] {
+        const int h = q_unit / per_head;
+        const T* x = row + (size_t)h * D + (q_unit - h * per_head) * 8;
+        ld8(x, a);
+        ld8(x + half, b);
+    };
+    if (q_unit < q_units) load_q();
+    // keys and values: a warp to each kv head's
+    float mine[kChunks][4], other[kChunks][4], v[kChunks][4];
+    auto load_kv = [&](int u) {
+        const T* kx = row + (size_t)(nq + u) * D;
+#pragma unroll
+        for (int ch = 0; ch < kChunks; ++ch) {
+            const int f = ch * 128 + lane * 4;
+            if (f >= D) break;
+            ld4(kx + f, mine[ch]);
+            ld4(kx + (f < half ? f + half : f - half), other[ch]);
+            ld4(kx + (size_t)nkv * D + f, v[ch]);
+        }
+    };
+    if (first < nkv) load_kv(first);
+    if (req < 0) return;  // a padding row
+    if (threadIdx.x == kThreads - 1) {
+        const int page = block_table[(size_t)req * table_stride + pos / page_size];
+        block_s = (long long)page * nkv * (long long)kv4_block_bytes(page_size, D);
+        slot_s = pos % page_size;
+    }
     for (int j = threadIdx.x; j < half; j += kThreads) {
         A s = 0, c = 1;
         if (j < pairs) angles(pos, inv_freq[j], c, s);
@@ -177,71 +223,49 @@ kv4_store_kernel(const T* __restrict__ qkv, long long ld, T* __restrict__ q_out,
         cs[half + j] = s;
     }
     __syncthreads();
-    ns_pdl_wait();
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = kThreads / 32 * gridDim.y;
-    const T* row = qkv + (size_t)n * ld;
-    const int first = blockIdx.y * (kThreads / 32) + warp;
-    // q: eight pairs of a head to a thread (both features of a pair: q may be rotated in place); nothing to do without a rotation whose output stays in place
-    if (pairs > 0 || q_out != qkv) {
-        const int per_head = half / 8;
-        for (int i = blockIdx.y * kThreads + threadIdx.x; i < nq * per_head; i += gridDim.y * kThreads) {
-            const int h = i / per_head, f = (i - h * per_head) * 8;
-            const T* x = row + (size_t)h * D + f;
-            T* y = q_out + (size_t)n * ldq + (size_t)h * D + f;
-            float a[8], b[8], oa[8], ob[8], c[8], s[8];
-            ld8(x, a);
-            ld8(x + half, b);
+    for (; q_unit < q_units; q_unit += gridDim.y * kThreads) {
+        if (q_unit >= (int)gridDim.y * kThreads) load_q();
+        const int h = q_unit / per_head, f = (q_unit - h * per_head) * 8;
+        T* y = q_out + (size_t)n * ldq + (size_t)h * D + f;
+        float oa[8], ob[8];
 #pragma unroll
-            for (int k = 0; k < 8; ++k) { c[k] = (float)cs[f + k]; s[k] = (float)cs[half + f + k]; }
-#pragma unroll
-            for (int k = 0; k < 8; ++k) {
-                oa[k] = __fmaf_rn(a[k], c[k], -__fmul_rn(b[k], s[k]));
-                ob[k] = __fmaf_rn(b[k], c[k], __fmul_rn(a[k], s[k]));
-            }
-            st8(y, oa);
-            st8(y + half, ob);
+        for (int k = 0; k < 8; ++k) {
+            const float c = (float)cs[f + k], s = (float)cs[half + f + k];
+            oa[k] = __fmaf_rn(a[k], c, -__fmul_rn(b[k], s));
+            ob[k] = __fmaf_rn(b[k], c, __fmul_rn(a[k], s));
         }
+        st8(y, oa);
+        st8(y + half, ob);
     }
-    // a warp to each kv head's key and value
+    const int slot = slot_s, pair_at = page_size * half + slot * (D / 8);
     for (int u = first; u < nkv; u += warps) {
-        const T* kx = row + (size_t)(nq + u) * D;
-        const T* vx = kx + (size_t)nkv * D;
-        float k[kChunks][4], v[kChunks][4];
+        if (u != first) load_kv(u);
+        float k[kChunks][4];
         Group gk[kChunks], gv[kChunks];
         bool bad = false;  // the token's key or value is not finite
 #pragma unroll
         for (int ch = 0; ch < kChunks; ++ch) {
-            const int f = ch * 128 + lane * 4;
+            const int f = ch * 128 + lane * 4, j = f < half ? f : f - half;
             const bool live = f < D;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) k[ch][i] = v[ch][i] = 0.f;
-            if (live) {
-                const bool low = f < half;
-                const int j = low ? f : f - half;
-                float mine[4], other[4];
-                ld4(kx + f, mine);
-                ld4(kx + (low ? f + half : j), other);
-                ld4(vx + f, v[ch]);
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    k[ch][i] = j + i < pairs ? rotated(qkv, mine[i], other[i], cs[j + i], cs[half + j + i], pos, inv_freq[j + i], low) : mine[i];
+            for (int i = 0; i < 4; ++i) {
+                k[ch][i] = !live ? 0.f : j + i < pairs ? rotated(qkv, mine[ch][i], other[ch][i], cs[j + i], cs[half + j + i], pos, inv_freq + j + i, f < half) : mine[ch][i];
+                if (!live) v[ch][i] = 0.f;
             }
             gk[ch] = group_of(qkv, k[ch], live);
             gv[ch] = group_of(qkv, v[ch], live);
             bad |= live && (__hisnan(gk[ch].S) || __hisnan(gv[ch].S));
         }
         bad = __any_sync(0xffffffffu, bad);
-        const size_t block = ((size_t)page * nkv + u) * kv4_block_bytes(page_size, D);
-        const int slot = pos % page_size;
+        const size_t block = (size_t)block_s + (size_t)u * kv4_block_bytes(page_size, D);
 #pragma unroll
         for (int ch = 0; ch < kChunks; ++ch) {
             const int f = ch * 128 + lane * 4;
             if (f >= D) break;
-            const size_t codes = block + (size_t)slot * half + f / 2;
-            const size_t pair = block + (size_t)page_size * half + ((size_t)slot * (D / kGroup) + f / kGroup) * 4;
+            const size_t codes = block + slot * half + f / 2, pair = block + pair_at + f / kGroup * 4;
             const Group nan = {__ushort_as_bfloat16(0x7fff), __ushort_as_bfloat16(0x7fff)}, zero = {__ushort_as_bfloat16(0), __ushort_as_bfloat16(0)};
-            put_group(k[ch], bad ? nan : gk[ch], k_pages + codes, k_pages + pair, (lane & 7) == 0);
-            put_group(v[ch], __hisnan(gv[ch].S) ? zero : gv[ch], v_pages + codes, v_pages + pair, (lane & 7) == 0);
+            put_group(qkv, k[ch], bad ? nan : gk[ch], k_pages + codes, k_pages + pair, (lane & 7) == 0);
+            put_group(qkv, v[ch], __hisnan(gv[ch].S) ? zero : gv[ch], v_pages + codes, v_pages + pair, (lane & 7) == 0);
         }
     }
 }

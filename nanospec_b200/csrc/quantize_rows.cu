@@ -24,13 +24,49 @@ __device__ __noinline__ int nearest(float x, float s, float inv) {
     return (int)r;
 }
 
+// A piece of eight elements as it lies in memory, the largest |x| of it, and its elements as floats.
+template <typename T> struct Piece;
+template <> struct Piece<float> {
+    float v[8];
+    __device__ __forceinline__ void load(const float* p) { ld8(p, v); }
+    __device__ __forceinline__ void set(int i, float x) { v[i] = x; }
+    __device__ __forceinline__ uint32_t top() const {
+        uint32_t m = 0u;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(v[i]) & 0x7fffffffu);
+        return m;
+    }
+    __device__ __forceinline__ void floats(float (&x)[8]) const {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = v[i];
+    }
+};
+template <> struct Piece<__nv_bfloat16> {
+    uint32_t u[4];
+    __device__ __forceinline__ void load(const __nv_bfloat16* p) {
+        const uint4 a = *reinterpret_cast<const uint4*>(p);
+        u[0] = a.x; u[1] = a.y; u[2] = a.z; u[3] = a.w;
+    }
+    __device__ __forceinline__ void set(int i, __nv_bfloat16 x) {
+        const uint32_t b = __bfloat16_as_ushort(x);
+        u[i >> 1] = i & 1 ? (u[i >> 1] & 0xffffu) | b << 16 : (u[i >> 1] & 0xffff0000u) | b;
+    }
+    __device__ __forceinline__ uint32_t top() const {  // (two at a time: the order of the bits is that of the numbers)
+        const uint32_t m = __vmaxu2(__vmaxu2(u[0] & 0x7fff7fffu, u[1] & 0x7fff7fffu), __vmaxu2(u[2] & 0x7fff7fffu, u[3] & 0x7fff7fffu));
+        return max(m << 16, m & 0xffff0000u);
+    }
+    __device__ __forceinline__ void floats(float (&x)[8]) const {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) { x[2 * i] = __uint_as_float(u[i] << 16); x[2 * i + 1] = __uint_as_float(u[i] & 0xffff0000u); }
+    }
+};
 template <typename T>
-__device__ __forceinline__ void load_piece(const T* row, int k, int K, bool wide, float (&v)[8]) {
+__device__ __forceinline__ void load_piece(Piece<T>& p, const T* row, int k, int K, bool wide) {
     if (wide && k + 8 <= K) {
-        ld8(row + k, v);
+        p.load(row + k);
     } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = k + i < K ? ns_ld(row, k + i) : 0.f;
+        for (int i = 0; i < 8; ++i) p.set(i, k + i < K ? row[k + i] : T(0.f));
     }
 }
 
@@ -68,18 +104,23 @@ quantize_rows_kernel(const T* __restrict__ x, long long ldx, int8_t* __restrict_
     ns_pdl_launch_dependents();  // in this order: the product asks for its weights without a wait of its own, and a kernel before this one may have written them
     __shared__ uint32_t tops[kThreads / 32];
     const T* row = x + (size_t)blockIdx.x * ldx;
-    float v[kHeld][8];
+    Piece<T> held[kHeld];
     uint32_t top = 0u;
-    for (int k = threadIdx.x * 8, i = 0; k < K; k += kThreads * 8, ++i) {
-        float t[8];
-        load_piece(row, k, K, wide, t);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) top = max(top, __float_as_uint(t[j]) & 0x7fffffffu);
+    for (int u = 0; u < kHeld; ++u) {
+        const int k = (u * kThreads + threadIdx.x) * 8;
+        if (k >= K) break;
+        load_piece(held[u], row, k, K, wide);
+    }
 #pragma unroll
-        for (int u = 0; u < kHeld; ++u)
-            if (u == i)
-#pragma unroll
-                for (int j = 0; j < 8; ++j) v[u][j] = t[j];
+    for (int u = 0; u < kHeld; ++u) {
+        if ((u * kThreads + threadIdx.x) * 8 >= K) break;
+        top = max(top, held[u].top());
+    }
+    for (int k = (kHeld * kThreads + threadIdx.x) * 8; k < K; k += kThreads * 8) {  // what is beyond the block's registers is read again below
+        Piece<T> p;
+        load_piece(p, row, k, K, wide);
+        top = max(top, p.top());
     }
     top = __reduce_max_sync(0xffffffffu, top);
     if ((threadIdx.x & 31) == 0) tops[threadIdx.x >> 5] = top;
@@ -92,18 +133,19 @@ quantize_rows_kernel(const T* __restrict__ x, long long ldx, int8_t* __restrict_
     else inv = __frcp_rn(s);
     if (threadIdx.x == 0) scale[blockIdx.x] = s;
     int8_t* out = q + (size_t)blockIdx.x * ldq;
-    for (int k = threadIdx.x * 8, i = 0; k < K; k += kThreads * 8, ++i) {
-        float t[8];
-        if (i < kHeld) {
+    float v[8];
 #pragma unroll
-            for (int u = 0; u < kHeld; ++u)
-                if (u == i)
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) t[j] = v[u][j];
-        } else {
-            load_piece(row, k, K, wide, t);
-        }
-        store_piece(out, k, K, t, s, inv);
+    for (int u = 0; u < kHeld; ++u) {
+        const int k = (u * kThreads + threadIdx.x) * 8;
+        if (k >= K) break;
+        held[u].floats(v);
+        store_piece(out, k, K, v, s, inv);
+    }
+    for (int k = (kHeld * kThreads + threadIdx.x) * 8; k < K; k += kThreads * 8) {
+        Piece<T> p;
+        load_piece(p, row, k, K, wide);
+        p.floats(v);
+        store_piece(out, k, K, v, s, inv);
     }
 }
 
