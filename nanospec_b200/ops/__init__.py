@@ -33,7 +33,7 @@ def _stream() -> int:
     """The current CUDA stream of the current device, as the integer that the C ABI takes (asked for
     at every launch, so that stream contexts and graph captures are followed)."""
     if _raw_stream is not None:
-        return _raw_stream(torch.cuda.current_device())
+        return _raw_stream(torch.cuda.current_device() if _current_device is None else _current_device())
     return torch.cuda.current_stream().cuda_stream
 
 
@@ -43,6 +43,9 @@ def _cuda(*tensors: torch.Tensor | None) -> None:
             raise KernelError("kernel operands must live on a CUDA device; there is no CPU path")
 
 
+_current_device = getattr(torch._C, "_cuda_getDevice", None)  # the number alone
+
+
 def _on_current_device(*tensors: torch.Tensor | None) -> None:
     """Operands of one launch: all on the current CUDA device, whose current stream the kernels go to."""
     dev = None
@@ -50,10 +53,11 @@ def _on_current_device(*tensors: torch.Tensor | None) -> None:
         if t is None:
             continue
         at = t.get_device()  # (-1: not on a CUDA device)
-        if at < 0:
-            _cuda(t)
+        if at == dev:
+            continue
+        _cuda(t)
         if dev is None:
-            dev = torch.cuda.current_device()
+            dev = torch.cuda.current_device() if _current_device is None else _current_device()
         if at != dev:
             raise KernelError(f"an operand lies on {t.device}, the current device is cuda:{dev}")
 
@@ -177,7 +181,7 @@ _sm_counts: dict[int, int] = {}
 def sm_count() -> int:
     """Streaming multiprocessors of the current device (148 on a B200): the one place the launch heuristics
     below take the size of the chip from."""
-    dev = torch.cuda.current_device()
+    dev = torch.cuda.current_device() if _current_device is None else _current_device()
     n = _sm_counts.get(dev)
     if n is None:
         n = _sm_counts[dev] = torch.cuda.get_device_properties(dev).multi_processor_count
@@ -1950,5 +1954,7 @@ def head_prepare_store(proj: torch.Tensor, out: torch.Tensor, ctx, lane, nq: int
                  ctx.state_slot.data_ptr(), cols, n_taps, ctx.n_requests, dtype_code(proj.dtype), _stream())
 
 
-from .int8 import I8_MAX_K, RowsI8, linear_i8, quantize_rows  # noqa: E402,F401
-from .kv4 import KV4_GROUP, attention_kv4, kv4_block_bytes, kv4_pages, kv4_read, kv4_store  # noqa: E402,F401
+from .int8 import I8_MAX_K, RowsI8, i8_tiles, linear_i8, quantize_rows  # noqa: E402,F401
+from .kv4 import (  # noqa: E402,F401
+    KV4_GROUP, KV4_UNFOLD_PAGE, attention_kv4, kv4_block_bytes, kv4_pages, kv4_read, kv4_shape, kv4_store, kv4_token_tiles, kv4_unfold_runs, kv4_unfolded,
+)

@@ -33,10 +33,11 @@ class RowsI8:
 def _check_rows(r: RowsI8, name: str) -> int:
     """Elements from one row to the next."""
     q, scale = r.q, r.scale
-    if q.dtype != torch.int8 or q.dim() != 2 or scale.dtype != torch.float32 or scale.shape != q.shape[:1] or not scale.is_contiguous():
+    shape = q.shape
+    if q.dtype is not torch.int8 or len(shape) != 2 or scale.dtype is not torch.float32 or scale.shape != shape[:1] or not scale.is_contiguous():
         raise KernelError(f"linear_i8: {name} must be int8 [R, K] with one contiguous float32 scale per row")
     step, inner = q.stride()
-    if q.numel() and (inner != 1 or step % 16 or q.data_ptr() % 16):
+    if shape[0] and (inner != 1 or step & 15 or q.data_ptr() & 15):
         raise KernelError(f"linear_i8: the rows of {name} must start on 16-byte boundaries with unit inner stride (quantize_rows makes them so)")
     return step
 
@@ -97,26 +98,29 @@ def linear_i8(x: torch.Tensor | RowsI8, w: RowsI8, out: torch.Tensor, bias: torc
     with unit inner stride."""
     ready = isinstance(x, RowsI8)
     held, wq, ws = x.q if ready else x, w.q, w.scale
-    _on_current_device(held, wq, ws, out, bias, x.scale if ready else None)
-    ldw = _check_rows(w, "w")
     if ready:
-        _check_rows(x, "x")
+        _on_current_device(held, x.scale, wq, ws, out, bias)
+        ldx = _check_rows(x, "x")
+    else:
+        _on_current_device(held, wq, ws, out, bias)
+        ldx = 0
+    ldw = _check_rows(w, "w")
     F, K = wq.shape
-    shape, (ldo, inner) = held.shape, out.stride() if out.dim() == 2 else (0, 0)
-    if len(shape) != 2 or shape[1] != K or not 1 <= K <= I8_MAX_K or (shape[0] and held.stride(1) != 1):
+    shape, steps, ldo = held.shape, held.stride(), out.stride()
+    if len(shape) != 2 or shape[1] != K or not 1 <= K <= I8_MAX_K or (steps[1] != 1 and shape[0]):
         raise KernelError(f"linear_i8: x {tuple(shape)} with unit inner stride and w {tuple(wq.shape)} must agree on K, which is {I8_MAX_K} at most")
     N = shape[0]
-    if out.shape != (N, F) or (N and F and inner != 1):
-        raise KernelError(f"linear_i8: out must be [{N}, {F}] with unit inner stride, not {tuple(out.shape)} with strides {out.stride()}")
+    if out.shape != (N, F) or (ldo[1] != 1 and N and F):
+        raise KernelError(f"linear_i8: out must be [{N}, {F}] with unit inner stride, not {tuple(out.shape)} with strides {ldo}")
     if bias is not None and (bias.dtype != torch.float32 or bias.shape != (F,) or not bias.is_contiguous()):
         raise KernelError("linear_i8: the bias is one contiguous float32 number per output feature")
     code, sms, dev = dtype_code(out.dtype), sm_count(), out.device
     tile, features, splits = tiles or i8_tiles(N, F, K, sms)
     if ready:
-        lib.call("ns_gemm_i8", held.data_ptr(), held.stride(0), x.scale.data_ptr(), wq.data_ptr(), ldw, ws.data_ptr(), _ptr(bias), out.data_ptr(), ldo, N, F, K,
+        lib.call("ns_gemm_i8", held.data_ptr(), ldx, x.scale.data_ptr(), wq.data_ptr(), ldw, ws.data_ptr(), _ptr(bias), out.data_ptr(), ldo[0], N, F, K,
                  code, tile, features, splits, 0, sms, _tc(dev).error.data_ptr(), _stream())
     else:
-        scratch = torch.empty(N * (-(-K // 16) * 16 + 4), dtype=torch.int8, device=dev)
-        lib.call("ns_linear_i8", held.data_ptr(), held.stride(0), dtype_code(held.dtype), scratch.data_ptr(), wq.data_ptr(), ldw, ws.data_ptr(), _ptr(bias),
-                 out.data_ptr(), ldo, N, F, K, code, tile, features, splits, sms, _tc(dev).error.data_ptr(), _stream())
+        scratch = torch.empty(N * (((K + 15) & -16) + 4), dtype=torch.int8, device=dev)
+        lib.call("ns_linear_i8", held.data_ptr(), steps[0], dtype_code(held.dtype), scratch.data_ptr(), wq.data_ptr(), ldw, ws.data_ptr(), _ptr(bias),
+                 out.data_ptr(), ldo[0], N, F, K, code, tile, features, splits, sms, _tc(dev).error.data_ptr(), _stream())
     return out

@@ -3,6 +3,7 @@ are then uint8 [pages, kv heads, page_size * head_dim * 5 / 8] (`kv4_pages`); cs
 
 from __future__ import annotations
 
+import functools
 import math
 from dataclasses import dataclass
 
@@ -15,6 +16,7 @@ KV4_GROUP = 32  # features that share a pair of numbers
 KV4_MAX_HEAD = 256
 
 
+@functools.lru_cache(maxsize=256)
 def kv4_block_bytes(page_size: int, head_dim: int) -> int:
     """Bytes of a page of one kv head (of keys, and as many of values): half a byte a feature and 4 bytes a group of 32."""
     if head_dim % KV4_GROUP or not KV4_GROUP <= head_dim <= KV4_MAX_HEAD or page_size < 1:
@@ -30,10 +32,10 @@ def kv4_pages(pages: int, kv_heads: int, page_size: int, head_dim: int, device: 
 def _check_lane(who: str, lane, nkv: int, head_dim: int) -> None:
     k, v, table = lane.k, lane.v, lane.block_table
     size = kv4_block_bytes(lane.page_size, head_dim)
-    if k is None or v is None or k.dtype != torch.uint8 or v.dtype != torch.uint8 or k.shape != v.shape or k.dim() != 3 or k.shape[1:] != (nkv, size) \
-            or not k.is_contiguous() or not v.is_contiguous() or (k.data_ptr() | v.data_ptr()) % 16:
+    if k is None or v is None or k.dtype is not torch.uint8 or v.dtype is not torch.uint8 or k.shape != v.shape or k.shape[1:] != (nkv, size) \
+            or not k.is_contiguous() or not v.is_contiguous() or (k.data_ptr() | v.data_ptr()) & 15:
         raise KernelError(f"{who}: the lane's pages must be contiguous uint8 [pages, {nkv}, {size}] on 16-byte boundaries (kv4_pages makes them)")
-    if table is None or table.dtype != torch.int32 or table.dim() != 2 or table.stride(1) != 1:
+    if table is None or table.dtype is not torch.int32 or table.dim() != 2 or table.stride()[1] != 1:
         raise KernelError(f"{who}: block_table must be int32 [requests, pages] with unit inner stride")
 
 
@@ -239,20 +241,22 @@ def attention_kv4(qkv: torch.Tensor, lane, ctx, out: torch.Tensor, nq: int, nkv:
     throughout (csrc/attention_kv4.cu)."""
     _on_current_device(qkv, out, lane.k, lane.v, lane.block_table, ctx.positions, ctx.token_req, sink)
     _check_lane("attention_kv4", lane, nkv, head_dim)
+    if qkv.dim() != 2 or out.dim() != 2:
+        raise KernelError("attention_kv4: q and out are matrices, a row to a token")
     n = out.shape[0]
     code = dtype_code(qkv.dtype)
     _check_step("attention_kv4", ctx.positions, ctx.token_req, n)
     if nq < 1 or nq % nkv or window < 0:
         raise KernelError(f"attention_kv4: {nq} query heads over {nkv}, a window of {window}")
-    if qkv.dim() != 2 or qkv.shape[0] != n or qkv.shape[1] < nq * head_dim or out.shape != (n, nq * head_dim) or out.dtype != qkv.dtype \
-            or (n and (qkv.stride(1) != 1 or out.stride(1) != 1)):
+    (ldq, inner), (ldo, inner_o) = qkv.stride(), out.stride()
+    if qkv.shape[0] != n or qkv.shape[1] < nq * head_dim or out.shape != (n, nq * head_dim) or out.dtype != qkv.dtype or (n and (inner != 1 or inner_o != 1)):
         raise KernelError(f"attention_kv4: q [N, >= {nq * head_dim}] and out [N, {nq * head_dim}] in one type with unit inner strides are needed")
     if sink is not None and (sink.dtype != torch.float32 or sink.numel() != nq or not sink.is_contiguous()):
         raise KernelError("attention_kv4: the sink is one contiguous float32 number per query head")
     scale = 1.0 / math.sqrt(head_dim) if scale is None else float(scale)
-    group, sms, window = nq // nkv, sm_count(), int(window)
+    group, sms, window = nq // nkv, sm_count(), min(int(window), 1 << 30)
     tensor_core = kv4_tensor_core_ok(qkv.dtype, head_dim, lane.page_size)
-    unfold = code == BF16 and head_dim <= 128 and qkv.stride(0) % 8 == 0 and out.stride(0) % 2 == 0 and qkv.data_ptr() % 16 == 0 and out.data_ptr() % 4 == 0
+    unfold = code == BF16 and head_dim <= 128 and ldq % 8 == 0 and ldo % 2 == 0 and qkv.data_ptr() % 16 == 0 and out.data_ptr() % 4 == 0
     plan = _kv4_plan(ctx, group, nkv, head_dim, window, tensor_core, unfold)
     if plan["n_rows"] and not tensor_core:
         longest, splits = plan["longest"], 1
@@ -274,7 +278,18 @@ def attention_kv4(qkv: torch.Tensor, lane, ctx, out: torch.Tensor, nq: int, nkv:
     return out
 
 
+KV4_GRID_MAX = 65535  # rows, or tiles, of one launch
+
+
 def _attend_tokens(qkv, lane, ctx, out, nq, nkv, head_dim, scale, window, sink, sms, rows, items, count, longest, blocks) -> None:
+    if count > KV4_GRID_MAX:
+        if items is None and rows is None:
+            rows = torch.arange(count, dtype=torch.int32, device=out.device)
+        for at in range(0, count, KV4_GRID_MAX):
+            part = slice(at, min(count, at + KV4_GRID_MAX))
+            _attend_tokens(qkv, lane, ctx, out, nq, nkv, head_dim, scale, window, sink, sms, None if rows is None else rows[part],
+                           None if items is None else items[part], part.stop - at, longest, blocks)
+        return
     if window and longest is not None:
         longest = min(longest, window + KV4_TILE)
     warps, splits = kv4_shape(count * nkv * -(-(nq // nkv) // (8 * blocks)), longest, sms)

@@ -42,3 +42,57 @@ def test_the_plain_statement_of_four_bits():
         assert to_bf16(torch.tensor([v], dtype=torch.float64)).item() == want
     q, s = rows_i8(torch.tensor([[127.0, 0.5, 1.5, -2.5], [0.0, 0.0, 0.0, 0.0]]))
     assert q.tolist() == [[127, 0, 2, -2], [0, 0, 0, 0]] and s.tolist() == [1.0, 0.0]
+
+
+@pytest.mark.parametrize("M,N,K,tile", [
+    (1, 2048, 2048, (16, 128, 8)), (8, 28672, 4096, (16, 128, 1)), (8, 4096, 14336, (16, 128, 8)), (32, 4096, 4096, (32, 128, 4)), (64, 28672, 4096, (64, 128, 1)),
+    (77, 1003, 2051, (128, 128, 8)), (128, 28672, 4096, (256, 256, 1)), (200, 4096, 4096, (256, 64, 1)), (256, 4096, 14336, (256, 128, 2)),
+    (512, 4096, 14336, (256, 256, 2)), (512, 6144, 4096, (256, 192, 1)), (4096, 28672, 4096, (256, 256, 1)), (5, 10, 1, (16, 128, 1)), (500, 10, 1, (256, 64, 1)),
+])
+def test_tiles_of_products(M, N, K, tile):
+    """The fastest of those measured, at sizes on both sides of every border."""
+    from nanospec_b200 import ops
+    assert ops.i8_tiles(M, N, K, 148) == tile
+
+
+@pytest.mark.parametrize("requests,group,nkv,dim,unfolded", [
+    # from the bytes, unfolded (us)
+    ([(64, 30064)], 4, 8, 128, False),             # 202, 328
+    ([(24, 3024)] * 8, 4, 8, 128, False),          # 74, 104
+    ([(64, 3064)] * 8, 4, 8, 128, True),           # 166, 106
+    ([(24, 1024)] * 32, 4, 8, 128, False),         # 113, 143
+    ([(48, 1048)] * 32, 4, 8, 128, True),          # 203, 154
+    ([(64, 564)] * 8, 4, 8, 128, True),            # 61, 35
+    ([(16, 516)] * 8, 4, 8, 128, False),           # 23, 33
+    ([(24, 3024)] * 8, 8, 8, 128, False),          # 135, 172
+    ([(48, 3048)] * 8, 8, 8, 128, True),           # 240, 175
+    ([(1, 5000)] * 4, 4, 8, 128, False),           # nothing but decoding
+    ([(2, 100), (512, 3512)], 4, 8, 128, True),
+])
+def test_which_portions_are_unfolded(requests, group, nkv, dim, unfolded):
+    from nanospec_b200 import ops
+    got = ops.kv4_unfolded(requests, group, nkv, dim, 0, 148, True)
+    assert bool(got) == unfolded
+    if unfolded:
+        assert got == [i for i, (n, _) in enumerate(requests) if n > 2]
+
+
+def test_runs_of_what_is_unfolded():
+    from nanospec_b200 import ops
+    one = ops.KV4_UNFOLD_PAGE * 128 * 4
+    runs = lambda chunks, limit: ops.kv4_unfold_runs(chunks, 4, 128, limit * one)  # noqa: E731
+    assert runs([3, 4, 5], 48) == [(0, 3, 0, 4)]
+    assert runs([3, 4, 5], 28) == [(0, 2, 0, 4), (2, 1, 0, 4)]
+    assert runs([3, 40, 5], 80) == [(0, 1, 0, 4), (1, 1, 0, 2), (1, 1, 2, 2), (2, 1, 0, 4)]
+    assert runs([40], 1) == [(0, 1, h, 1) for h in range(4)]
+    assert runs([], 10) == []
+
+
+def test_tiles_of_a_few_tokens():
+    from nanospec_b200 import ops
+    assert ops.kv4_token_tiles([(0, 2, 9), (5, 6, 9)], 4) == ([(0, 2), (5, 4), (9, 2)], 2)
+    assert ops.kv4_token_tiles([(3, 2, 9)], 4) == ([(3, 2)], 1)
+    assert ops.kv4_token_tiles([(0, 3, 9)], 20) == ([(0, 1), (1, 1), (2, 1)], 2)
+    for blocks, longest in ((1, 1), (8, 1000), (512, 2300), (16, 100000), (8, None), (100000, 5)):
+        warps, splits = ops.kv4_shape(blocks, longest, 148)
+        assert warps in (4, 8) and splits in (1, 2, 4, 8, 16) and (splits == 1 or longest is None or longest > 16 * warps * splits)

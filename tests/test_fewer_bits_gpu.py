@@ -133,6 +133,36 @@ def test_product_with_strides_and_what_lies_beside(M):
         assert (buf[0] == 7).all() and (buf[-1] == 7).all() and (buf[:, :off] == 7).all() and (buf[:, off + N:] == 7).all()
 
 
+@pytest.mark.parametrize("M,N,K", [(200, 300, 520), (300, 129, 2051), (40, 770, 1000)])
+def test_product_has_the_same_bits_in_every_tile(M, N, K):
+    from nanospec_b200 import ops
+    x, w, bias = ops.quantize_rows(_rand(M, K, seed=1)), ops.quantize_rows(_rand(N, K, seed=2)), _rand(N, seed=3)
+    tiles = [(t, 128, s) for t in (16, 32, 64, 128) for s in (1, 2, 4)] + [(256, f, s) for f in (64, 128, 192, 256) for s in (1, 2)]
+    outs = [ops.linear_i8(x, w, torch.empty((M, N), device="cuda"), bias, t) for t in tiles]
+    assert all(torch.equal(outs[0], o) for o in outs)
+    ops.check_kernel_errors()
+
+
+def test_weights_quantised_directly_before_the_product():
+    """The product asks for its weights ahead of its turn: not before the kernel that writes them is through."""
+    from nanospec_b200 import ops
+    x = _rand(8, 4096, seed=1, dtype=BF16)
+    raw = [_rand(8192, 4096, seed=s) for s in (2, 3)]
+    want = []
+    for r in raw:
+        w = ops.quantize_rows(r)
+        torch.cuda.synchronize()
+        want.append(ops.linear_i8(x, w, torch.empty((8, 8192), device="cuda")))
+    torch.cuda.synchronize()
+    held = ops.quantize_rows(raw[0])
+    for i in range(20):
+        new = ops.quantize_rows(raw[i % 2])
+        held.q.copy_(new.q), held.scale.copy_(new.scale)
+        assert torch.equal(ops.linear_i8(x, ops.quantize_rows(raw[i % 2]), torch.empty((8, 8192), device="cuda")), want[i % 2])
+        assert torch.equal(ops.linear_i8(x, held, torch.empty((8, 8192), device="cuda")), want[i % 2])
+        assert torch.equal(ops.linear_i8(ops.quantize_rows(x), ops.quantize_rows(raw[i % 2]), torch.empty((8, 8192), device="cuda")), want[i % 2])
+
+
 def test_product_keeps_what_is_not_finite_in_its_row():
     from nanospec_b200 import ops
     for M in (4, 90, 300):
@@ -324,6 +354,82 @@ def test_windows(window, dim, dtype):
 @pytest.mark.parametrize("nq,nkv,dim,page", [(32, 8, 128, 16), (8, 2, 64, 16), (5, 5, 128, 32), (9, 1, 64, 8)])
 def test_portions(lens, nq, nkv, dim, page):
     _check(lens, page, nq, nkv, dim)
+
+
+@pytest.mark.parametrize("nq,nkv,dim,page,dtype", [(32, 8, 128, 16, BF16), (16, 2, 64, 8, BF16), (6, 2, 96, 16, BF16), (8, 4, 256, 32, BF16), (4, 2, 64, 16, F32)])
+def test_steps_of_every_kind_of_request(nq, nkv, dim, page, dtype):
+    """Single tokens, a few tokens, portions and requests that bring none in one step."""
+    _check([(500, 1), (0, 200), (90, 3), (1200, 300), (3, 1), (40, 17), (0, 1), (300, 2)], page, nq, nkv, dim, dtype, padding=3)
+    _check([(500, 1), (20, 200), (90, 3), (1200, 300), (3, 1)], page, nq, nkv, dim, dtype, window=150)
+
+
+@pytest.mark.parametrize("lens", [[(900, 1), (300, 1)], [(900, 3), (20, 2)], [(900, 80), (10, 200)]])
+@pytest.mark.parametrize("dim,page,dtype", [(128, 16, BF16), (64, 8, BF16), (128, 32, BF16), (128, 5, BF16), (64, 16, F32)])
+def test_pages_behind_a_window_may_be_given_back(lens, dim, page, dtype):
+    """Their table entries are then -1, and the pages hold somebody else's bytes, NaN among what those stand for."""
+    from nanospec_b200 import ops
+    window = 100
+    ctx, lane, qkv = step(lens, page, 2, dim, dtype, 4)
+    k, v = fill(ctx, lane, 4, 2, dim, dtype)
+    for i, (held, _) in enumerate(lens):
+        gone = max(0, held - window + 1) // page
+        lane.k[lane.block_table[i, :gone].long()] = 255
+        lane.v[lane.block_table[i, :gone].long()] = 255
+        lane.block_table[i, :gone] = -1
+    out = torch.empty((ctx.n_tokens, 4 * dim), dtype=dtype, device="cuda")
+    ops.attention_kv4(qkv, lane, ctx, out, 4, 2, dim, window=window)
+    want, tol8, tol32 = attend(qkv[:, : 4 * dim], k, v, ctx, 4, dim ** -0.5, window)
+    _near(out, want, (tol32 if dtype == F32 else tol8) + want.abs() * 1.01 * half_step(dtype))
+
+
+def test_portions_beyond_what_is_unfolded_at_a_time(monkeypatch):
+    """Requests one after another, and a request whose kv heads go in parts: the same bits as together."""
+    from nanospec_b200 import ops
+    from nanospec_b200.ops import kv4
+    ctx, lane, qkv = step([(0, 200), (700, 100), (64, 300), (10, 1)], 16, 4, 128, BF16, 8)
+    fill(ctx, lane, 8, 4, 128)
+    sink = _rand(8, seed=4)
+    monkeypatch.setattr(kv4, "kv4_unfolded", lambda requests, *a: [i for i, (n, _) in enumerate(requests) if n > 1])
+    want = ops.attention_kv4(qkv, lane, ctx, torch.zeros((ctx.n_tokens, 1024), dtype=BF16, device="cuda"), 8, 4, 128, sink=sink)
+    one = kv4.KV4_UNFOLD_PAGE * 128 * 4
+    for limit in (13 * 4 * one, 10 * 2 * one, one):
+        monkeypatch.setattr(kv4, "KV4_UNFOLD_MAX", limit)
+        ctx.extras = {}
+        got = ops.attention_kv4(qkv, lane, ctx, torch.zeros_like(want), 8, 4, 128, sink=sink)
+        assert torch.equal(got, want)
+
+
+def test_more_rows_than_a_grid_holds(monkeypatch):
+    from nanospec_b200 import ops
+    from nanospec_b200.ops import kv4
+    for lens in ([(i, 1) for i in range(40)], [(i, 3) for i in range(20)]):
+        ctx, lane, qkv = step(lens, 16, 2, 64, BF16, 4)
+        fill(ctx, lane, 4, 2, 64)
+        monkeypatch.setattr(kv4, "KV4_GRID_MAX", 65535)
+        monkeypatch.setattr(kv4, "kv4_shape", lambda *a: (4, 2))
+        want = ops.attention_kv4(qkv, lane, ctx, torch.zeros((ctx.n_tokens, 256), dtype=BF16, device="cuda"), 4, 2, 64)
+        monkeypatch.setattr(kv4, "KV4_GRID_MAX", 7)
+        got = ops.attention_kv4(qkv, lane, ctx, torch.zeros_like(want), 4, 2, 64)
+        assert torch.equal(got, want)
+
+
+def test_two_calls_at_once():
+    """The same cache read by two streams, and products of two streams: no scratch is shared."""
+    from nanospec_b200 import ops
+    ctx, lane, qkv = step([(700, 1), (90, 5), (30, 120)], 16, 2, 128, BF16, 8)
+    fill(ctx, lane, 8, 2, 128)
+    x, w = _rand(90, 1024, dtype=BF16), ops.quantize_rows(_rand(1024, 1024, seed=2))
+    want = ops.attention_kv4(qkv, lane, ctx, torch.zeros((ctx.n_tokens, 1024), dtype=BF16, device="cuda"), 8, 2, 128)
+    product = ops.linear_i8(x, w, torch.empty((90, 1024), dtype=BF16, device="cuda"))
+    torch.cuda.synchronize()
+    streams, results = [torch.cuda.Stream() for _ in range(3)], []
+    for _ in range(5):
+        for s in streams:
+            with torch.cuda.stream(s):
+                results.append((ops.attention_kv4(qkv, lane, ctx, torch.zeros_like(want), 8, 2, 128), ops.linear_i8(x, w, torch.empty_like(product))))
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, want) and torch.equal(b, product) for a, b in results)
+    ops.check_kernel_errors()
 
 
 @pytest.mark.parametrize("lens", [[(300, 1), (9, 1)], [(200, 3)], [(40, 90)]])
