@@ -92,11 +92,14 @@ def kv4_tensor_core_ok(dtype: torch.dtype, head_dim: int, page_size: int) -> boo
     return dtype == torch.bfloat16 and head_dim in (64, 128, 256) and (page_size in (8, 16) or page_size % 32 == 0)
 
 
-def kv4_shape(blocks: int, longest: int | None, sms: int) -> tuple[int, int]:
-    """(warps of a block, blocks of a cluster) that share a request's keys."""
+def kv4_shape(blocks: int, longest: int | None, sms: int, resident: int = 16) -> tuple[int, int]:
+    """(warps of a block, blocks of a cluster) that share a request's keys; `resident`: warps that an SM holds.  While blocks fill the SMs, four warps a block and
+    one block a request (64 requests of 8 kv heads on up to 2,300 positions: 45 us, with two blocks each 49); else eight, and blocks until the SMs are full, but a
+    tile of keys to every warp (one request on 1,000 positions: one block of eight 12.3 us, four 10.2, sixteen 12.3; two on 100,000: four 152, sixteen 72).
+    Clusters of sixteen blocks that take an SM each do not all find a place."""
     warps = 4 if blocks >= 2 * sms else 8
-    splits = 1
-    while splits < 16 and blocks * splits * 2 <= sms * 16 // warps and (longest is None or longest > KV4_TILE * warps * splits):
+    splits, most = 1, 16 if resident >= 16 else 8
+    while splits < most and blocks * splits * 2 <= sms * resident // warps and (longest is None or longest > KV4_TILE * warps * splits):
         splits *= 2
     return warps, splits
 
@@ -292,7 +295,7 @@ def _attend_tokens(qkv, lane, ctx, out, nq, nkv, head_dim, scale, window, sink, 
         return
     if window and longest is not None:
         longest = min(longest, window + KV4_TILE)
-    warps, splits = kv4_shape(count * nkv * -(-(nq // nkv) // (8 * blocks)), longest, sms)
+    warps, splits = kv4_shape(count * nkv * -(-(nq // nkv) // (8 * blocks)), longest, sms, 8 if head_dim > 128 else 16)
     lib.call("ns_attention_kv4_tc", qkv.data_ptr(), qkv.stride(0), lane.k.data_ptr(), lane.v.data_ptr(), lane.block_table.data_ptr(),
              lane.block_table.stride(0), ctx.token_req.data_ptr(), ctx.positions.data_ptr(), _ptr(rows), _ptr(items), count, out.data_ptr(), out.stride(0), nq,
              nkv, head_dim, lane.page_size, scale, window, _ptr(sink), blocks, warps, splits, _stream())

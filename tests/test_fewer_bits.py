@@ -96,3 +96,4 @@ def test_tiles_of_a_few_tokens():
     for blocks, longest in ((1, 1), (8, 1000), (512, 2300), (16, 100000), (8, None), (100000, 5)):
         warps, splits = ops.kv4_shape(blocks, longest, 148)
         assert warps in (4, 8) and splits in (1, 2, 4, 8, 16) and (splits == 1 or longest is None or longest > 16 * warps * splits)
+        assert ops.kv4_shape(blocks, longest, 148, 8)[1] <= 8
