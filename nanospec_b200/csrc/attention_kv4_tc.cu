@@ -91,7 +91,7 @@ attention_kv4_tc_kernel(const __nv_bfloat16* __restrict__ q, long long ldq, cons
     const int step = splits * kWarps, first = (int)blockIdx.x * kWarps + warp;
 
     // a tile: 16-byte pieces, codes and pairs of keys and of values, from the pages that it lies in (1, 2 or 4)
-    const int page_log = 31 - __clz(min(kTile, page_size)), pages = kTile >> page_log;  // keys of a page in a tile
+    const int page_log = kPages == 1 ? 5 : kPages == 2 ? 4 : 31 - __clz(min(kTile, page_size)), pages = kTile >> page_log;  // keys of a page in a tile
     const unsigned block_bytes = (unsigned)kv4_block_bytes(page_size, D);
     // Where the blocks of a tile begin, or -1 (the table is read a tile ahead: its latency would stand before every copy): each lane knows the one or two,
     // or lane i the i-th of more.
