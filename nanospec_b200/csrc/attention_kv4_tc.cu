@@ -9,12 +9,19 @@
 //     the scores' layout into the right operand's by one 8 x 8 transposition of 16-bit numbers in registers.
 // Rows of the score tile are dealt to keys (key_of_row) such that both sides' reads of shared memory spread over the banks.
 //
-// Every warp is on its own: it takes every (warps of the cluster)-th tile of 32 keys, brings it in 16-byte pieces into its own ring (bulk copies, a lane each for the codes and pairs of a page, took as
-// long as the tile's arithmetic: their addresses are not a warp's but a lane's), and keeps its own maximum, sum and output; the block's warps, then the cluster's blocks are
-// joined at the end in a fixed order.  The running maximum moves only when a score exceeds it by more than 2^8 (weights are then at most 256,
-// far from any limit of float or bfloat16); the common tile costs a vote.
+// Every warp is on its own: it takes every (warps of the request's blocks)-th tile of 32 keys, brings it in 16-byte pieces into its own ring (bulk copies, a
+// lane each for the codes and pairs of a page, took as long as the tile's arithmetic: their addresses are not a warp's but a lane's), and keeps its own maximum,
+// sum and output; the block's warps are joined at its end in a fixed order.  A request that has several blocks leaves their parts in a workspace, which a second
+// kernel joins in a fixed order too: blocks of one size then fill the SMs whatever the requests' lengths are (a cluster that joins its blocks over distributed shared
+// memory ends at sixteen and leaves the SMs beyond its own idle: one request on 100,000 keys took 72 us so, 47 now).  The running maximum moves only when a score
+// exceeds it by more than 2^8 (weights are then at most 256, far from any limit of float or bfloat16); the common tile costs a vote.
 //
 // The weights meet the values as bfloat16, as in the attention over a bfloat16 cache; sums, maximum and outputs are float.
+//
+// Bound by the SMs' integer pipe, not by memory: 384 of a tile's about 690 instructions a warp (heads of 128) make values of codes, more than half of those in the logic
+// pipe, which issues every second cycle and is busy for 60 % of 1,160 cycles a tile and scheduler; the rest is four warps a scheduler that wait for it or for
+// one another's turn.  74 requests on 4,096 keys of 8 kv heads: 86 us (pages of 64 tokens; 94 of 16), 4.5 TB/s, the same where all requests read the same
+// page.  The ragged 64 on up to 2,300 keys, 111 MB: 43 us; 2 on 100,000, 170 MB: 53 us.
 #include "kv4.cuh"
 #include "mma_utils.cuh"
 #include "tcgen05_utils.cuh"
@@ -49,7 +56,8 @@ __device__ __forceinline__ void lds(uint32_t (&v)[N], const unsigned char* p) {
 
 template <int D, int NB, int kWarps>
 struct Shape {
-    static constexpr int kThreads = 32 * kWarps, kResident = D > 128 ? 8 / kWarps : NB == 2 && kWarps == 4 ? 3 : 16 / kWarps;  // blocks an SM
+    static constexpr int kThreads = 32 * kWarps, kResident = D > 128 ? 8 / kWarps : kWarps == 8 ? 2 : NB == 2 ? 3 : D == 64 ? 6 : 4;  // blocks an SM (185 requests on
+    // 1,023 keys, heads of 64: four 52 us, six 49; of 128, whose registers would do for five, no gain)
     static constexpr int kCols = 8 * NB, kWords = D / 32, kVWords = D / 64, kBlocks = D / 16;  // words of a lane per key; m-blocks of features
     static constexpr int kCodes = kTile * D / 2, kPairs = kTile * D / 8, kStage = 2 * (kCodes + kPairs);
     static constexpr int kRing = kStages * kStage;
@@ -58,14 +66,32 @@ struct Shape {
     static constexpr size_t kSmem = (size_t)kWarps * kRing + kQBytes;
 };
 
-// tokens: `items` [n, 2] = (first row, tokens), rows `rows` [n] of one token each, or row blockIdx.z
+// What a block, or all blocks of a (row, kv head), have in common.  tokens: `items` [n, 2] = (first row, tokens), rows `rows` [n] of one token each, or row z.
+struct Place {
+    int n0, count, req, pos0, hk, h0, heads, cols, end, start, tile0, tiles;
+    __device__ __forceinline__ Place(int z, int y, const int* items, const int* rows, const int* token_req, const int* positions, int nq, int nkv, int head_tiles,
+                                     int kCols, int window) {
+        n0 = items ? items[2 * z] : rows ? rows[z] : z, count = items ? items[2 * z + 1] : 1;
+        req = token_req[n0], pos0 = positions[n0];
+        const int G = nq / nkv, ht = y % head_tiles, per = min(G, kCols);
+        hk = y / head_tiles, h0 = hk * G + ht * per, heads = min(per, hk * G + G - h0);  // heads of a token here
+        cols = count * heads;
+        end = pos0 + count;  // keys below `end` are seen by some column
+        start = window > 0 ? max(0, pos0 - window + 1) : 0;
+        tile0 = start / kTile, tiles = (end + kTile - 1) / kTile - tile0;
+    }
+    __device__ __forceinline__ int parts(int most, int least) const { return max(1, min(most, (tiles + least - 1) / least)); }  // blocks, of `least` tiles or more each
+};
+// A warp's part of a column, or a block's: 2^(its maximum - the whole's); one that saw no key adds nothing, one whose scores are all NaN makes the column NaN.
+__device__ __forceinline__ float share(float m_part, float l_part, float top) { return m_part == -INFINITY ? 0.f * l_part : ns_exp2(m_part - top); }
+
 // kPages: pages of a tile, 1 or 2 (whole or half tiles in a page), or 0: by page_size
 template <int D, int NB, int kWarps, int kPages>
 __global__ void __launch_bounds__(32 * kWarps, Shape<D, NB, kWarps>::kResident)
 attention_kv4_tc_kernel(const __nv_bfloat16* __restrict__ q, long long ldq, const uint8_t* __restrict__ k_pages, const uint8_t* __restrict__ v_pages,
                         const int* __restrict__ block_table, int table_stride, const int* __restrict__ token_req, const int* __restrict__ positions,
                         const int* __restrict__ rows, const int* __restrict__ items, __nv_bfloat16* __restrict__ out, long long ldo, int nq, int nkv,
-                        int page_size, float scale, int window, const float* __restrict__ sink, int head_tiles, int splits, int page_shift) {
+                        int page_size, float scale, int window, const float* __restrict__ sink, int head_tiles, int splits, int page_shift, float* __restrict__ part, int least) {
     using S = Shape<D, NB, kWarps>;
     constexpr int kThreads = S::kThreads;
     extern __shared__ __align__(128) unsigned char smem[];
@@ -77,18 +103,13 @@ attention_kv4_tc_kernel(const __nv_bfloat16* __restrict__ q, long long ldq, cons
     ns_pdl_launch_dependents();
     ns_pdl_wait();
 
-    const int z = blockIdx.z;
-    const int n0 = items ? items[2 * z] : rows ? rows[z] : z, count = items ? items[2 * z + 1] : 1;
-    const int req = token_req[n0], pos0 = positions[n0];
-    if (req < 0) return;  // a row of padding (all blocks of its cluster leave)
-    const int G = nq / nkv, hk = blockIdx.y / head_tiles, ht = blockIdx.y % head_tiles;
-    const int per = min(G, S::kCols), h0 = hk * G + ht * per, heads = min(per, hk * G + G - h0);  // heads of a token here
-    const int cols = count * heads;
-    const int end = pos0 + count;  // keys below `end` are seen by some column
-    const int start = window > 0 ? max(0, pos0 - window + 1) : 0;
-    const int tile0 = start / kTile, tiles = (end + kTile - 1) / kTile - tile0;
-    const int* bt = block_table + (size_t)req * table_stride;
-    const int step = splits * kWarps, first = (int)blockIdx.x * kWarps + warp;
+    const Place at(blockIdx.z, blockIdx.y, items, rows, token_req, positions, nq, nkv, head_tiles, S::kCols, window);
+    if (at.req < 0) return;  // a row of padding
+    const int n0 = at.n0, pos0 = at.pos0, hk = at.hk, h0 = at.h0, heads = at.heads, cols = at.cols, end = at.end, start = at.start, tile0 = at.tile0, tiles = at.tiles;
+    const int* bt = block_table + (size_t)at.req * table_stride;
+    const int blocks = part ? at.parts(splits, least) : splits;
+    if ((int)blockIdx.x >= blocks) return;
+    const int step = blocks * kWarps, first = (int)blockIdx.x * kWarps + warp;
 
     // a tile: 16-byte pieces, codes and pairs of keys and of values, from the pages that it lies in (1, 2 or 4)
     const int page_log = kPages == 1 ? 5 : kPages == 2 ? 4 : 31 - __clz(min(kTile, page_size)), pages = kTile >> page_log;  // keys of a page in a tile
@@ -353,8 +374,6 @@ attention_kv4_tc_kernel(const __nv_bfloat16* __restrict__ q, long long ldq, cons
         }
     }
     __syncthreads();
-    // a warp's part: 2^(its maximum - the block's); one that saw no key adds nothing, one whose scores are all NaN makes the column NaN
-    auto share = [](float m_part, float l_part, float top) { return m_part == -INFINITY ? 0.f * l_part : ns_exp2(m_part - top); };
     float* block_o = reinterpret_cast<float*>(smem);  // (warp 0's: every thread reads its own elements before it writes them)
     for (int e = threadIdx.x; e < cols * D; e += kThreads) {
         const int c = e / D;
@@ -371,86 +390,104 @@ attention_kv4_tc_kernel(const __nv_bfloat16* __restrict__ q, long long ldq, cons
         if (e % D == 0) { mb_s[c] = top; lb_s[c] = sum; }
     }
     __syncthreads();
-    // ---- the cluster's blocks: each writes a share of the outputs ----------------------------------------------------------------------
-    if (splits > 1) cluster_sync();
-    const int total = cols * D / 2, share_n = (total + splits - 1) / splits;
-    for (int e = (int)blockIdx.x * share_n + threadIdx.x; e < min(total, ((int)blockIdx.x + 1) * share_n); e += kThreads) {
-        const int c = 2 * e / D, f = 2 * e - c * D, h = h0 + c % heads;
-        const float sink2 = sink ? sink[h] * kLog2e : -INFINITY;
-        float top = sink2, a0 = 0.f, a1 = 0.f, sum = 0.f;
-        if (splits == 1) {
-            top = fmaxf(top, mb_s[c]);
-            const float w = share(mb_s[c], lb_s[c], top);
-            sum = w * lb_s[c];
-            a0 = w * block_o[2 * e];
-            a1 = w * block_o[2 * e + 1];
-        } else {
-            float ms[16];
-#pragma unroll
-            for (int b = 0; b < 16; ++b)
-                if (b < splits) top = fmaxf(top, ms[b] = ld_cluster_f32(smem_u32(&mb_s[c]), b));
-#pragma unroll
-            for (int b = 0; b < 16; ++b)
-                if (b < splits) {
-                    const float ls = ld_cluster_f32(smem_u32(&lb_s[c]), b), w = share(ms[b], ls, top);
-                    sum += w * ls;
-                    a0 += w * ld_cluster_f32(smem_u32(block_o + 2 * e), b);
-                    a1 += w * ld_cluster_f32(smem_u32(block_o + 2 * e + 1), b);
-                }
-        }
-        if (sink) sum += ns_exp2(sink2 - top);
-        __nv_bfloat16* to = out + (size_t)(n0 + c / heads) * ldo + (size_t)h * D + f;
-        to[0] = __float2bfloat16_rn(a0 / sum);
-        to[1] = __float2bfloat16_rn(a1 / sum);
+    if (part) {  // attention_kv4_join_kernel goes on from here
+        float* to = part + (((size_t)blockIdx.z * gridDim.y + blockIdx.y) * splits + blockIdx.x) * S::kCols * (D + 2);
+        for (int c = threadIdx.x; c < cols; c += kThreads) { to[2 * c] = mb_s[c]; to[2 * c + 1] = lb_s[c]; }
+        for (int e = threadIdx.x; e < cols * D / 4; e += kThreads) reinterpret_cast<float4*>(to + 2 * S::kCols)[e] = reinterpret_cast<const float4*>(block_o)[e];
+        return;
     }
-    if (splits > 1) {
-        __syncthreads();
-        cluster_sync();  // nobody's shared memory goes while another block reads it
+    for (int e = threadIdx.x; e < cols * D / 2; e += kThreads) {
+        const int c = 2 * e / D, f = 2 * e - c * D, h = h0 + c % heads;
+        const float sink2 = sink ? sink[h] * kLog2e : -INFINITY, top = fmaxf(sink2, mb_s[c]), w = share(mb_s[c], lb_s[c], top);
+        const float sum = w * lb_s[c] + (sink ? ns_exp2(sink2 - top) : 0.f);
+        __nv_bfloat16* to = out + (size_t)(n0 + c / heads) * ldo + (size_t)h * D + f;
+        to[0] = __float2bfloat16_rn(w * block_o[2 * e] / sum);
+        to[1] = __float2bfloat16_rn(w * block_o[2 * e + 1] / sum);
+    }
+}
+
+// Joins the blocks of a (row, kv head): a block a column, whose threads take four features of every (kJoinThreads / (D / 4))-th part, so
+// that the reads of all parts are under way together, and add those in their order.
+constexpr int kMostParts = 160, kJoinThreads = 256;
+template <int D>
+__global__ void __launch_bounds__(kJoinThreads)
+attention_kv4_join_kernel(const float* __restrict__ part, const int* __restrict__ token_req, const int* __restrict__ positions, const int* __restrict__ rows,
+                          const int* __restrict__ items, __nv_bfloat16* __restrict__ out, long long ldo, int nq, int nkv, int kCols, int window,
+                          const float* __restrict__ sink, int head_tiles, int splits, int least) {
+    constexpr int kGroups = kJoinThreads / (D / 4), kWarps = kJoinThreads / 32;
+    __shared__ float w_s[kMostParts], max_s[kWarps], sum_s[kWarps];
+    __shared__ float4 o_s[kGroups][D / 4];
+    ns_pdl_launch_dependents();
+    ns_pdl_wait();
+    const Place at(blockIdx.y, blockIdx.x, items, rows, token_req, positions, nq, nkv, head_tiles, kCols, window);
+    const int c = blockIdx.z, warp = threadIdx.x >> 5;
+    if (at.req < 0 || c >= at.cols) return;
+    const int blocks = at.parts(splits, least), h = at.h0 + c % at.heads;
+    const size_t each = (size_t)kCols * (D + 2);
+    const float* from = part + ((size_t)blockIdx.y * gridDim.x + blockIdx.x) * splits * each;
+    const float sink2 = sink ? sink[h] * kLog2e : -INFINITY;
+    static_assert(kMostParts <= kJoinThreads, "a thread a part");
+    float2 ml = make_float2(-INFINITY, 0.f);
+    if (threadIdx.x < blocks) ml = *reinterpret_cast<const float2*>(from + threadIdx.x * each + 2 * c);
+    float top = ml.x;
+#pragma unroll
+    for (int d = 16; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+    if ((threadIdx.x & 31) == 0) max_s[warp] = top;
+    __syncthreads();
+    top = sink2;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) top = fmaxf(top, max_s[w]);
+    float sum = 0.f;
+    if (threadIdx.x < blocks) {
+        const float w = share(ml.x, ml.y, top);
+        w_s[threadIdx.x] = w;
+        sum = w * ml.y;
+    }
+#pragma unroll
+    for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+    if ((threadIdx.x & 31) == 0) sum_s[warp] = sum;
+    __syncthreads();
+    const int f4 = threadIdx.x % (D / 4), g = threadIdx.x / (D / 4);
+    const float* o = from + 2 * kCols + c * D + 4 * f4;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+    for (int b = g; b < blocks; b += kGroups) {
+        const float4 v = *reinterpret_cast<const float4*>(o + b * each);
+        const float w = w_s[b];
+        acc.x += w * v.x; acc.y += w * v.y; acc.z += w * v.z; acc.w += w * v.w;
+    }
+    o_s[g][f4] = acc;
+    __syncthreads();
+    if (threadIdx.x < D) {
+        float a = 0.f;
+#pragma unroll
+        for (int i = 0; i < kGroups; ++i) a += reinterpret_cast<const float*>(o_s[i])[threadIdx.x];
+        sum = sink ? ns_exp2(sink2 - top) : 0.f;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) sum += sum_s[w];
+        out[(size_t)(at.n0 + c / at.heads) * ldo + (size_t)h * D + threadIdx.x] = __float2bfloat16_rn(a / sum);
     }
 }
 
 template <int D, int NB, int kWarps, int kPages>
 int launch(const void* q, long long ldq, const void* k, const void* v, const int* table, int table_stride, const int* token_req, const int* positions,
            const int* rows, const int* items, int n, void* out, long long ldo, int nq, int nkv, int page_size, float scale, int window, const float* sink,
-           int splits, cudaStream_t stream) {
+           int splits, float* part, int least, cudaStream_t stream) {
     using S = Shape<D, NB, kWarps>;
-    static std::atomic<unsigned long long> allowed{0}, wide{0};
+    static std::atomic<unsigned long long> allowed{0};
     auto* kernel = attention_kv4_tc_kernel<D, NB, kWarps, kPages>;
     NS_CUDA(ns_allow_smem((const void*)kernel, (int)S::kSmem, allowed));
-    if (splits > 8) {
-        int dev = 0;
-        NS_CUDA(cudaGetDevice(&dev));
-        const unsigned long long bit = dev < 64 ? 1ull << dev : 0ull;
-        if (!(wide.load() & bit)) {
-            NS_CUDA(cudaFuncSetAttribute((const void*)kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
-            wide.fetch_or(bit);
-        }
-    }
     const int head_tiles = (nq / nkv + S::kCols - 1) / S::kCols;
     if ((long long)nkv * head_tiles > 65535 || n > 65535) NS_FAIL(NS_ERR_UNSUPPORTED, "ns_attention_kv4_tc: %d tokens, %d heads exceed the grid", n, nq);
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(splits, nkv * head_tiles, n);
-    cfg.blockDim = dim3(S::kThreads);
-    cfg.dynamicSmemBytes = S::kSmem;
-    cfg.stream = stream;
-    cudaLaunchAttribute attr[2];
-    int n_attr = 0;
-    if (ns_take_pdl()) {
-        attr[n_attr].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-        attr[n_attr++].val.programmaticStreamSerializationAllowed = 1;
-    }
-    if (splits > 1) {
-        attr[n_attr].id = cudaLaunchAttributeClusterDimension;
-        attr[n_attr].val.clusterDim.x = splits;
-        attr[n_attr].val.clusterDim.y = 1;
-        attr[n_attr++].val.clusterDim.z = 1;
-    }
-    cfg.attrs = attr;
-    cfg.numAttrs = n_attr;
-    (void)cudaLaunchKernelEx(&cfg, kernel, (const __nv_bfloat16*)q, ldq, (const uint8_t*)k, (const uint8_t*)v, table, table_stride, token_req, positions, rows, items,
-                             (__nv_bfloat16*)out, ldo, nq, nkv, page_size, scale, window, sink, head_tiles, splits,
-                             (page_size & (page_size - 1)) == 0 ? 31 - __builtin_clz(page_size) : -1);
+    NS_LAUNCH(kernel, dim3(splits, nkv * head_tiles, n), S::kThreads, S::kSmem, stream, (const __nv_bfloat16*)q, ldq, (const uint8_t*)k, (const uint8_t*)v, table,
+              table_stride, token_req, positions, rows, items, (__nv_bfloat16*)out, ldo, nq, nkv, page_size, scale, window, sink, head_tiles, splits,
+              (page_size & (page_size - 1)) == 0 ? 31 - __builtin_clz(page_size) : -1, part, least);
     NS_CHECK_LAUNCH("ns_attention_kv4_tc");
+    if (part) {
+        NS_LAUNCH((attention_kv4_join_kernel<D>), dim3(nkv * head_tiles, n, S::kCols), kJoinThreads, 0, stream, part, token_req, positions, rows, items, (__nv_bfloat16*)out, ldo,
+                  nq, nkv, S::kCols, window, sink, head_tiles, splits, least);
+        NS_CHECK_LAUNCH("ns_attention_kv4_tc");
+    }
     return NS_OK;
 }
 
@@ -458,19 +495,21 @@ int launch(const void* q, long long ldq, const void* k, const void* v, const int
 
 // bfloat16 q [tokens, ldq] and out [tokens, ldo]; heads of 64, 128 or 256; pages of 8, 16 or a multiple of 32 tokens.  Which tokens: `items` [n, 2] =
 // (first row, tokens of one request, of which the heads that share a kv head fill at most 8 * n_blocks columns), or one token each: rows [n], or all n.
-// splits: blocks of a cluster that share a request's keys (1, 2, 4, 8 or 16).
+// A block to a (token or item, kv head), or, with `part` (a workspace of n * nkv * tiles of heads * splits * 8 * n_blocks * (D + 2) floats), up to `splits` blocks,
+// of `least` tiles of 32 keys or more each, and a second kernel that joins them.
 NS_API int ns_attention_kv4_tc(const void* q, long long ldq, const void* k, const void* v, const int* table, int table_stride, const int* token_req,
                                const int* positions, const int* rows, const int* items, int n, void* out, long long ldo, int nq, int nkv, int D, int page_size,
-                               float scale, int window, const float* sink, int n_blocks, int warps, int splits, cudaStream_t stream) {
+                               float scale, int window, const float* sink, int n_blocks, int warps, int splits, float* part, int least, cudaStream_t stream) {
     if (n <= 0) return NS_OK;
     if (nkv < 1 || nq < 1 || nq % nkv || window < 0 || !(page_size == 8 || page_size == 16 || (page_size > 0 && page_size % 32 == 0)))
         NS_FAIL(NS_ERR_UNSUPPORTED, "ns_attention_kv4_tc: %d heads over %d, pages of %d, a window of %d", nq, nkv, page_size, window);
-    if (splits < 1 || splits > 16 || (splits & (splits - 1)) || ((uintptr_t)k | (uintptr_t)v) % 16)
-        NS_FAIL(NS_ERR_ARGUMENT, "ns_attention_kv4_tc: %d blocks to a request, pages on 16-byte boundaries", splits);
+    if (splits < 1 || splits > (part ? kMostParts : 1) || (part && least < 1) || (uintptr_t)part % 16)
+        NS_FAIL(NS_ERR_ARGUMENT, "ns_attention_kv4_tc: %d blocks to a request, of %d tiles or more", splits, least);
+    if (((uintptr_t)k | (uintptr_t)v) % 16) NS_FAIL(NS_ERR_ARGUMENT, "ns_attention_kv4_tc: pages on 16-byte boundaries");
 #define NS_KV4_CASE(DD, NBB, WW)                                                                                                                        \
     if (D == DD && n_blocks == NBB && warps == WW)                                                                                                     \
         return (page_size == 16 ? launch<DD, NBB, WW, 2> : page_size < 16 ? launch<DD, NBB, WW, 0> : launch<DD, NBB, WW, 1>)(q, ldq, k, v, table, table_stride, token_req, positions, rows, items, n, out, ldo, nq, nkv, page_size, scale,     \
-                                   window, sink, splits, stream);
+                                   window, sink, splits, part, least, stream);
     NS_KV4_CASE(64, 1, 4) NS_KV4_CASE(64, 2, 4) NS_KV4_CASE(128, 1, 4) NS_KV4_CASE(128, 2, 4) NS_KV4_CASE(256, 1, 4) NS_KV4_CASE(256, 2, 4)
     NS_KV4_CASE(64, 1, 8) NS_KV4_CASE(64, 2, 8) NS_KV4_CASE(128, 1, 8) NS_KV4_CASE(128, 2, 8) NS_KV4_CASE(256, 1, 8) NS_KV4_CASE(256, 2, 8)
 #undef NS_KV4_CASE

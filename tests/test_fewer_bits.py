@@ -93,7 +93,21 @@ def test_tiles_of_a_few_tokens():
     assert ops.kv4_token_tiles([(0, 2, 9), (5, 6, 9)], 4) == ([(0, 2), (5, 4), (9, 2)], 2)
     assert ops.kv4_token_tiles([(3, 2, 9)], 4) == ([(3, 2)], 1)
     assert ops.kv4_token_tiles([(0, 3, 9)], 20) == ([(0, 1), (1, 1), (2, 1)], 2)
-    for blocks, longest in ((1, 1), (8, 1000), (512, 2300), (16, 100000), (8, None), (100000, 5)):
-        warps, splits = ops.kv4_shape(blocks, longest, 148)
-        assert warps in (4, 8) and splits in (1, 2, 4, 8, 16) and (splits == 1 or longest is None or longest > 16 * warps * splits)
-        assert ops.kv4_shape(blocks, longest, 148, 8)[1] <= 8
+
+
+@pytest.mark.parametrize("head_dim,n_blocks,resident", [(128, 1, 4), (128, 2, 3), (64, 1, 6), (64, 2, 3), (256, 1, 2), (256, 2, 2)])
+def test_shape_of_a_launch(head_dim, n_blocks, resident):
+    from nanospec_b200 import ops
+    for per_row in (1, 2, 8, 1000):
+        for lengths in ((1,), (0,), (33,), (1000,), (100000,), (3000000,), (100000, 61000), (5, 100000), (700,) * 16, (4000,) * 16, (2300, 500) * 32, (9,) * 5000):
+            for known in (True, False):
+                warps, splits, least = ops.kv4_shape(lengths if known else None, len(lengths), per_row, 148, head_dim, n_blocks)
+                assert warps in (4, 8) and 1 <= splits <= 160 and (least > 0) == (splits > 1)
+                if splits > 1:
+                    assert warps == 4 and len(lengths) * per_row * 2 <= 148 * resident
+                    if known:  # every block has its place at once
+                        assert least >= 4 and per_row * sum(-(-n // (32 * least)) for n in lengths) <= 148 * resident
+                        assert splits == -(-max(lengths) // (32 * least))
+                    else:
+                        assert len(lengths) * per_row * splits <= 148 * resident
+    assert ops.kv4_shape((100000,), 1, 8, 148, 128)[1] > 60 and ops.kv4_shape((16,), 1, 8, 148, 128) == (8, 1, 0)

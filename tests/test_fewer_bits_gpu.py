@@ -406,9 +406,10 @@ def test_more_rows_than_a_grid_holds(monkeypatch):
         ctx, lane, qkv = step(lens, 16, 2, 64, BF16, 4)
         fill(ctx, lane, 4, 2, 64)
         monkeypatch.setattr(kv4, "KV4_GRID_MAX", 65535)
-        monkeypatch.setattr(kv4, "kv4_shape", lambda *a: (4, 2))
+        monkeypatch.setattr(kv4, "kv4_shape", lambda *a: (4, 2, 1))
         want = ops.attention_kv4(qkv, lane, ctx, torch.zeros((ctx.n_tokens, 256), dtype=BF16, device="cuda"), 4, 2, 64)
         monkeypatch.setattr(kv4, "KV4_GRID_MAX", 7)
+        ctx.extras = {}
         got = ops.attention_kv4(qkv, lane, ctx, torch.zeros_like(want), 4, 2, 64)
         assert torch.equal(got, want)
 
@@ -465,6 +466,33 @@ def test_a_token_that_is_not_finite_reaches_those_that_see_it(lens, dim, dtype):
         assert torch.equal(out[:, 2 * dim:].isnan(), sees)
         assert torch.equal(out[:, 2 * dim:][~sees], clean[:, 2 * dim:][~sees])
         lane.k.copy_(kept[0]), lane.v.copy_(kept[1])
+
+
+@pytest.mark.parametrize("nq,nkv,dim,page", [(8, 2, 128, 16), (4, 4, 64, 8), (20, 1, 128, 32), (6, 1, 256, 16)])
+@pytest.mark.parametrize("tokens", [1, 3])
+def test_requests_over_several_blocks(nq, nkv, dim, page, tokens, monkeypatch):
+    """The same step with its keys dealt to one block or to many: blocks without a tile, the most there may be, fewer than a request has tiles."""
+    from nanospec_b200 import ops
+    from nanospec_b200.ops import kv4
+    lens = [(5200, tokens), (70, tokens), (0, tokens), (2111, tokens)]
+    sink = _rand(nq, seed=3)
+    ctx, lane, qkv = step(lens, page, nkv, dim, BF16, nq, padding=2)
+    lane.k.fill_(255), lane.v.fill_(255)
+    k, v = fill(ctx, lane, nq, nkv, dim)
+    n = ctx.n_tokens - 2
+    for window in (0, 100):
+        want, tol, _ = attend(qkv[:n, : nq * dim], k, v, ctx, nq, dim ** -0.5, window, sink)
+        tol = tol + want.abs() * 1.01 * half_step(BF16)
+        for graph in (False, True) if tokens == 1 else (False,):
+            for shape in (None, (4, 1, 0), (8, 1, 0), (4, 160, 1), (4, 7, 9), (4, 2, 100), (8, 3, 1)):
+                if shape:
+                    monkeypatch.setattr(kv4, "kv4_shape", lambda *a: shape)
+                ctx.extras = {"graph": True} if graph else {}
+                out = torch.full((ctx.n_tokens, nq * dim), 5.0, dtype=BF16, device="cuda")
+                ops.attention_kv4(qkv, lane, ctx, out, nq, nkv, dim, window=window, sink=sink)
+                _near(out[:n].double().reshape(want.shape), want, tol)
+                assert (out[n:] == 5).all()
+                monkeypatch.undo()
 
 
 def test_scores_far_apart():
