@@ -7,7 +7,7 @@
 //   out^T [features x columns] += V^T [features x keys] weights^T.  A lane takes an eighth of four keys' features; the codes of two keys are
 //     brought side by side (two byte permutations for eight features), and the same shift, mask and fma make two values.  The weights turn from
 //     the scores' layout into the right operand's by one 8 x 8 transposition of 16-bit numbers in registers.
-// Rows of the score tile are dealt to keys (key_of_row) such that both sides' reads of shared memory spread over the banks.
+// Rows of the score tile are dealt to keys (row_key) such that both sides' reads of shared memory spread over the banks.
 //
 // Every warp is on its own: it takes every (warps of the request's blocks)-th tile of 32 keys, brings it in 16-byte pieces into its own ring (bulk copies, a
 // lane each for the codes and pairs of a page, took as long as the tile's arithmetic: their addresses are not a warp's but a lane's), and keeps its own maximum,
@@ -408,7 +408,7 @@ attention_kv4_tc_kernel(const __nv_bfloat16* __restrict__ q, long long ldq, cons
 
 // Joins the blocks of a (row, kv head): a block a column, whose threads take four features of every (kJoinThreads / (D / 4))-th part, so
 // that the reads of all parts are under way together, and add those in their order.
-constexpr int kMostParts = 160, kJoinThreads = 256;
+constexpr int kMostParts = 256, kJoinThreads = 256;
 template <int D>
 __global__ void __launch_bounds__(kJoinThreads)
 attention_kv4_join_kernel(const float* __restrict__ part, const int* __restrict__ token_req, const int* __restrict__ positions, const int* __restrict__ rows,

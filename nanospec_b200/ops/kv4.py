@@ -92,7 +92,7 @@ def kv4_tensor_core_ok(dtype: torch.dtype, head_dim: int, page_size: int) -> boo
     return dtype == torch.bfloat16 and head_dim in (64, 128, 256) and (page_size in (8, 16) or page_size % 32 == 0)
 
 
-KV4_PARTS_MAX = 160
+KV4_PARTS_MAX = 256  # blocks of a row and kv head
 
 
 def kv4_shape(lengths: tuple[int, ...] | None, rows: int, per_row: int, sms: int, head_dim: int, n_blocks: int = 1) -> tuple[int, int, int]:
@@ -112,12 +112,12 @@ def kv4_shape(lengths: tuple[int, ...] | None, rows: int, per_row: int, sms: int
     tiles = [-(-n // KV4_TILE) for n in lengths]
     longest = max(tiles)
     if total * 2 <= slots:
-        least = max(4, -(-sum(tiles) // room))
+        least = max(4, -(-sum(tiles) // room), -(-longest // KV4_PARTS_MAX))
         while sum(-(-t // least) for t in tiles) > room:
             least += 1
         splits, wave = -(-longest // least), sum(-(-t // least) for t in tiles) * per_row / slots
         one = 9 + longest * 0.18 * head_dim / 128 * (1.5 if n_blocks > 1 else 1) * (1 if total <= sms else 1.5)
-        if 1 < splits <= KV4_PARTS_MAX and 12 + least * max(0.33, wave) * 0.9 * slots / sms * head_dim / 512 < one:
+        if splits > 1 and 12 + least * max(0.33, wave) * 0.9 * slots / sms * head_dim / 512 < one:
             return 4, splits, least
     return 8 if total <= 2 * sms or total * 32 <= sms * longest else 4, 1, 0
 

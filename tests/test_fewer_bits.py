@@ -102,7 +102,7 @@ def test_shape_of_a_launch(head_dim, n_blocks, resident):
         for lengths in ((1,), (0,), (33,), (1000,), (100000,), (3000000,), (100000, 61000), (5, 100000), (700,) * 16, (4000,) * 16, (2300, 500) * 32, (9,) * 5000):
             for known in (True, False):
                 warps, splits, least = ops.kv4_shape(lengths if known else None, len(lengths), per_row, 148, head_dim, n_blocks)
-                assert warps in (4, 8) and 1 <= splits <= 160 and (least > 0) == (splits > 1)
+                assert warps in (4, 8) and 1 <= splits <= 256 and (least > 0) == (splits > 1)
                 if splits > 1:
                     assert warps == 4 and len(lengths) * per_row * 2 <= 148 * resident
                     if known:  # every block has its place at once
@@ -110,4 +110,5 @@ def test_shape_of_a_launch(head_dim, n_blocks, resident):
                         assert splits == -(-max(lengths) // (32 * least))
                     else:
                         assert len(lengths) * per_row * splits <= 148 * resident
+    assert ops.kv4_shape((100000,), 1, 1, 148, 128)[1] > 200  # (one kv head: more blocks than are joined would find a place)
     assert ops.kv4_shape((100000,), 1, 8, 148, 128)[1] > 60 and ops.kv4_shape((16,), 1, 8, 148, 128) == (8, 1, 0)
