@@ -2,9 +2,10 @@
 //
 // What the cache holds is the definition's to the last bit: k rotated exactly and rounded once to the activations' type, S and B rounded once, codes decided by
 // exact remainders.  One rounding that fell on the other side of a border would move a feature by a whole code, or a group by its S.  Computed in double
-// throughout, a prompt is bound by its instructions (3,745 tokens of the 8B shape 53 us, 96 MB); so everything is first done in float, with a bound of
-// its error, and again in double where a border between two roundings lies within the bound - one element in some thousands.  float32 activations, which have
-// no bits to spare in float, are rotated in double.  q, which is rounded to the activations' type and not quantised, is rotated in float.
+// throughout, a prompt is bound by its instructions (3,739 tokens of 32 + 2 x 8 heads of 128, 96 MB: 53 us); so everything is first done in float, with a bound of
+// its error, and again in double where a border between two roundings lies within the bound - one element in some thousands.  The same tokens now take 37.9
+// us, of which 14.7 are their bytes at the rate of a copy: instructions still bound it, the schedulers issue in two cycles of three.  float32 activations, which
+// have no bits to spare in float, are rotated in double.  q, which is rounded to the activations' type and not quantised, is rotated in float.
 #include "kv4.cuh"
 
 namespace {
@@ -170,11 +171,14 @@ template <typename T> struct Angle { using type = float; };
 template <> struct Angle<float> { using type = double; };
 
 // One block (or `gridDim.y` blocks, which share its heads) per token.  For keys and values a lane holds four neighbouring features of every 128, eight lanes a group.
-template <typename T, int kChunks>
-__global__ void __launch_bounds__(kThreads)
+// kD: the size of a head, where it is a usual one (3,739 tokens of 32 + 2 x 8 heads of 128: 44.0 us without, 39.9), or 0.  bfloat16 in 48 registers, which spills a
+// little, holds five blocks an SM rather than four (37.9).
+template <typename T, int kChunks, int kD>
+__global__ void __launch_bounds__(kThreads, sizeof(T) == 2 && kChunks == 1 ? 5 : 1)
 kv4_store_kernel(const T* __restrict__ qkv, long long ld, T* __restrict__ q_out, long long ldq, const int* __restrict__ positions,
                  const int* __restrict__ token_req, const int* __restrict__ block_table, int table_stride, const float* __restrict__ inv_freq,
-                 int pairs, uint8_t* __restrict__ k_pages, uint8_t* __restrict__ v_pages, int page_size, int nq, int nkv, int D) {
+                 int pairs, uint8_t* __restrict__ k_pages, uint8_t* __restrict__ v_pages, int page_size, int nq, int nkv, int any_D) {
+    const int D = kD ? kD : any_D;
     using A = typename Angle<T>::type;
     __shared__ __align__(16) A cs[256];  // cosines of the token's angles, then their sines
     __shared__ long long block_s;        // where the token's page begins
@@ -326,13 +330,15 @@ NS_API int ns_kv4_store(const void* qkv, long long ld, void* q_out, long long ld
     int parts = (2 * sms + n_tokens - 1) / n_tokens;
     parts = parts < 1 ? 1 : parts > most ? most : parts;
     dim3 grid(n_tokens, parts);
-#define NS_KV4_STORE(T, CHUNKS)                                                                                                       \
-    NS_LAUNCH((kv4_store_kernel<T, CHUNKS>), grid, kThreads, 0, stream, (const T*)qkv, ld, (T*)q_out, ldq, positions, token_req,    \
+#define NS_KV4_STORE(T, CHUNKS, DD)                                                                                                   \
+    NS_LAUNCH((kv4_store_kernel<T, CHUNKS, DD>), grid, kThreads, 0, stream, (const T*)qkv, ld, (T*)q_out, ldq, positions, token_req,    \
               block_table, table_stride, inv_freq, pairs, (uint8_t*)k_pages, (uint8_t*)v_pages, page_size, nq, nkv, D)
-    if (dtype == NS_BF16 && D <= 128) NS_KV4_STORE(__nv_bfloat16, 1);
-    else if (dtype == NS_BF16) NS_KV4_STORE(__nv_bfloat16, 2);
-    else if (dtype == NS_F32 && D <= 128) NS_KV4_STORE(float, 1);
-    else if (dtype == NS_F32) NS_KV4_STORE(float, 2);
+    if (dtype == NS_BF16 && D == 128) NS_KV4_STORE(__nv_bfloat16, 1, 128);
+    else if (dtype == NS_BF16 && D == 64) NS_KV4_STORE(__nv_bfloat16, 1, 64);
+    else if (dtype == NS_BF16 && D < 128) NS_KV4_STORE(__nv_bfloat16, 1, 0);
+    else if (dtype == NS_BF16) NS_KV4_STORE(__nv_bfloat16, 2, 0);
+    else if (dtype == NS_F32 && D <= 128) NS_KV4_STORE(float, 1, 0);
+    else if (dtype == NS_F32) NS_KV4_STORE(float, 2, 0);
     else NS_FAIL(NS_ERR_UNSUPPORTED, "ns_kv4_store: float32 and bfloat16, not type %d", dtype);
 #undef NS_KV4_STORE
     NS_CHECK_LAUNCH("ns_kv4_store");
