@@ -91,7 +91,8 @@ __global__ void __launch_bounds__(32 * kWarps, Shape<D, NB, kWarps>::kResident)
 attention_kv4_tc_kernel(const __nv_bfloat16* __restrict__ q, long long ldq, const uint8_t* __restrict__ k_pages, const uint8_t* __restrict__ v_pages,
                         const int* __restrict__ block_table, int table_stride, const int* __restrict__ token_req, const int* __restrict__ positions,
                         const int* __restrict__ rows, const int* __restrict__ items, __nv_bfloat16* __restrict__ out, long long ldo, int nq, int nkv,
-                        int page_size, float scale, int window, const float* __restrict__ sink, int head_tiles, int splits, int page_shift, float* __restrict__ part, int least) {
+                        int page_size, float scale, int window, const float* __restrict__ sink, int head_tiles, int splits, int page_shift, float* __restrict__ part,
+                        const int* __restrict__ jobs, int least) {
     using S = Shape<D, NB, kWarps>;
     constexpr int kThreads = S::kThreads;
     extern __shared__ __align__(128) unsigned char smem[];
@@ -103,13 +104,15 @@ attention_kv4_tc_kernel(const __nv_bfloat16* __restrict__ q, long long ldq, cons
     ns_pdl_launch_dependents();
     ns_pdl_wait();
 
-    const Place at(blockIdx.z, blockIdx.y, items, rows, token_req, positions, nq, nkv, head_tiles, S::kCols, window);
+    const int unit = (int)blockIdx.x / (nkv * head_tiles), y = (int)blockIdx.x - unit * nkv * head_tiles;  // (a row's heads come together: the longest rows first)
+    const int z = jobs ? jobs[3 * unit] : unit / splits, which_part = jobs ? jobs[3 * unit + 1] : unit - z * splits;
+    const Place at(z, y, items, rows, token_req, positions, nq, nkv, head_tiles, S::kCols, window);
     if (at.req < 0) return;  // a row of padding
     const int n0 = at.n0, pos0 = at.pos0, hk = at.hk, h0 = at.h0, heads = at.heads, cols = at.cols, end = at.end, start = at.start, tile0 = at.tile0, tiles = at.tiles;
     const int* bt = block_table + (size_t)at.req * table_stride;
-    const int blocks = part ? at.parts(splits, least) : splits;
-    if ((int)blockIdx.x >= blocks) return;
-    const int step = blocks * kWarps, first = (int)blockIdx.x * kWarps + warp;
+    const int blocks = jobs ? jobs[3 * unit + 2] : part ? at.parts(splits, least) : 1;
+    if (which_part >= blocks) return;
+    const int step = blocks * kWarps, first = which_part * kWarps + warp;
 
     // a tile: 16-byte pieces, codes and pairs of keys and of values, from the pages that it lies in (1, 2 or 4)
     const int page_log = kPages == 1 ? 5 : kPages == 2 ? 4 : 31 - __clz(min(kTile, page_size)), pages = kTile >> page_log;  // keys of a page in a tile
@@ -391,7 +394,7 @@ attention_kv4_tc_kernel(const __nv_bfloat16* __restrict__ q, long long ldq, cons
     }
     __syncthreads();
     if (part) {  // attention_kv4_join_kernel goes on from here
-        float* to = part + (((size_t)blockIdx.z * gridDim.y + blockIdx.y) * splits + blockIdx.x) * S::kCols * (D + 2);
+        float* to = part + (size_t)blockIdx.x * S::kCols * (D + 2);
         for (int c = threadIdx.x; c < cols; c += kThreads) { to[2 * c] = mb_s[c]; to[2 * c + 1] = lb_s[c]; }
         for (int e = threadIdx.x; e < cols * D / 4; e += kThreads) reinterpret_cast<float4*>(to + 2 * S::kCols)[e] = reinterpret_cast<const float4*>(block_o)[e];
         return;
@@ -413,18 +416,19 @@ template <int D>
 __global__ void __launch_bounds__(kJoinThreads)
 attention_kv4_join_kernel(const float* __restrict__ part, const int* __restrict__ token_req, const int* __restrict__ positions, const int* __restrict__ rows,
                           const int* __restrict__ items, __nv_bfloat16* __restrict__ out, long long ldo, int nq, int nkv, int kCols, int window,
-                          const float* __restrict__ sink, int head_tiles, int splits, int least) {
+                          const float* __restrict__ sink, int head_tiles, int splits, const int* __restrict__ spans, int least) {
     constexpr int kGroups = kJoinThreads / (D / 4), kWarps = kJoinThreads / 32;
     __shared__ float w_s[kMostParts], max_s[kWarps], sum_s[kWarps];
     __shared__ float4 o_s[kGroups][D / 4];
     ns_pdl_launch_dependents();
     ns_pdl_wait();
-    const Place at(blockIdx.y, blockIdx.x, items, rows, token_req, positions, nq, nkv, head_tiles, kCols, window);
-    const int c = blockIdx.z, warp = threadIdx.x >> 5;
+    const int per_row = nkv * head_tiles, z = (int)blockIdx.x / per_row, y = (int)blockIdx.x - z * per_row;
+    const Place at(z, y, items, rows, token_req, positions, nq, nkv, head_tiles, kCols, window);
+    const int c = blockIdx.y, warp = threadIdx.x >> 5;
     if (at.req < 0 || c >= at.cols) return;
-    const int blocks = at.parts(splits, least), h = at.h0 + c % at.heads;
-    const size_t each = (size_t)kCols * (D + 2);
-    const float* from = part + ((size_t)blockIdx.y * gridDim.x + blockIdx.x) * splits * each;
+    const int blocks = spans ? spans[2 * z + 1] : at.parts(splits, least), h = at.h0 + c % at.heads;
+    const size_t each = (size_t)per_row * kCols * (D + 2);  // from a part of the row to its next one
+    const float* from = part + ((size_t)(spans ? spans[2 * z] : z * splits) * per_row + y) * kCols * (D + 2);
     const float sink2 = sink ? sink[h] * kLog2e : -INFINITY;
     static_assert(kMostParts <= kJoinThreads, "a thread a part");
     float2 ml = make_float2(-INFINITY, 0.f);
@@ -472,20 +476,21 @@ attention_kv4_join_kernel(const float* __restrict__ part, const int* __restrict_
 template <int D, int NB, int kWarps, int kPages>
 int launch(const void* q, long long ldq, const void* k, const void* v, const int* table, int table_stride, const int* token_req, const int* positions,
            const int* rows, const int* items, int n, void* out, long long ldo, int nq, int nkv, int page_size, float scale, int window, const float* sink,
-           int splits, float* part, int least, cudaStream_t stream) {
+           int splits, float* part, const int* jobs, int n_jobs, int least, cudaStream_t stream) {
     using S = Shape<D, NB, kWarps>;
     static std::atomic<unsigned long long> allowed{0};
     auto* kernel = attention_kv4_tc_kernel<D, NB, kWarps, kPages>;
     NS_CUDA(ns_allow_smem((const void*)kernel, (int)S::kSmem, allowed));
     const int head_tiles = (nq / nkv + S::kCols - 1) / S::kCols;
-    if ((long long)nkv * head_tiles > 65535 || n > 65535) NS_FAIL(NS_ERR_UNSUPPORTED, "ns_attention_kv4_tc: %d tokens, %d heads exceed the grid", n, nq);
-    NS_LAUNCH(kernel, dim3(splits, nkv * head_tiles, n), S::kThreads, S::kSmem, stream, (const __nv_bfloat16*)q, ldq, (const uint8_t*)k, (const uint8_t*)v, table,
+    const long long per_row = (long long)nkv * head_tiles, grid = per_row * (jobs ? n_jobs : (long long)n * splits);
+    if (grid > 0x7fffffff) NS_FAIL(NS_ERR_UNSUPPORTED, "ns_attention_kv4_tc: %d tokens, %d heads exceed the grid", n, nq);
+    NS_LAUNCH(kernel, (unsigned)grid, S::kThreads, S::kSmem, stream, (const __nv_bfloat16*)q, ldq, (const uint8_t*)k, (const uint8_t*)v, table,
               table_stride, token_req, positions, rows, items, (__nv_bfloat16*)out, ldo, nq, nkv, page_size, scale, window, sink, head_tiles, splits,
-              (page_size & (page_size - 1)) == 0 ? 31 - __builtin_clz(page_size) : -1, part, least);
+              (page_size & (page_size - 1)) == 0 ? 31 - __builtin_clz(page_size) : -1, part, jobs, least);
     NS_CHECK_LAUNCH("ns_attention_kv4_tc");
     if (part) {
-        NS_LAUNCH((attention_kv4_join_kernel<D>), dim3(nkv * head_tiles, n, S::kCols), kJoinThreads, 0, stream, part, token_req, positions, rows, items, (__nv_bfloat16*)out, ldo,
-                  nq, nkv, S::kCols, window, sink, head_tiles, splits, least);
+        NS_LAUNCH((attention_kv4_join_kernel<D>), dim3((unsigned)(per_row * n), S::kCols), kJoinThreads, 0, stream, part, token_req, positions, rows, items, (__nv_bfloat16*)out, ldo,
+                  nq, nkv, S::kCols, window, sink, head_tiles, splits, jobs ? jobs + 3 * n_jobs : nullptr, least);
         NS_CHECK_LAUNCH("ns_attention_kv4_tc");
     }
     return NS_OK;
@@ -495,21 +500,22 @@ int launch(const void* q, long long ldq, const void* k, const void* v, const int
 
 // bfloat16 q [tokens, ldq] and out [tokens, ldo]; heads of 64, 128 or 256; pages of 8, 16 or a multiple of 32 tokens.  Which tokens: `items` [n, 2] =
 // (first row, tokens of one request, of which the heads that share a kv head fill at most 8 * n_blocks columns), or one token each: rows [n], or all n.
-// A block to a (token or item, kv head), or, with `part` (a workspace of n * nkv * tiles of heads * splits * 8 * n_blocks * (D + 2) floats), up to `splits` blocks,
-// of `least` tiles of 32 keys or more each, and a second kernel that joins them.
+// A block to a (token or item, kv head), or, with `part`, several and a second kernel that joins them: `splits` (256 at most), of which those beyond one for each `least`
+// tiles of 32 keys leave at once, or those of `jobs` [n_jobs, 3] = (token or item, which part, of how many), each token's in order and together, which
+// [n, 2] = (first job, how many) follow.  `part`: nkv * tiles of heads * (n * splits or n_jobs) * 8 * n_blocks * (D + 2) floats.
 NS_API int ns_attention_kv4_tc(const void* q, long long ldq, const void* k, const void* v, const int* table, int table_stride, const int* token_req,
                                const int* positions, const int* rows, const int* items, int n, void* out, long long ldo, int nq, int nkv, int D, int page_size,
-                               float scale, int window, const float* sink, int n_blocks, int warps, int splits, float* part, int least, cudaStream_t stream) {
+                               float scale, int window, const float* sink, int n_blocks, int warps, int splits, float* part, const int* jobs, int n_jobs, int least, cudaStream_t stream) {
     if (n <= 0) return NS_OK;
     if (nkv < 1 || nq < 1 || nq % nkv || window < 0 || !(page_size == 8 || page_size == 16 || (page_size > 0 && page_size % 32 == 0)))
         NS_FAIL(NS_ERR_UNSUPPORTED, "ns_attention_kv4_tc: %d heads over %d, pages of %d, a window of %d", nq, nkv, page_size, window);
-    if (splits < 1 || splits > (part ? kMostParts : 1) || (part && least < 1) || (uintptr_t)part % 16)
+    if (splits < 1 || splits > (part ? kMostParts : 1) || (part && least < 1) || (uintptr_t)part % 16 || (jobs && (!part || n_jobs < 1)))
         NS_FAIL(NS_ERR_ARGUMENT, "ns_attention_kv4_tc: %d blocks to a request, of %d tiles or more", splits, least);
     if (((uintptr_t)k | (uintptr_t)v) % 16) NS_FAIL(NS_ERR_ARGUMENT, "ns_attention_kv4_tc: pages on 16-byte boundaries");
 #define NS_KV4_CASE(DD, NBB, WW)                                                                                                                        \
     if (D == DD && n_blocks == NBB && warps == WW)                                                                                                     \
         return (page_size == 16 ? launch<DD, NBB, WW, 2> : page_size < 16 ? launch<DD, NBB, WW, 0> : launch<DD, NBB, WW, 1>)(q, ldq, k, v, table, table_stride, token_req, positions, rows, items, n, out, ldo, nq, nkv, page_size, scale,     \
-                                   window, sink, splits, part, least, stream);
+                                   window, sink, splits, part, jobs, n_jobs, least, stream);
     NS_KV4_CASE(64, 1, 4) NS_KV4_CASE(64, 2, 4) NS_KV4_CASE(128, 1, 4) NS_KV4_CASE(128, 2, 4) NS_KV4_CASE(256, 1, 4) NS_KV4_CASE(256, 2, 4)
     NS_KV4_CASE(64, 1, 8) NS_KV4_CASE(64, 2, 8) NS_KV4_CASE(128, 1, 8) NS_KV4_CASE(128, 2, 8) NS_KV4_CASE(256, 1, 8) NS_KV4_CASE(256, 2, 8)
 #undef NS_KV4_CASE

@@ -1956,5 +1956,5 @@ def head_prepare_store(proj: torch.Tensor, out: torch.Tensor, ctx, lane, nq: int
 
 from .int8 import I8_MAX_K, RowsI8, i8_tiles, linear_i8, quantize_rows  # noqa: E402,F401
 from .kv4 import (  # noqa: E402,F401
-    KV4_GROUP, KV4_UNFOLD_PAGE, attention_kv4, kv4_block_bytes, kv4_pages, kv4_read, kv4_shape, kv4_store, kv4_token_tiles, kv4_unfold_runs, kv4_unfolded,
+    KV4_GROUP, KV4_UNFOLD_PAGE, attention_kv4, kv4_block_bytes, kv4_jobs, kv4_pages, kv4_read, kv4_shape, kv4_store, kv4_token_tiles, kv4_unfold_runs, kv4_unfolded,
 )

@@ -16,7 +16,7 @@ I8_MAX_K = 131072  # 127 * 127 * K stays within 32 bits
 
 @dataclass
 class RowsI8:
-    """A matrix in 8-bit integers: `q` [R, K] int8 (rows on 16-byte boundaries) and `scale` [R] float32; row r stands for q[r] * scale[r]."""
+    """A matrix in 8-bit integers from -127 to 127: `q` [R, K] int8 (rows on 16-byte boundaries) and `scale` [R] float32; row r stands for q[r] * scale[r]."""
 
     q: torch.Tensor
     scale: torch.Tensor
@@ -37,7 +37,7 @@ def _check_rows(r: RowsI8, name: str) -> int:
     if q.dtype is not torch.int8 or len(shape) != 2 or scale.dtype is not torch.float32 or scale.shape != shape[:1] or not scale.is_contiguous():
         raise KernelError(f"linear_i8: {name} must be int8 [R, K] with one contiguous float32 scale per row")
     step, inner = q.stride()
-    if shape[0] and (inner != 1 or step & 15 or q.data_ptr() & 15):
+    if shape[0] and (inner != 1 or step & 15 or not step or q.data_ptr() & 15):
         raise KernelError(f"linear_i8: the rows of {name} must start on 16-byte boundaries with unit inner stride (quantize_rows makes them so)")
     return step
 

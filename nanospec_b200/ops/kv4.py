@@ -100,26 +100,39 @@ def kv4_shape(lengths: tuple[int, ...] | None, rows: int, per_row: int, sms: int
 
     `lengths`: keys of each row (or tile of tokens), None when the device alone knows them; `per_row`: (kv head, column tile) pairs.  Us on a B200, the requests
     ragged down to a fifth of the length, 8 kv heads of 128:
-    Several blocks while one each would take no more than half of the places.  One request on 1,000 keys: one block of eight warps 14.4, several 12.3; on 100,000: (a
-    cluster of sixteen blocks) 71.7, several 46.6; 16 requests on 1,000: 16.4, 18.4; on 4,000: 34.8, 30.7.  The two costs below are fits to such figures.
+    Several blocks while one each would take no more than half of the places, or while one request would outlast the others.  One request on 1,000 keys: one block of
+    eight warps 14.4, several 12.3; on 100,000: a cluster of sixteen blocks 71.7, several 46.6; 16 requests on 1,000: 16.4, 18.4; on 4,000: 34.8, 30.7; one on 100,000
+    among 63 on 500: 580, 63.  The two costs below are fits to such figures.
     Blocks of eight warps rather than four while places are left, or while the longest row would outlast the others: 48 requests on 3,000 keys 43.0, 49.2; 96 on
     8,000 143, 154; 64 on 500 22.5, 20.5; 200 on 2,300 107, 96."""
     slots = sms * (2 if head_dim > 128 else 3 if n_blocks > 1 else 6 if head_dim == 64 else 4)  # blocks of four warps that the SMs hold
     total = rows * per_row
-    room = slots // per_row if per_row <= slots else 0  # blocks of a kv head of all rows
     if lengths is None:
-        return (4, min(KV4_PARTS_MAX, room // rows), 8) if total * 2 <= slots else (8 if total <= 2 * sms else 4, 1, 0)
+        return (4, min(KV4_PARTS_MAX, slots // total), 8) if total * 2 <= slots else (8 if total <= 2 * sms else 4, 1, 0)
     tiles = [-(-n // KV4_TILE) for n in lengths]
-    longest = max(tiles)
-    if total * 2 <= slots:
-        least = max(4, -(-sum(tiles) // room), -(-longest // KV4_PARTS_MAX))
-        while sum(-(-t // least) for t in tiles) > room:
-            least += 1
-        splits, wave = -(-longest // least), sum(-(-t // least) for t in tiles) * per_row / slots
-        one = 9 + longest * 0.18 * head_dim / 128 * (1.5 if n_blocks > 1 else 1) * (1 if total <= sms else 1.5)
-        if splits > 1 and 12 + least * max(0.33, wave) * 0.9 * slots / sms * head_dim / 512 < one:
+    longest, all_tiles = max(tiles), sum(tiles)
+    rate = 0.75 * slots / sms * head_dim / 512                            # us a tile of each block while all places are taken
+    chain = 0.18 * head_dim / 128 * (1.5 if n_blocks > 1 else 1)          # us a tile of a block of eight warps, one an SM
+    if longest > 4 and (total * 2 <= slots or longest * chain > 2 * (10 + all_tiles * per_row / slots * rate)):
+        room = max(slots // per_row, 2 * rows)  # blocks of a kv head of all rows
+        least = max(4, -(-all_tiles // room), -(-longest // KV4_PARTS_MAX))
+        while (blocks := sum(-(-t // least) for t in tiles)) > room:
+            least += 1 + least // 16
+        splits, wave = -(-longest // least), blocks * per_row / slots
+        if splits > 1 and 12 + 2 * wave + least * max(0.33, wave) * rate < 9 + longest * chain * (1 if total <= sms else 1.5):
             return 4, splits, least
     return 8 if total <= 2 * sms or total * 32 <= sms * longest else 4, 1, 0
+
+
+def kv4_jobs(lengths: tuple[int, ...], least: int) -> list[int]:
+    """(row, part, parts) of every block's share of a row's tiles, then (first of them, parts) of every row."""
+    jobs, spans = [], []
+    for z, n in enumerate(lengths):
+        parts = max(1, -(-n // (KV4_TILE * least)))
+        spans += (len(jobs) // 3, parts)
+        for p in range(parts):
+            jobs += (z, p, parts)
+    return jobs + spans
 
 
 def kv4_token_tiles(requests: list[tuple[int, int, int]], group: int) -> tuple[list[tuple[int, int]], int]:
@@ -183,10 +196,9 @@ def _kv4_plan(ctx, group: int, nkv: int, head_dim: int, window: int, tensor_core
         return plan
     total = ctx.positions.numel()
     on_device = lambda v: torch.tensor(v, dtype=torch.int32).to(ctx.device, non_blocking=True) if v else None  # noqa: E731
-    sms = sm_count()
     if ctx.extras.get("graph"):  # every row is a request's one token, and lengths are the device's
-        plan = {"rows": None, "n_rows": total, "longest": None, "portions": [],
-                "runs": _kv4_runs(None, None, total, (window,) * total if window else None, nkv, group, head_dim, 1 if group <= 8 else 2, sms, ctx.device) if tensor_core else []}
+        plan = {"rows": None, "n_rows": total, "longest": None, "held": 0, "requests": 0, "portions": [],
+                "runs": [_kv4_run(None, None, total, (window,) * total if window else None, nkv, group, head_dim, 1 if group <= 8 else 2)] if tensor_core and total else []}
     else:
         if sum(ctx.q_lens) > total:
             raise KernelError(f"attention_kv4: the requests bring {sum(ctx.q_lens)} tokens, the step holds {total}")
@@ -195,20 +207,22 @@ def _kv4_plan(ctx, group: int, nkv: int, head_dim: int, window: int, tensor_core
             starts.append(row)
             row += n
         requests = list(zip(starts, ctx.q_lens, ctx.kv_lens))
-        long = kv4_unfolded(list(zip(ctx.q_lens, ctx.kv_lens)), group, nkv, head_dim, window, sms, tensor_core) if unfold else []
+        long = kv4_unfolded(list(zip(ctx.q_lens, ctx.kv_lens)), group, nkv, head_dim, window, sm_count(), tensor_core) if unfold else []
         rest = [(s, n, kv) for i, (s, n, kv) in enumerate(requests) if i not in set(long)]
         rest.sort(key=lambda r: -r[2])  # the longest first: blocks are scheduled in this order
         rows = [s + i for s, n, _ in rest for i in range(n) if n == 1 or not tensor_core]
         plan = {"rows": None if rows == list(range(total)) else on_device(rows), "n_rows": len(rows),
-                "longest": max((kv for _, n, kv in rest if n == 1 or not tensor_core), default=0), "portions": [], "runs": []}
+                "longest": max((kv for _, n, kv in rest if n == 1 or not tensor_core), default=0), "held": max(ctx.kv_lens, default=0),
+                "requests": len(ctx.kv_lens), "portions": [], "runs": []}
         if tensor_core:
             seen = tuple(min(kv, window or kv) for _, n, kv in rest if n == 1)
-            plan["runs"] += _kv4_runs(plan["rows"], None, len(rows), seen, nkv, group, head_dim, 1 if group <= 8 else 2, sms, ctx.device)
+            if rows:
+                plan["runs"].append(_kv4_run(plan["rows"], None, len(rows), seen, nkv, group, head_dim, 1 if group <= 8 else 2, on_device))
             few = [r for r in rest if r[1] > 1]
             if few:
                 tiles, n_blocks = kv4_token_tiles(few, group)
                 keys = {row + i: min(kv, window + n) if window else kv for row, n, kv in few for i in range(n)}
-                plan["runs"] += _kv4_runs(None, on_device(tiles), len(tiles), tuple(keys[row] for row, _ in tiles), nkv, group, head_dim, n_blocks, sms, ctx.device)
+                plan["runs"].append(_kv4_run(None, on_device(tiles), len(tiles), tuple(keys[row] for row, _ in tiles), nkv, group, head_dim, n_blocks, on_device))
         for first, count, head, heads in kv4_unfold_runs([-(-ctx.kv_lens[i] // KV4_UNFOLD_PAGE) - _first_chunk(ctx, i, window) for i in long], nkv, head_dim,
                                                          KV4_UNFOLD_MAX):
             plan["portions"].append(_kv4_portion(ctx, long[first: first + count], window, head, heads, on_device))
@@ -216,19 +230,15 @@ def _kv4_plan(ctx, group: int, nkv: int, head_dim: int, window: int, tensor_core
     return plan
 
 
-KV4_GRID_MAX = 65535  # rows, or tiles, of one launch
-
-
-def _kv4_runs(rows, items, count: int, lengths, nkv: int, group: int, head_dim: int, n_blocks: int, sms: int, device) -> list[tuple]:
-    """(rows, items, how many, n-blocks of columns, shape of the launch) of the launches that take `count` rows, or tiles of tokens."""
-    if count > KV4_GRID_MAX and rows is None and items is None:
-        rows = torch.arange(count, dtype=torch.int32, device=device)
-    runs, per_row = [], nkv * -(-group // (8 * n_blocks))
-    for at in range(0, count, KV4_GRID_MAX):
-        part, n = slice(at, at + KV4_GRID_MAX), min(KV4_GRID_MAX, count - at)
-        runs.append((None if rows is None else rows[part], None if items is None else items[part], n, n_blocks, per_row,
-                     kv4_shape(lengths and lengths[part], n, per_row, sms, head_dim, n_blocks)))
-    return runs
+def _kv4_run(rows, items, count: int, lengths, nkv: int, group: int, head_dim: int, n_blocks: int, on_device=None) -> tuple:
+    """What the launch for `count` rows, or tiles of tokens, is: (rows, items, how many, n-blocks of columns, shape, jobs, how many, floats of the workspace)."""
+    per_row = nkv * -(-group // (8 * n_blocks))
+    warps, splits, least = kv4_shape(lengths, count, per_row, sm_count(), head_dim, n_blocks)
+    units, jobs = (count * splits, None) if least else (0, None)
+    if least and on_device:
+        listed = kv4_jobs(lengths, least)
+        units, jobs = (len(listed) - 2 * count) // 3, on_device(listed)
+    return rows, items, count, n_blocks, (warps, splits, least), jobs, units if jobs is not None else 0, units * per_row * 8 * n_blocks * (head_dim + 2)
 
 
 def _first_chunk(ctx, i: int, window: int) -> int:
@@ -300,6 +310,8 @@ def attention_kv4(qkv: torch.Tensor, lane, ctx, out: torch.Tensor, nq: int, nkv:
     tensor_core = kv4_tensor_core_ok(qkv.dtype, head_dim, lane.page_size)
     unfold = code == BF16 and head_dim <= 128 and ldq % 8 == 0 and ldo % 2 == 0 and qkv.data_ptr() % 16 == 0 and out.data_ptr() % 4 == 0
     plan = _kv4_plan(ctx, group, nkv, head_dim, window, tensor_core, unfold)
+    if plan["held"] > lane.block_table.shape[1] * lane.page_size or plan["requests"] > lane.block_table.shape[0]:
+        raise KernelError(f"attention_kv4: {plan['requests']} requests of up to {plan['held']} positions, the block table holds {tuple(lane.block_table.shape)} pages of {lane.page_size}")
     if plan["n_rows"] and not tensor_core:
         longest, splits = plan["longest"], 1
         if window and longest is not None:
@@ -310,11 +322,11 @@ def attention_kv4(qkv: torch.Tensor, lane, ctx, out: torch.Tensor, nq: int, nkv:
         lib.call("ns_attention_kv4", qkv.data_ptr(), qkv.stride(0), lane.k.data_ptr(), lane.v.data_ptr(), lane.block_table.data_ptr(),
                  lane.block_table.stride(0), ctx.token_req.data_ptr(), ctx.positions.data_ptr(), _ptr(plan["rows"]), plan["n_rows"], out.data_ptr(),
                  out.stride(0), nq, nkv, head_dim, lane.page_size, scale, window, _ptr(sink), splits, code, _stream())
-    for rows, items, count, n_blocks, per_row, (warps, splits, least) in plan["runs"]:
-        part = torch.empty(count * per_row * splits * 8 * n_blocks * (head_dim + 2), dtype=torch.float32, device=out.device) if least else None
+    for rows, items, count, n_blocks, (warps, splits, least), jobs, n_jobs, floats in plan["runs"]:
+        part = torch.empty(floats, dtype=torch.float32, device=out.device) if floats else None
         lib.call("ns_attention_kv4_tc", qkv.data_ptr(), ldq, lane.k.data_ptr(), lane.v.data_ptr(), lane.block_table.data_ptr(), lane.block_table.stride(0),
                  ctx.token_req.data_ptr(), ctx.positions.data_ptr(), _ptr(rows), _ptr(items), count, out.data_ptr(), ldo, nq, nkv, head_dim, lane.page_size,
-                 scale, window, _ptr(sink), n_blocks, warps, splits, _ptr(part), least, _stream())
+                 scale, window, _ptr(sink), n_blocks, warps, splits, _ptr(part), _ptr(jobs), n_jobs, least, _stream())
     for portion in plan["portions"]:
         _attend_unfolded(qkv, lane, ctx, out, nkv, group, head_dim, scale, window, sink, portion)
     return out

@@ -99,16 +99,23 @@ def test_tiles_of_a_few_tokens():
 def test_shape_of_a_launch(head_dim, n_blocks, resident):
     from nanospec_b200 import ops
     for per_row in (1, 2, 8, 1000):
-        for lengths in ((1,), (0,), (33,), (1000,), (100000,), (3000000,), (100000, 61000), (5, 100000), (700,) * 16, (4000,) * 16, (2300, 500) * 32, (9,) * 5000):
+        for lengths in ((1,), (0,), (33,), (1000,), (100000,), (3000000,), (100000, 61000), (5, 100000), (700,) * 16, (4000,) * 16, (2300, 500) * 32, (9,) * 5000,
+                        (100000,) + (500,) * 63):
+            slots, rows = 148 * resident, len(lengths)
             for known in (True, False):
-                warps, splits, least = ops.kv4_shape(lengths if known else None, len(lengths), per_row, 148, head_dim, n_blocks)
+                warps, splits, least = ops.kv4_shape(lengths if known else None, rows, per_row, 148, head_dim, n_blocks)
                 assert warps in (4, 8) and 1 <= splits <= 256 and (least > 0) == (splits > 1)
-                if splits > 1:
-                    assert warps == 4 and len(lengths) * per_row * 2 <= 148 * resident
-                    if known:  # every block has its place at once
-                        assert least >= 4 and per_row * sum(-(-n // (32 * least)) for n in lengths) <= 148 * resident
-                        assert splits == -(-max(lengths) // (32 * least))
-                    else:
-                        assert len(lengths) * per_row * splits <= 148 * resident
+                if splits > 1 and known:
+                    jobs = ops.kv4_jobs(lengths, least)
+                    n = (len(jobs) - 2 * rows) // 3
+                    assert warps == 4 and least >= 4 and n <= max(slots // per_row, 2 * rows)  # every block has its place at once, or two waves at most
+                    spans = [jobs[3 * n + 2 * z: 3 * n + 2 * z + 2] for z in range(rows)]
+                    for (first, parts), keys in zip(spans, lengths):
+                        assert parts == max(1, -(-keys // (32 * least))) <= splits
+                    assert [jobs[3 * i: 3 * i + 3] for i in range(n)] == [[z, p, parts] for z, (_, parts) in enumerate(spans) for p in range(parts)]
+                    assert [first for first, _ in spans] == [sum(parts for _, parts in spans[:z]) for z in range(rows)]
+                elif splits > 1:
+                    assert rows * per_row * splits <= slots
+    assert ops.kv4_shape((100000,) + (500,) * 63, 64, 8, 148, 128)[1] > 50  # (one request would outlast all others)
     assert ops.kv4_shape((100000,), 1, 1, 148, 128)[1] > 200  # (one kv head: more blocks than are joined would find a place)
     assert ops.kv4_shape((100000,), 1, 8, 148, 128)[1] > 60 and ops.kv4_shape((16,), 1, 8, 148, 128) == (8, 1, 0)

@@ -399,19 +399,20 @@ def test_portions_beyond_what_is_unfolded_at_a_time(monkeypatch):
         assert torch.equal(got, want)
 
 
-def test_more_rows_than_a_grid_holds(monkeypatch):
+def test_more_rows_than_a_grid_dimension_holds():
     from nanospec_b200 import ops
-    from nanospec_b200.ops import kv4
-    for lens in ([(i, 1) for i in range(40)], [(i, 3) for i in range(20)]):
-        ctx, lane, qkv = step(lens, 16, 2, 64, BF16, 4)
-        fill(ctx, lane, 4, 2, 64)
-        monkeypatch.setattr(kv4, "KV4_GRID_MAX", 65535)
-        monkeypatch.setattr(kv4, "kv4_shape", lambda *a: (4, 2, 1))
-        want = ops.attention_kv4(qkv, lane, ctx, torch.zeros((ctx.n_tokens, 256), dtype=BF16, device="cuda"), 4, 2, 64)
-        monkeypatch.setattr(kv4, "KV4_GRID_MAX", 7)
-        ctx.extras = {}
-        got = ops.attention_kv4(qkv, lane, ctx, torch.zeros_like(want), 4, 2, 64)
-        assert torch.equal(got, want)
+    rows = 66000
+    ctx, lane, qkv = step([(i, 1) for i in range(40)], 8, 1, 64, BF16, 1)
+    k, v = fill(ctx, lane, 1, 1, 64)
+    want, tol, _ = attend(qkv[:, :64], k, v, ctx, 1, 0.125)
+    tol = tol + want.abs() * 1.01 * half_step(BF16)
+    many = torch.arange(rows, device="cuda") % 40  # the same requests over and over
+    ctx.positions, ctx.token_req, lane.block_table = ctx.positions[many], torch.arange(rows, dtype=torch.int32, device="cuda"), lane.block_table[many]
+    ctx.q_lens, ctx.kv_lens = [1] * rows, [i % 40 + 1 for i in range(rows)]
+    for graph in (False, True):
+        ctx.extras = {"graph": True} if graph else {}
+        got = ops.attention_kv4(qkv[many], lane, ctx, torch.empty((rows, 64), dtype=BF16, device="cuda"), 1, 1, 64)
+        _near(got.double().reshape(rows, *want.shape[1:]), want[many], tol[many])
 
 
 def test_two_calls_at_once():
@@ -487,7 +488,7 @@ def test_requests_over_several_blocks(nq, nkv, dim, page, tokens, monkeypatch):
             for shape in (None, (4, 1, 0), (8, 1, 0), (4, 256, 1), (4, 7, 9), (4, 2, 100), (8, 3, 1)):
                 if shape:
                     monkeypatch.setattr(kv4, "kv4_shape", lambda *a: shape)
-                ctx.extras = {"graph": True} if graph else {}
+                ctx.extras = {"graph": True} if graph else {}  # (with the blocks of each row listed, or as many for every row)
                 out = torch.full((ctx.n_tokens, nq * dim), 5.0, dtype=BF16, device="cuda")
                 ops.attention_kv4(qkv, lane, ctx, out, nq, nkv, dim, window=window, sink=sink)
                 _near(out[:n].double().reshape(want.shape), want, tol)
@@ -548,6 +549,7 @@ def test_cache_refusals():
         lambda: attn(qkv.half()), lambda: attn(out=out.float()), lambda: attn(out=out[:, :-1]), lambda: attn(nq=3), lambda: attn(window=-1),
         lambda: attn(qkv[:, :200]), lambda: attn(sink=torch.zeros(3, device="cuda")), lambda: attn(sink=torch.zeros(4, device="cuda", dtype=BF16)),
         lambda: attn(lane=other(lane, v=lane.v.int())), lambda: attn(dim=288), lambda: attn(out=out.cpu()), lambda: attn(ctx=other(ctx, positions=ctx.positions[:1])),
+        lambda: attn(ctx=other(ctx, kv_lens=[33], extras={})), lambda: attn(lane=other(lane, block_table=lane.block_table[:0])),
         lambda: ops.kv4_read(lane, ctx.positions.long(), ctx.token_req, 2, 64), lambda: ops.kv4_read(lane, ctx.positions, ctx.token_req[:1], 2, 64),
         lambda: ops.kv4_pages(3, 2, 0, 64), lambda: ops.kv4_pages(3, 2, 16, 288), lambda: ops.kv4_pages(3, 2, 16, 40),
     ]
