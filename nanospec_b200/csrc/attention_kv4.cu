@@ -1,17 +1,20 @@
 // Attention over the 4-bit cache (kv4.cuh) for every head size, page size and type: softmax(q k^T scale) v over the positions
 // max(0, p - window + 1) .. p of a token at position p, in float from the cached values on.
 //
-// A block takes a token and up to eight query heads of a kv head; its eight warps, and those of up to seven more blocks of a cluster, take tiles of 32 keys in turn, each with a
-// running maximum and sum of its own, and are joined at the end in a fixed order.  Scores: a lane holds a key; weighted values: a lane holds features, and asks for the
-// codes of eight keys before it uses the first (one at a time, the latency of each bounds the kernel: 2,236 keys of 16 heads of 32 168 us).
+// A block takes a token and two, four or eight query heads of a kv head; its eight warps, and those of up to seven more blocks of a cluster, take tiles of 32 keys in
+// turn, each with a running maximum and sum of its own, and are joined at the end in a fixed order.  Scores: a lane holds a key; weighted values: a lane holds
+// features, and asks for the codes of eight keys before it uses the first (one at a time, the latency of each bounds the kernel: 2,236 keys of 16 heads of 32 168 us).
+//
+// Bound by its float arithmetic, two fused multiply-adds a feature, key and head, and by the reads of shared memory that feed them.  64 requests on up to 2,000 keys,
+// four heads to each of 8 kv heads of 128: 162 us, 256 where every block computed for eight heads; four portions of up to 64 tokens on up to 500: 145, 273.
 #include "kv4.cuh"
 #include "tcgen05_utils.cuh"
 
 namespace {
 
-constexpr int kWarps = 8, kThreads = 32 * kWarps, kHeads = 8, kAhead = 8;
+constexpr int kWarps = 8, kThreads = 32 * kWarps, kAhead = 8;
 
-template <typename T, int kChunks>  // kChunks of 128 features
+template <typename T, int kChunks, int kHeads>  // kChunks of 128 features, kHeads query heads
 __global__ void __launch_bounds__(kThreads)
 attention_kv4_kernel(const T* __restrict__ q, long long ldq, const uint8_t* __restrict__ k_pages, const uint8_t* __restrict__ v_pages,
                      const int* __restrict__ block_table, int table_stride, const int* __restrict__ token_req, const int* __restrict__ positions,
@@ -176,11 +179,11 @@ int launch(const void* q, long long ldq, const void* k, const void* v, const int
            const int* rows, int n_rows, void* out, long long ldo, int nq, int nkv, int D, int page_size, float scale, int window, const float* sink,
            int splits, cudaStream_t stream) {
     const int G = nq / nkv;
-    auto run = [&](auto* kernel, int chunks, std::atomic<unsigned long long>& allowed) -> int {
-        const int bytes = kWarps * kHeads * 128 * chunks * 4;
+    auto run = [&](auto* kernel, int chunks, int heads, std::atomic<unsigned long long>& allowed) -> int {
+        const int bytes = kWarps * heads * 128 * chunks * 4;
         NS_CUDA(ns_allow_smem((const void*)kernel, bytes, allowed));
         cudaLaunchConfig_t cfg = {};
-        cfg.gridDim = dim3(n_rows * splits, nkv * ((G + kHeads - 1) / kHeads));
+        cfg.gridDim = dim3(n_rows * splits, nkv * ((G + heads - 1) / heads));
         cfg.blockDim = dim3(kThreads);
         cfg.dynamicSmemBytes = bytes;
         cfg.stream = stream;
@@ -203,8 +206,15 @@ int launch(const void* q, long long ldq, const void* k, const void* v, const int
         NS_CHECK_LAUNCH("ns_attention_kv4");
         return NS_OK;
     };
-    static std::atomic<unsigned long long> one{0}, two{0};
-    return D <= 128 ? run(attention_kv4_kernel<T, 1>, 1, one) : run(attention_kv4_kernel<T, 2>, 2, two);
+#define NS_KV4_HEADS(H)                                                                                   \
+    {                                                                                                      \
+        static std::atomic<unsigned long long> one{0}, two{0};                                            \
+        return D <= 128 ? run(attention_kv4_kernel<T, 1, H>, 1, H, one) : run(attention_kv4_kernel<T, 2, H>, 2, H, two); \
+    }
+    if (G <= 2) NS_KV4_HEADS(2)
+    if (G <= 4) NS_KV4_HEADS(4)
+    NS_KV4_HEADS(8)
+#undef NS_KV4_HEADS
 }
 
 }  // namespace
@@ -216,7 +226,7 @@ NS_API int ns_attention_kv4(const void* q, long long ldq, const void* k, const v
     if (n_rows <= 0) return NS_OK;
     if (D < kGroup || D % kGroup || D > 256 || nkv < 1 || nq < 1 || nq % nkv || page_size < 1 || window < 0)
         NS_FAIL(NS_ERR_UNSUPPORTED, "ns_attention_kv4: %d heads of %d over %d, pages of %d, a window of %d", nq, D, nkv, page_size, window);
-    if (nkv * ((nq / nkv + kHeads - 1) / kHeads) > 65535) NS_FAIL(NS_ERR_UNSUPPORTED, "ns_attention_kv4: too many heads (%d)", nq);
+    if (nkv * ((nq / nkv + 7) / 8) > 65535) NS_FAIL(NS_ERR_UNSUPPORTED, "ns_attention_kv4: too many heads (%d)", nq);
     if (splits < 1 || splits > 8 || (splits & (splits - 1)) || (long long)n_rows * splits > 0x7fffffff) NS_FAIL(NS_ERR_ARGUMENT, "ns_attention_kv4: %d blocks to each of %d tokens", splits, n_rows);
     if (dtype == NS_BF16)
         return launch<__nv_bfloat16>(q, ldq, k, v, table, table_stride, token_req, positions, rows, n_rows, out, ldo, nq, nkv, D, page_size, scale, window, sink, splits, stream);

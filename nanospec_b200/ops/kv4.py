@@ -152,14 +152,14 @@ def kv4_unfolded(requests: list[tuple[int, int]], group: int, nkv: int, head_dim
     tokens.  From the bytes the keys are unpacked again for every 16 (query head, token) pairs: about 17,000 keys of a head of 128 a us; unfolded they cost 3.3
     MB a us, and a block of 256 tokens of a head takes 11 ns a key, one block an SM.  Us on a B200, from the bytes / unfolded, heads of 128, 4 to each of
     8 kv heads: one request on 30,000 positions, 64 tokens 202 / 328, 96 378 / 330; 8 on 3,000, 24 tokens 74 / 104, 48 137 / 104; 32 on 1,000, 32
-    tokens 141 / 152, 48 203 / 154; 8 on 500, 24 tokens 27 / 34, 48 45 / 35.  Without the tensor cores a token goes by itself, 2,000 keys a us."""
+    tokens 141 / 152, 48 203 / 154; 8 on 500, 24 tokens 27 / 34, 48 45 / 35.  Without the tensor cores a token goes by itself, 3,000 keys a us."""
     scale = head_dim / 128
     cost = []  # (request, from the bytes, unfolding and blocks together, one block)
     for i, (n, kv) in enumerate(requests):
         if n < 2:
             continue
         seen = min(kv, window + n) if window else kv
-        packed = -(-n * group // 16) * seen * nkv * scale / 17000 if tensor_core else n * -(-group // 8) * seen * nkv * scale / 2000
+        packed = -(-n * group // 16) * seen * nkv * scale / 17000 if tensor_core else n * -(-group // 8) * seen * nkv * scale / 3000
         cost.append((i, packed, seen * nkv * head_dim * 4 / 3.3e6 + nkv * group * -(-n // 256) * seen * 0.011 / sms, seen * 0.011))
     chosen = [c for c in cost if c[1] > c[2]]
     if not chosen or sum(c[1] for c in chosen) < 10 + max(sum(c[2] for c in chosen), max(c[3] for c in chosen)):
