@@ -425,14 +425,15 @@ attention_kv4_join_kernel(const float* __restrict__ part, const int* __restrict_
     const int per_row = nkv * head_tiles, z = (int)blockIdx.x / per_row, y = (int)blockIdx.x - z * per_row;
     const Place at(z, y, items, rows, token_req, positions, nq, nkv, head_tiles, kCols, window);
     const int c = blockIdx.y, warp = threadIdx.x >> 5;
-    if (at.req < 0 || c >= at.cols) return;
-    const int blocks = spans ? spans[2 * z + 1] : at.parts(splits, least), h = at.h0 + c % at.heads;
+    const int blocks = spans ? spans[2 * z + 1] : at.parts(splits, least);
     const size_t each = (size_t)per_row * kCols * (D + 2);  // from a part of the row to its next one
     const float* from = part + ((size_t)(spans ? spans[2 * z] : z * splits) * per_row + y) * kCols * (D + 2);
-    const float sink2 = sink ? sink[h] * kLog2e : -INFINITY;
     static_assert(kMostParts <= kJoinThreads, "a thread a part");
     float2 ml = make_float2(-INFINITY, 0.f);
-    if (threadIdx.x < blocks) ml = *reinterpret_cast<const float2*>(from + threadIdx.x * each + 2 * c);
+    if (threadIdx.x < blocks) ml = *reinterpret_cast<const float2*>(from + threadIdx.x * each + 2 * c);  // (under way while the row is looked up, whatever it is)
+    if (at.req < 0 || c >= at.cols) return;
+    const int h = at.h0 + c % at.heads;
+    const float sink2 = sink ? sink[h] * kLog2e : -INFINITY;
     float top = ml.x;
 #pragma unroll
     for (int d = 16; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
