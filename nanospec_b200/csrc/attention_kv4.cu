@@ -14,8 +14,10 @@ namespace {
 
 constexpr int kWarps = 8, kThreads = 32 * kWarps, kAhead = 8;
 
-template <typename T, int kChunks, int kHeads>  // kChunks of 128 features, kHeads query heads
-__global__ void __launch_bounds__(kThreads)
+// kChunks of 128 features, kHeads query heads.  Two blocks an SM, which costs eight heads a few spilled registers: 16 requests on up to 2,000 keys, eight heads to each of 4
+// kv heads of 128: 64 us with one block, 49 with two.
+template <typename T, int kChunks, int kHeads>
+__global__ void __launch_bounds__(kThreads, kChunks == 1 ? 2 : 1)
 attention_kv4_kernel(const T* __restrict__ q, long long ldq, const uint8_t* __restrict__ k_pages, const uint8_t* __restrict__ v_pages,
                      const int* __restrict__ block_table, int table_stride, const int* __restrict__ token_req, const int* __restrict__ positions,
                      const int* __restrict__ rows, T* __restrict__ out, long long ldo, int nq, int nkv, int D, int page_size, float scale, int window,
