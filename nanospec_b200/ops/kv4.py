@@ -187,7 +187,13 @@ def kv4_unfold_runs(chunks: list[int], nkv: int, head_dim: int, limit: int) -> l
     return runs
 
 
-def _kv4_plan(ctx, group: int, nkv: int, head_dim: int, window: int, tensor_core: bool, unfold: bool) -> dict:
+def _check_table(lane, held: int, requests: int) -> None:
+    rows, columns = lane.block_table.shape
+    if held > columns * lane.page_size or requests > rows:
+        raise KernelError(f"attention_kv4: {requests} requests of up to {held} positions, the block table has {rows} rows of {columns} pages of {lane.page_size}")
+
+
+def _kv4_plan(ctx, lane, group: int, nkv: int, head_dim: int, window: int, tensor_core: bool, unfold: bool) -> dict:
     """Once per step and kind of layer: which rows run by themselves, the tiles of a few tokens, and the portions that are unfolded.  `tensor_core`: rows and
     tiles are those of csrc/attention_kv4_tc.cu; else rows alone, of csrc/attention_kv4.cu."""
     key = ("kv4_plan", group, nkv, head_dim, window, tensor_core, unfold)
@@ -195,24 +201,34 @@ def _kv4_plan(ctx, group: int, nkv: int, head_dim: int, window: int, tensor_core
     if plan is not None:
         return plan
     total = ctx.positions.numel()
-    on_device = lambda v: torch.tensor(v, dtype=torch.int32).to(ctx.device, non_blocking=True) if v else None  # noqa: E731
+    made = []
+
+    def on_device(v):
+        if not v:
+            return None
+        made.append(torch.tensor(v, dtype=torch.int32).to(ctx.device, non_blocking=True))
+        return made[-1]
+
     if ctx.extras.get("graph"):  # every row is a request's one token, and lengths are the device's
         plan = {"rows": None, "n_rows": total, "longest": None, "held": 0, "requests": 0, "portions": [],
                 "runs": [_kv4_run(None, None, total, (window,) * total if window else None, nkv, group, head_dim, 1 if group <= 8 else 2)] if tensor_core and total else []}
     else:
         if sum(ctx.q_lens) > total:
             raise KernelError(f"attention_kv4: the requests bring {sum(ctx.q_lens)} tokens, the step holds {total}")
+        held = max(ctx.kv_lens, default=0)
+        _check_table(lane, held, len(ctx.kv_lens))
         starts, row = [], 0
         for n in ctx.q_lens:
             starts.append(row)
             row += n
         requests = list(zip(starts, ctx.q_lens, ctx.kv_lens))
         long = kv4_unfolded(list(zip(ctx.q_lens, ctx.kv_lens)), group, nkv, head_dim, window, sm_count(), tensor_core) if unfold else []
-        rest = [(s, n, kv) for i, (s, n, kv) in enumerate(requests) if i not in set(long)]
+        unfolded = set(long)
+        rest = [(s, n, kv) for i, (s, n, kv) in enumerate(requests) if i not in unfolded]
         rest.sort(key=lambda r: -r[2])  # the longest first: blocks are scheduled in this order
         rows = [s + i for s, n, _ in rest for i in range(n) if n == 1 or not tensor_core]
         plan = {"rows": None if rows == list(range(total)) else on_device(rows), "n_rows": len(rows),
-                "longest": max((kv for _, n, kv in rest if n == 1 or not tensor_core), default=0), "held": max(ctx.kv_lens, default=0),
+                "longest": max((kv for _, n, kv in rest if n == 1 or not tensor_core), default=0), "held": held,
                 "requests": len(ctx.kv_lens), "portions": [], "runs": []}
         if tensor_core:
             seen = tuple(min(kv, window or kv) for _, n, kv in rest if n == 1)
@@ -226,8 +242,24 @@ def _kv4_plan(ctx, group: int, nkv: int, head_dim: int, window: int, tensor_core
         for first, count, head, heads in kv4_unfold_runs([-(-ctx.kv_lens[i] // KV4_UNFOLD_PAGE) - _first_chunk(ctx, i, window) for i in long], nkv, head_dim,
                                                          KV4_UNFOLD_MAX):
             plan["portions"].append(_kv4_portion(ctx, long[first: first + count], window, head, heads, on_device))
+        if made:  # (a captured step has none)
+            ready = torch.cuda.Event()
+            ready.record()
+            plan.update(lists=made, ready=ready, streams={_stream()})
     ctx.extras[key] = plan
     return plan
+
+
+def _plan_on_this_stream(plan: dict, stream: int) -> None:
+    """The plan's lists go to the device on the stream of the step's first call; a call on another one waits for them there."""
+    streams = plan.get("streams")
+    if streams is None or stream in streams or torch.cuda.is_current_stream_capturing():
+        return
+    here = torch.cuda.current_stream()
+    here.wait_event(plan["ready"])
+    for t in plan["lists"]:
+        t.record_stream(here)
+    streams.add(stream)
 
 
 def _kv4_run(rows, items, count: int, lengths, nkv: int, group: int, head_dim: int, n_blocks: int, on_device=None) -> tuple:
@@ -309,9 +341,9 @@ def attention_kv4(qkv: torch.Tensor, lane, ctx, out: torch.Tensor, nq: int, nkv:
     group, sms, window = nq // nkv, sm_count(), min(int(window), 1 << 30)
     tensor_core = kv4_tensor_core_ok(qkv.dtype, head_dim, lane.page_size)
     unfold = code == BF16 and head_dim <= 128 and ldq % 8 == 0 and ldo % 2 == 0 and qkv.data_ptr() % 16 == 0 and out.data_ptr() % 4 == 0
-    plan = _kv4_plan(ctx, group, nkv, head_dim, window, tensor_core, unfold)
-    if plan["held"] > lane.block_table.shape[1] * lane.page_size or plan["requests"] > lane.block_table.shape[0]:
-        raise KernelError(f"attention_kv4: {plan['requests']} requests of up to {plan['held']} positions, the block table holds {tuple(lane.block_table.shape)} pages of {lane.page_size}")
+    plan, stream = _kv4_plan(ctx, lane, group, nkv, head_dim, window, tensor_core, unfold), _stream()
+    _check_table(lane, plan["held"], plan["requests"])
+    _plan_on_this_stream(plan, stream)
     if plan["n_rows"] and not tensor_core:
         longest, splits = plan["longest"], 1
         if window and longest is not None:
@@ -321,12 +353,12 @@ def attention_kv4(qkv: torch.Tensor, lane, ctx, out: torch.Tensor, nq: int, nkv:
             splits *= 2
         lib.call("ns_attention_kv4", qkv.data_ptr(), qkv.stride(0), lane.k.data_ptr(), lane.v.data_ptr(), lane.block_table.data_ptr(),
                  lane.block_table.stride(0), ctx.token_req.data_ptr(), ctx.positions.data_ptr(), _ptr(plan["rows"]), plan["n_rows"], out.data_ptr(),
-                 out.stride(0), nq, nkv, head_dim, lane.page_size, scale, window, _ptr(sink), splits, code, _stream())
+                 out.stride(0), nq, nkv, head_dim, lane.page_size, scale, window, _ptr(sink), splits, code, stream)
     for rows, items, count, n_blocks, (warps, splits, least), jobs, n_jobs, floats in plan["runs"]:
         part = torch.empty(floats, dtype=torch.float32, device=out.device) if floats else None
         lib.call("ns_attention_kv4_tc", qkv.data_ptr(), ldq, lane.k.data_ptr(), lane.v.data_ptr(), lane.block_table.data_ptr(), lane.block_table.stride(0),
                  ctx.token_req.data_ptr(), ctx.positions.data_ptr(), _ptr(rows), _ptr(items), count, out.data_ptr(), ldo, nq, nkv, head_dim, lane.page_size,
-                 scale, window, _ptr(sink), n_blocks, warps, splits, _ptr(part), _ptr(jobs), n_jobs, least, _stream())
+                 scale, window, _ptr(sink), n_blocks, warps, splits, _ptr(part), _ptr(jobs), n_jobs, least, stream)
     for portion in plan["portions"]:
         _attend_unfolded(qkv, lane, ctx, out, nkv, group, head_dim, scale, window, sink, portion)
     return out

@@ -434,6 +434,26 @@ def test_two_calls_at_once():
     ops.check_kernel_errors()
 
 
+@pytest.mark.parametrize("lens", [[(9, 1), (900, 1), (100, 1)], [(20, 1), (200, 3), (40, 90)]])
+@pytest.mark.parametrize("dim,dtype", [(128, BF16), (64, F32)])
+def test_a_step_whose_calls_run_on_several_streams(lens, dim, dtype):
+    """The first call's stream is late with the step's lists; the calls on others wait for them."""
+    from nanospec_b200 import ops
+    ctx, lane, qkv = step(lens, 16, 2, dim, dtype, 8)
+    fill(ctx, lane, 8, 2, dim, dtype)
+    want = ops.attention_kv4(qkv, lane, ctx, torch.zeros((ctx.n_tokens, 8 * dim), dtype=dtype, device="cuda"), 8, 2, dim)
+    outs = [torch.zeros_like(want) for _ in range(3)]
+    ctx.extras = {}
+    torch.cuda.synchronize()
+    for i, (out, s) in enumerate(zip(outs, [torch.cuda.Stream() for _ in outs])):
+        with torch.cuda.stream(s):
+            if i == 0:
+                torch.cuda._sleep(20_000_000)
+            ops.attention_kv4(qkv, lane, ctx, out, 8, 2, dim)
+    torch.cuda.synchronize()
+    assert all(torch.equal(out, want) for out in outs)
+
+
 @pytest.mark.parametrize("lens", [[(300, 1), (9, 1)], [(200, 3)], [(40, 90)]])
 @pytest.mark.parametrize("dim,dtype", [(128, BF16), (64, F32)])
 def test_sink_scale_and_padding(lens, dim, dtype):
