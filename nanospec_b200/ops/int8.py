@@ -95,7 +95,8 @@ def linear_i8(x: torch.Tensor | RowsI8, w: RowsI8, out: torch.Tensor, bias: torc
               tiles: tuple[int, int, int] | None = None) -> torch.Tensor:
     """out[n, f] = (sum_k xq[n, k] wq[f, k]) * xs[n] * ws[f] (+ bias[f], float32), the sum exact in 32-bit integers.  `x` [N, K] is quantised by
     rows on the way (`quantize_rows`) unless it comes so, for several products of the same activations; `out` [N, F] is float32 or bfloat16
-    with unit inner stride."""
+    with unit inner stride.  `tiles` (tokens and features of a tile, blocks or pairs that divide k): `i8_tiles`' choice when None; an output's
+    bits are the same in all of them."""
     ready = isinstance(x, RowsI8)
     held, wq, ws = x.q if ready else x, w.q, w.scale
     if ready:

@@ -50,7 +50,7 @@ def kv4_store(qkv: torch.Tensor, ctx, lane, nq: int, nkv: int, head_dim: int, in
     """Rotates q and k of the packed [q | k | v] rows (pairs j and j + head_dim / 2 by position * inv_freq[j]; None: as they are), writes k
     and v in 4 bits at each token's position, and q to `q_out` ([N, nq * head_dim]; None: in place).  The rotated k is rounded to the
     activations' type before it is quantised, as a cache in that type would hold it.  Rows of padding (token_req < 0) are left as they
-    are.  Returns where q went."""
+    are; no two rows of a step have the same position of the same request.  Returns where q went."""
     _on_current_device(qkv, ctx.positions, ctx.token_req, lane.block_table, lane.k, lane.v, inv_freq, q_out)
     _check_lane("kv4_store", lane, nkv, head_dim)
     code, size = dtype_code(qkv.dtype), qkv.element_size()
