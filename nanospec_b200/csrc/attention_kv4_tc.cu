@@ -70,8 +70,10 @@ struct Shape {
 struct Place {
     int n0, count, req, pos0, hk, h0, heads, cols, end, start, tile0, tiles;
     __device__ __forceinline__ Place(int z, int y, const int* items, const int* rows, const int* token_req, const int* positions, int nq, int nkv, int head_tiles,
-                                     int kCols, int window) {
-        n0 = items ? items[2 * z] : rows ? rows[z] : z, count = items ? items[2 * z + 1] : 1;
+                                     int kCols, int window)
+        : Place(items ? items[2 * z] : rows ? rows[z] : z, items ? items[2 * z + 1] : 1, y, token_req, positions, nq, nkv, head_tiles, kCols, window) {}
+    __device__ __forceinline__ Place(int row, int tokens, int y, const int* token_req, const int* positions, int nq, int nkv, int head_tiles, int kCols, int window) {
+        n0 = row, count = tokens;
         req = token_req[n0], pos0 = positions[n0];
         const int G = nq / nkv, ht = y % head_tiles, per = min(G, kCols);
         hk = y / head_tiles, h0 = hk * G + ht * per, heads = min(per, hk * G + G - h0);  // heads of a token here
@@ -92,7 +94,7 @@ attention_kv4_tc_kernel(const __nv_bfloat16* __restrict__ q, long long ldq, cons
                         const int* __restrict__ block_table, int table_stride, const int* __restrict__ token_req, const int* __restrict__ positions,
                         const int* __restrict__ rows, const int* __restrict__ items, __nv_bfloat16* __restrict__ out, long long ldo, int nq, int nkv,
                         int page_size, float scale, int window, const float* __restrict__ sink, int head_tiles, int splits, int page_shift, float* __restrict__ part,
-                        const int* __restrict__ jobs, int least) {
+                        const int4* __restrict__ jobs, int least) {
     using S = Shape<D, NB, kWarps>;
     constexpr int kThreads = S::kThreads;
     extern __shared__ __align__(128) unsigned char smem[];
@@ -105,14 +107,15 @@ attention_kv4_tc_kernel(const __nv_bfloat16* __restrict__ q, long long ldq, cons
     ns_pdl_wait();
 
     const int unit = (int)blockIdx.x / (nkv * head_tiles), y = (int)blockIdx.x - unit * nkv * head_tiles;  // (a row's heads come together: the longest rows first)
-    const int z = jobs ? jobs[3 * unit] : unit / splits, which_part = jobs ? jobs[3 * unit + 1] : unit - z * splits;
-    const Place at(z, y, items, rows, token_req, positions, nq, nkv, head_tiles, S::kCols, window);
+    const int z = unit / splits;
+    const int4 job = jobs ? jobs[unit] : make_int4(items ? items[2 * z] : rows ? rows[z] : z, items ? items[2 * z + 1] : 1, unit - z * splits, 0);  // row, tokens, part, of how many
+    const Place at(job.x, job.y, y, token_req, positions, nq, nkv, head_tiles, S::kCols, window);
     if (at.req < 0) return;  // a row of padding
     const int n0 = at.n0, pos0 = at.pos0, hk = at.hk, h0 = at.h0, heads = at.heads, cols = at.cols, end = at.end, start = at.start, tile0 = at.tile0, tiles = at.tiles;
     const int* bt = block_table + (size_t)at.req * table_stride;
-    const int blocks = jobs ? jobs[3 * unit + 2] : part ? at.parts(splits, least) : 1;
-    if (which_part >= blocks) return;
-    const int step = blocks * kWarps, first = which_part * kWarps + warp;
+    const int blocks = jobs ? job.w : part ? at.parts(splits, least) : 1;
+    if (job.z >= blocks) return;
+    const int step = blocks * kWarps, first = job.z * kWarps + warp;
 
     // a tile: 16-byte pieces, codes and pairs of keys and of values, from the pages that it lies in (1, 2 or 4)
     const int page_log = kPages == 1 ? 5 : kPages == 2 ? 4 : 31 - __clz(min(kTile, page_size)), pages = kTile >> page_log;  // keys of a page in a tile
@@ -502,13 +505,13 @@ int launch(const void* q, long long ldq, const void* k, const void* v, const int
     if (grid > 0x7fffffff) NS_FAIL(NS_ERR_UNSUPPORTED, "ns_attention_kv4_tc: %d tokens, %d heads exceed the grid", n, nq);
     NS_LAUNCH(kernel, (unsigned)grid, S::kThreads, S::kSmem, stream, (const __nv_bfloat16*)q, ldq, (const uint8_t*)k, (const uint8_t*)v, table,
               table_stride, token_req, positions, rows, items, (__nv_bfloat16*)out, ldo, nq, nkv, page_size, scale, window, sink, head_tiles, splits,
-              (page_size & (page_size - 1)) == 0 ? 31 - __builtin_clz(page_size) : -1, part, jobs, least);
+              (page_size & (page_size - 1)) == 0 ? 31 - __builtin_clz(page_size) : -1, part, reinterpret_cast<const int4*>(jobs), least);
     NS_CHECK_LAUNCH("ns_attention_kv4_tc");
     if (part) {
         const int columns = items ? S::kCols : nq / nkv < S::kCols ? nq / nkv : S::kCols, team = splits <= 8 ? 1 : splits <= 16 ? 2 : splits <= 32 ? 4 : 8;
         NS_LAUNCH((attention_kv4_join_kernel<D>), dim3((unsigned)(per_row * n), (columns * team + kJoinWarps - 1) / kJoinWarps), 32 * kJoinWarps, 0, stream, part,
                   token_req, positions, rows, items, (__nv_bfloat16*)out, ldo, nq, nkv, S::kCols, window, sink, head_tiles, splits,
-                  jobs ? jobs + 3 * n_jobs : nullptr, least, team);
+                  jobs ? jobs + 4 * n_jobs : nullptr, least, team);
         NS_CHECK_LAUNCH("ns_attention_kv4_tc");
     }
     return NS_OK;
@@ -519,7 +522,7 @@ int launch(const void* q, long long ldq, const void* k, const void* v, const int
 // bfloat16 q [tokens, ldq] and out [tokens, ldo]; heads of 64, 128 or 256; pages of 8, 16 or a multiple of 32 tokens.  Which tokens: `items` [n, 2] =
 // (first row, tokens of one request, of which the heads that share a kv head fill at most 8 * n_blocks columns), or one token each: rows [n], or all n.
 // A block to a (token or item, kv head), or, with `part`, several and a second kernel that joins them: `splits` (256 at most), of which those beyond one for each `least`
-// tiles of 32 keys leave at once, or those of `jobs` [n_jobs, 3] = (token or item, which part, of how many), each token's in order and together, which
+// tiles of 32 keys leave at once, or those of `jobs` [n_jobs, 4] = (first row, tokens, which part, of how many), each token's or item's in order and together, which
 // [n, 2] = (first job, how many) follow.  `part`: nkv * tiles of heads * (n * splits or n_jobs) * 8 * n_blocks * (D + 2) floats.
 NS_API int ns_attention_kv4_tc(const void* q, long long ldq, const void* k, const void* v, const int* table, int table_stride, const int* token_req,
                                const int* positions, const int* rows, const int* items, int n, void* out, long long ldo, int nq, int nkv, int D, int page_size,
@@ -527,7 +530,7 @@ NS_API int ns_attention_kv4_tc(const void* q, long long ldq, const void* k, cons
     if (n <= 0) return NS_OK;
     if (nkv < 1 || nq < 1 || nq % nkv || window < 0 || !(page_size == 8 || page_size == 16 || (page_size > 0 && page_size % 32 == 0)))
         NS_FAIL(NS_ERR_UNSUPPORTED, "ns_attention_kv4_tc: %d heads over %d, pages of %d, a window of %d", nq, nkv, page_size, window);
-    if (splits < 1 || splits > (part ? kMostParts : 1) || (part && least < 1) || (uintptr_t)part % 16 || (jobs && (!part || n_jobs < 1)))
+    if (splits < 1 || splits > (part ? kMostParts : 1) || (part && least < 1) || ((uintptr_t)part | (uintptr_t)jobs) % 16 || (jobs && (!part || n_jobs < 1)))
         NS_FAIL(NS_ERR_ARGUMENT, "ns_attention_kv4_tc: %d blocks to a request, of %d tiles or more", splits, least);
     if (((uintptr_t)k | (uintptr_t)v) % 16) NS_FAIL(NS_ERR_ARGUMENT, "ns_attention_kv4_tc: pages on 16-byte boundaries");
 #define NS_KV4_CASE(DD, NBB, WW)                                                                                                                        \

@@ -124,14 +124,14 @@ def kv4_shape(lengths: tuple[int, ...] | None, rows: int, per_row: int, sms: int
     return 8 if total <= 2 * sms or total * 32 <= sms * longest else 4, 1, 0
 
 
-def kv4_jobs(lengths: tuple[int, ...], least: int) -> list[int]:
-    """(row, part, parts) of every block's share of a row's tiles, then (first of them, parts) of every row."""
+def kv4_jobs(rows: list[tuple[int, int]], lengths: tuple[int, ...], least: int) -> list[int]:
+    """(first row, tokens, part, parts) of every block's share of the tiles of (first row, tokens), then (first of them, parts) of each."""
     jobs, spans = [], []
-    for z, n in enumerate(lengths):
+    for (row, tokens), n in zip(rows, lengths):
         parts = max(1, -(-n // (KV4_TILE * least)))
-        spans += (len(jobs) // 3, parts)
+        spans += (len(jobs) // 4, parts)
         for p in range(parts):
-            jobs += (z, p, parts)
+            jobs += (row, tokens, p, parts)
     return jobs + spans
 
 
@@ -233,12 +233,12 @@ def _kv4_plan(ctx, lane, group: int, nkv: int, head_dim: int, window: int, tenso
         if tensor_core:
             seen = tuple(min(kv, window or kv) for _, n, kv in rest if n == 1)
             if rows:
-                plan["runs"].append(_kv4_run(plan["rows"], None, len(rows), seen, nkv, group, head_dim, 1 if group <= 8 else 2, on_device))
+                plan["runs"].append(_kv4_run(plan["rows"], None, len(rows), seen, nkv, group, head_dim, 1 if group <= 8 else 2, on_device, [(row, 1) for row in rows]))
             few = [r for r in rest if r[1] > 1]
             if few:
                 tiles, n_blocks = kv4_token_tiles(few, group)
                 keys = {row + i: min(kv, window + n) if window else kv for row, n, kv in few for i in range(n)}
-                plan["runs"].append(_kv4_run(None, on_device(tiles), len(tiles), tuple(keys[row] for row, _ in tiles), nkv, group, head_dim, n_blocks, on_device))
+                plan["runs"].append(_kv4_run(None, on_device(tiles), len(tiles), tuple(keys[row] for row, _ in tiles), nkv, group, head_dim, n_blocks, on_device, tiles))
         for first, count, head, heads in kv4_unfold_runs([-(-ctx.kv_lens[i] // KV4_UNFOLD_PAGE) - _first_chunk(ctx, i, window) for i in long], nkv, head_dim,
                                                          KV4_UNFOLD_MAX):
             plan["portions"].append(_kv4_portion(ctx, long[first: first + count], window, head, heads, on_device))
@@ -262,14 +262,15 @@ def _plan_on_this_stream(plan: dict, stream: int) -> None:
     streams.add(stream)
 
 
-def _kv4_run(rows, items, count: int, lengths, nkv: int, group: int, head_dim: int, n_blocks: int, on_device=None) -> tuple:
-    """What the launch for `count` rows, or tiles of tokens, is: (rows, items, how many, n-blocks of columns, shape, jobs, how many, floats of the workspace)."""
+def _kv4_run(rows, items, count: int, lengths, nkv: int, group: int, head_dim: int, n_blocks: int, on_device=None, taken=None) -> tuple:
+    """What the launch for `count` rows, or tiles of tokens (`taken`: (first row, tokens) of them, where the host knows their lengths), is: (rows, items, how many,
+    n-blocks of columns, shape, jobs, how many, floats of the workspace)."""
     per_row = nkv * -(-group // (8 * n_blocks))
     warps, splits, least = kv4_shape(lengths, count, per_row, sm_count(), head_dim, n_blocks)
     units, jobs = (count * splits, None) if least else (0, None)
     if least and on_device:
-        listed = kv4_jobs(lengths, least)
-        units, jobs = (len(listed) - 2 * count) // 3, on_device(listed)
+        listed = kv4_jobs(taken, lengths, least)
+        units, jobs = (len(listed) - 2 * count) // 4, on_device(listed)
     return rows, items, count, n_blocks, (warps, splits, least), jobs, units if jobs is not None else 0, units * per_row * 8 * n_blocks * (head_dim + 2)
 
 

@@ -106,13 +106,13 @@ def test_shape_of_a_launch(head_dim, n_blocks, resident):
                 warps, splits, least = ops.kv4_shape(lengths if known else None, rows, per_row, 148, head_dim, n_blocks)
                 assert warps in (4, 8) and 1 <= splits <= 256 and (least > 0) == (splits > 1)
                 if splits > 1 and known:
-                    jobs = ops.kv4_jobs(lengths, least)
-                    n = (len(jobs) - 2 * rows) // 3
+                    jobs = ops.kv4_jobs([(7 * z, z % 3 + 1) for z in range(rows)], lengths, least)
+                    n = (len(jobs) - 2 * rows) // 4
                     assert warps == 4 and least >= 4 and n <= max(slots // per_row, 2 * rows)  # every block has its place at once, or two waves at most
-                    spans = [jobs[3 * n + 2 * z: 3 * n + 2 * z + 2] for z in range(rows)]
+                    spans = [jobs[4 * n + 2 * z: 4 * n + 2 * z + 2] for z in range(rows)]
                     for (first, parts), keys in zip(spans, lengths):
                         assert parts == max(1, -(-keys // (32 * least))) <= splits
-                    assert [jobs[3 * i: 3 * i + 3] for i in range(n)] == [[z, p, parts] for z, (_, parts) in enumerate(spans) for p in range(parts)]
+                    assert [jobs[4 * i: 4 * i + 4] for i in range(n)] == [[7 * z, z % 3 + 1, p, parts] for z, (_, parts) in enumerate(spans) for p in range(parts)]
                     assert [first for first, _ in spans] == [sum(parts for _, parts in spans[:z]) for z in range(rows)]
                 elif splits > 1:
                     assert rows * per_row * splits <= slots
