@@ -89,7 +89,7 @@ __device__ __forceinline__ void bounds(const __nv_bfloat16*, float& lo, float& h
     hi = -__high2float(b);
 }
 
-// S and B of a group, four features in each of 8 neighbouring lanes; S is NaN where the group is not finite
+// S and B of a group, four features in each of 8 neighbouring lanes; S is NaN where the group, or what its largest code would stand for, is not finite
 template <typename T>
 __device__ __forceinline__ Group group_of(const T* type, const float (&x)[4], bool live) {
     float lo = fminf(fminf(x[0], x[1]), fminf(x[2], x[3])), hi = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
@@ -105,8 +105,9 @@ __device__ __forceinline__ Group group_of(const T* type, const float (&x)[4], bo
     // (the difference of two bfloat16 numbers is mostly exact, and often just in the middle)
     const bool inexact = __fadd_rn(__fsub_rn(lo, __fsub_rn(base, back)), __fsub_rn(-S, back)) != 0.f;
     if (near_middle(spread) || (inexact && near_middle(base)) || spread < 1.5777218e-30f /* 2^-99 */) g = exact_group(lo, hi);
-    const float s = __bfloat162float(g.S), b = __bfloat162float(g.B);
-    if (bad || !((s - s) + (b - b) == 0.f)) g.S = g.B = __ushort_as_bfloat16(0x7fff);
+    // (what the largest code stands for is not finite either where S or B is not)
+    const float top = __bfloat162float(__hfma(g.S, __float2bfloat16_rn(1.9375f), g.B));
+    if (bad || !(top - top == 0.f)) g.S = g.B = __ushort_as_bfloat16(0x7fff);
     return g;
 }
 

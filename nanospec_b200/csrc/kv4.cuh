@@ -4,9 +4,10 @@
 // largest and smallest feature, each rounded once.  A code c of 0 to 15 stands for the bfloat16 nearest to B + S (1 + c / 16): 1 + c / 16 is a
 // bfloat16 whose four upper mantissa bits are c, so a shift, a mask and one fused multiply-add of two numbers give two values, and B,
 // rounded at about S's size, misses lo by no more than half of its own last bit.  A feature x takes the code nearest to 16 (x - B) / S - 16 (ties to even).
-// A group whose S would be below 2^-100 holds B = lo and codes of 0 (S = 0).  A token whose key or value (of one kv head) holds an infinity
-// or a NaN, or a spread that bfloat16 cannot hold, has NaN for all S and B of that key, and zeros for the groups of its value that are
-// not finite: a query that sees the token gets NaN, and one that does not meets finite values only.
+// A group whose S would be below 2^-100 holds B = lo and codes of 0 (S = 0).  A group is not finite where a feature is an infinity or a NaN, where bfloat16 cannot
+// hold S or B, or where B + S (1 + 15 / 16) rounds to an infinity (S and B are finite then, hi is within a few steps of bfloat16's largest number).  A token whose key
+// or value (of one kv head) has such a group has NaN for all S and B of that key, and zeros for the groups of its value that are not finite: a query that sees the
+// token gets NaN, and one that does not meets finite values only.
 //
 // A page of a kv head is one run of page_size * D * 5 / 8 bytes: the codes of all its tokens (D / 2 bytes each, byte j feature 2j in
 // the low half and 2j + 1 in the high one), then their groups' (S, B) pairs (D / 8 bytes each).  Codes and pairs lie apart, so that a

@@ -684,3 +684,56 @@ def test_pages_far_into_a_large_pool():
     want, tol8, _ = attend(qkv[:, : 8 * dim], k, v, ctx, 8, dim ** -0.5)
     _near(out, want, tol8 + want.abs() * 1.01 * half_step(BF16))
     assert k.abs().sum() > 0
+
+
+# ---- values at the end of bfloat16's range ------------------------------------------------------------------------------------------------
+BIG = torch.finfo(BF16).max
+BEYOND = 0.148  # features from here to 1 times the largest: S and B are finite, what the largest feature's code stands for rounds beyond it
+
+
+def test_the_borders_of_a_group_at_the_end_of_the_range():
+    """What the tests below are about, in 64 bits."""
+    for at, beyond in ((BEYOND, True), (0.5, False)):
+        lo = torch.tensor([at * BIG]).bfloat16().double()
+        S = to_bf16((BIG - lo) * 16 / 15)
+        B = to_bf16(lo - S)
+        assert S < BIG and B.abs() < BIG and bool(to_bf16(B + S * 31 / 16) > BIG) == beyond
+
+
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_store_of_a_group_whose_largest_code_is_beyond_the_range(dim, dtype):
+    from nanospec_b200 import ops
+    ctx, lane, qkv = step([(0, 4)], 16, 2, dim, dtype, 1)
+    x = qkv.reshape(4, 5, dim)
+    ramp = torch.linspace(BEYOND, 1.0, 32, device="cuda").double() * BIG
+    ramp[0], ramp[-1] = torch.tensor(BEYOND * BIG).bfloat16().double(), BIG
+    x[1, 2, :32] = ramp.to(dtype).clamp(max=BIG)            # a key of head 1
+    x[2, 3, dim - 32:] = ramp.to(dtype).clamp(max=BIG)      # a value of head 0
+    half = torch.linspace(0.5, 1.0, 32, device="cuda").double() * BIG
+    x[3, 1, :32] = half.to(dtype).clamp(max=BIG)            # (within the range: held as it is)
+    ops.kv4_store(qkv, ctx, lane, 1, 2, dim)
+    k, v = ops.kv4_read(lane, ctx.positions, ctx.token_req, 2, dim)
+    assert v.isfinite().all()
+    nan = k.isnan()
+    assert nan.all(-1).tolist() == [[False, False], [False, True], [True, False], [False, False]] and torch.equal(nan.any(-1), nan.all(-1))
+    assert (k.isfinite() | nan).all() and (v[2, 0, -32:] == 0).all()
+    assert torch.equal(k[3, 0].double(), held4(x[3, 1].double()))
+
+
+@pytest.mark.parametrize("tokens", [3, 100])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_a_value_beyond_the_range_reaches_only_those_that_see_it(tokens, dim):
+    """A few tokens in one tile, and a portion: the rows before the token's position meet a weight of zero for it."""
+    from nanospec_b200 import ops
+    ctx, lane, qkv = step([(40, tokens)], 16, 2, dim, BF16, 4)
+    fill(ctx, lane, 4, 2, dim)
+    key = 40 + tokens - 1
+    one = type(ctx)(**{**vars(ctx), "positions": ctx.positions[-1:].clone(), "token_req": ctx.token_req[-1:].clone()})
+    bad = _rand(1, 8 * dim, dtype=BF16)
+    bad[0, 7 * dim: 7 * dim + 32] = torch.linspace(BEYOND, 1.0, 32).double().mul(BIG).bfloat16().cuda().clamp(max=BIG)  # the value of kv head 1
+    ops.kv4_store(bad, one, lane, 4, 2, dim)
+    out = torch.empty((ctx.n_tokens, 4 * dim), dtype=BF16, device="cuda")
+    ops.attention_kv4(qkv, lane, ctx, out, 4, 2, dim)
+    sees = (ctx.positions[:, None] >= key).expand(-1, 2 * dim)
+    assert torch.equal(out[:, 2 * dim:].isnan(), sees) and out[:, : 2 * dim].isfinite().all()
