@@ -49,8 +49,16 @@ __device__ __forceinline__ void ld4(const __nv_bfloat16* p, float (&v)[4]) {
 
 constexpr float kMagic = 12582912.f;  // 1.5 * 2^23: added to it, a small number is rounded to an integer, which the last bits hold
 
+constexpr float kHugeS = 8.507059173023462e37f;  // 2^126: from here on x - B, up to 1.95 S, may lie beyond float's range
+
 // the code of x in a group: the integer nearest to 16 (x - B) / S - 16, ties to even, within 0 .. 15
 __device__ __noinline__ uint32_t code_of(float x, float S, float B, float inv) {
+    if (S >= kHugeS) {  // a quarter of everything: exact but for an x that counts in a tie only, by its sign
+        if (fabsf(x) >= 1.f) x *= 0.25f;
+        S *= 0.25f;
+        B *= 0.25f;
+        inv *= 4.f;
+    }
     // d + rest = x - B without error
     const float d = __fsub_rn(x, B), back = __fsub_rn(d, x);
     const float rest = __fadd_rn(__fsub_rn(x, __fsub_rn(d, back)), __fsub_rn(-B, back));
@@ -123,7 +131,7 @@ __device__ __forceinline__ void put_group(const T* type, const float (&x)[4], Gr
     if (S > 0.f) {
         const float inv = __fdividef(16.f, S), step = S * 0.0625f, half = 0.5f * step;
         uint32_t t[4];
-        bool again = false;
+        bool again = S >= kHugeS;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const float d = __fsub_rn(x[i], B);

@@ -737,3 +737,26 @@ def test_a_value_beyond_the_range_reaches_only_those_that_see_it(tokens, dim):
     ops.attention_kv4(qkv, lane, ctx, out, 4, 2, dim)
     sees = (ctx.positions[:, None] >= key).expand(-1, 2 * dim)
     assert torch.equal(out[:, 2 * dim:].isnan(), sees) and out[:, : 2 * dim].isfinite().all()
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_codes_of_features_further_apart_from_the_base_than_float_reaches(dtype):
+    """x - B is up to 1.95 S: beyond float's range for the largest S."""
+    from nanospec_b200 import ops
+    lens = [(0, 6)]
+    ctx, lane, qkv = step(lens, 16, 1, 64, dtype, 1)
+    v = qkv[:, 128:]
+    for i, (lo, hi) in enumerate(((-1.3e38, 0.575e38), (-1.0e38, 2.0e38), (0.0, 3.0e38), (-0.2e38, 2.9e38), (1.0e38, 1.9e38))):
+        v[i, :32] = torch.linspace(lo, hi, 32).to(dtype).cuda()
+        v[i, 32:] = torch.linspace(lo, hi, 32).flip(0).to(dtype).cuda()
+    v[2, 5], v[2, 40] = 1e-30, -1e-38 if dtype == BF16 else -1e-44
+    g = v.double().reshape(6, 2, 32)
+    lo, hi = g.amin(-1, keepdim=True), g.amax(-1, keepdim=True)
+    S = to_bf16((hi - lo) * 16 / 15)
+    B = to_bf16(lo - S)
+    beyond = (S > BIG) | (B.abs() > BIG) | (to_bf16(B + S * 31 / 16).abs() > BIG)  # groups that count as not finite: zeros
+    assert beyond[..., 0].tolist() == [[False, False], [True, True], [False, False], [True, True], [False, False], [False, False]]
+    want = held4(v.double().unsqueeze(1)).masked_fill(beyond.expand(-1, -1, 32).reshape(6, 1, 64), 0.0)
+    ops.kv4_store(qkv, ctx, lane, 1, 1, 64)
+    _, got = ops.kv4_read(lane, ctx.positions, ctx.token_req, 1, 64)
+    assert torch.equal(got.double(), want)
