@@ -244,8 +244,9 @@ kv4_store_kernel(const T* __restrict__ qkv, long long ld, T* __restrict__ q_out,
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
             const float c = (float)cs[f + k], s = (float)cs[half + f + k];
-            oa[k] = __fmaf_rn(a[k], c, -__fmul_rn(b[k], s));
-            ob[k] = __fmaf_rn(b[k], c, __fmul_rn(a[k], s));
+            const bool turned = f + k < pairs;  // (what is not rotated does not meet its partner, which may not be finite)
+            oa[k] = turned ? __fmaf_rn(a[k], c, -__fmul_rn(b[k], s)) : a[k];
+            ob[k] = turned ? __fmaf_rn(b[k], c, __fmul_rn(a[k], s)) : b[k];
         }
         st8(y, oa);
         st8(y + half, ob);

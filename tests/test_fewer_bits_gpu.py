@@ -760,3 +760,22 @@ def test_codes_of_features_further_apart_from_the_base_than_float_reaches(dtype)
     ops.kv4_store(qkv, ctx, lane, 1, 1, 64)
     _, got = ops.kv4_read(lane, ctx.positions, ctx.token_req, 1, 64)
     assert torch.equal(got.double(), want)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("pairs", [None, 0, 8])
+def test_features_of_q_that_are_not_rotated_stay_as_they_are(pairs, dtype):
+    """Also beside a partner that is not finite, and to a buffer of its own."""
+    from nanospec_b200 import ops
+    ctx, lane, qkv = step([(7, 3)], 16, 1, 64, dtype, 2)
+    f = None if pairs is None else _inv_freq(64, pairs=pairs)
+    n = pairs or 0
+    x = qkv[:, :128].reshape(3, 2, 64)
+    x[0, 0, 20], x[1, 1, 31], x[2, 0, 32 + 9], x[2, 1, 63] = math.inf, math.nan, -math.inf, math.nan
+    q = x.clone()
+    still = torch.tensor([j % 32 >= n for j in range(64)], device="cuda")
+    out = ops.kv4_store(qkv, ctx, lane, 2, 1, 64, f, q_out=torch.empty((3, 128), dtype=dtype, device="cuda"))
+    for got in (out, ops.kv4_store(qkv, ctx, lane, 2, 1, 64, f)[:, :128]):
+        got = got.reshape(3, 2, 64)
+        assert torch.equal(got[..., still].isnan(), q[..., still].isnan())
+        assert torch.equal(got[..., still].nan_to_num(0.25), q[..., still].nan_to_num(0.25)) and got[..., ~still].isfinite().all()
