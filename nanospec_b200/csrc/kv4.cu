@@ -284,11 +284,11 @@ kv4_store_kernel(const T* __restrict__ qkv, long long ld, T* __restrict__ q_out,
     }
 }
 
-// One value of a word (eight features) per thread: k and v of (token, kv head).
+// One value of a word (eight features) per thread: k and v of (token, kv head); zeros where the table holds no page of the pool for the position.
 __global__ void __launch_bounds__(kThreads)
 kv4_read_kernel(const uint8_t* __restrict__ k_pages, const uint8_t* __restrict__ v_pages, const int* __restrict__ positions,
-                const int* __restrict__ token_req, const int* __restrict__ block_table, int table_stride, __nv_bfloat16* __restrict__ k_out,
-                __nv_bfloat16* __restrict__ v_out, int n_tokens, int page_size, int nkv, int D) {
+                const int* __restrict__ token_req, const int* __restrict__ block_table, int table_stride, int table_rows, int table_columns, int n_pages,
+                __nv_bfloat16* __restrict__ k_out, __nv_bfloat16* __restrict__ v_out, int n_tokens, int page_size, int nkv, int D) {
     ns_pdl_launch_dependents();
     ns_pdl_wait();
     const int words = D / 8, per_token = nkv * words;
@@ -300,11 +300,12 @@ kv4_read_kernel(const uint8_t* __restrict__ k_pages, const uint8_t* __restrict__
     for (int u = threadIdx.x - part * lanes; u < per_token; u += lanes) {
         const long long i = n * per_token + u;
         const int h = u / words, w = u - h * words;
-        const int req = token_req[n];
+        const int req = token_req[n], pos = positions[n];
+        const bool listed = req >= 0 && req < table_rows && pos >= 0 && pos / page_size < table_columns;
+        const int page = listed ? block_table[(size_t)req * table_stride + pos / page_size] : -1;
         uint4 k = make_uint4(0u, 0u, 0u, 0u), v = k;
-        if (req >= 0) {
-            const int pos = positions[n], slot = pos % page_size;
-            const int page = block_table[(size_t)req * table_stride + pos / page_size];
+        if (page >= 0 && page < n_pages) {
+            const int slot = pos % page_size;
             const size_t block = ((size_t)page * nkv + h) * kv4_block_bytes(page_size, D);
             const size_t codes = block + ((size_t)slot * words + w) * 4;
             const size_t pair = block + (size_t)page_size * (D / 2) + ((size_t)slot * (D / kGroup) + w / 4) * 4;
@@ -355,16 +356,17 @@ NS_API int ns_kv4_store(const void* qkv, long long ld, void* q_out, long long ld
     return NS_OK;
 }
 
-// k_out, v_out [n_tokens, nkv, D]: what the cache holds at positions[n] of request token_req[n] (zeros where that is negative).
+// k_out, v_out [n_tokens, nkv, D]: what the cache (`n_pages` pages) holds at positions[n] of request token_req[n]; zeros where that is negative, or where the table
+// [table_rows, table_columns] does not say in which page: a page given back, a position that nobody has.
 NS_API int ns_kv4_read(const void* k_pages, const void* v_pages, const int* positions, const int* token_req, const int* block_table, int table_stride,
-                       void* k_out, void* v_out, int n_tokens, int page_size, int nkv, int D, int sms, cudaStream_t stream) {
+                       int table_rows, int table_columns, int n_pages, void* k_out, void* v_out, int n_tokens, int page_size, int nkv, int D, int sms, cudaStream_t stream) {
     if (n_tokens <= 0) return NS_OK;
     int rc = check_geometry("ns_kv4_read", D, nkv, page_size);
     if (rc) return rc;
     const int per_token = nkv * (D / 8), side = per_token < kThreads ? kThreads / per_token : 1, blocks = (n_tokens + side - 1) / side;
     const int grid = blocks < 16 * sms ? blocks : 16 * sms;
     NS_LAUNCH(kv4_read_kernel, grid, kThreads, 0, stream, (const uint8_t*)k_pages, (const uint8_t*)v_pages, positions, token_req, block_table, table_stride,
-              (__nv_bfloat16*)k_out, (__nv_bfloat16*)v_out, n_tokens, page_size, nkv, D);
+              table_rows, table_columns, n_pages, (__nv_bfloat16*)k_out, (__nv_bfloat16*)v_out, n_tokens, page_size, nkv, D);
     NS_CHECK_LAUNCH("ns_kv4_read");
     return NS_OK;
 }

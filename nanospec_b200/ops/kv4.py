@@ -74,14 +74,15 @@ def kv4_store(qkv: torch.Tensor, ctx, lane, nq: int, nkv: int, head_dim: int, in
 
 def kv4_read(lane, positions: torch.Tensor, token_req: torch.Tensor, nkv: int, head_dim: int) -> tuple[torch.Tensor, torch.Tensor]:
     """What the cache holds at positions[n] of request token_req[n]: keys and values [N, nkv, head_dim] in bfloat16, as `attention_kv4` sees them
-    (zeros where token_req is negative)."""
+    (zeros where token_req is negative, and where the block table has no page for the position, as behind a window)."""
     _on_current_device(lane.k, lane.v, lane.block_table, positions, token_req)
     _check_lane("kv4_read", lane, nkv, head_dim)
     n = positions.numel()
     _check_step("kv4_read", positions, token_req, n)
     k, v = torch.empty((2, n, nkv, head_dim), dtype=torch.bfloat16, device=lane.k.device).unbind(0)
     lib.call("ns_kv4_read", lane.k.data_ptr(), lane.v.data_ptr(), positions.data_ptr(), token_req.data_ptr(), lane.block_table.data_ptr(),
-             lane.block_table.stride(0), k.data_ptr(), v.data_ptr(), n, lane.page_size, nkv, head_dim, sm_count(), _stream())
+             lane.block_table.stride(0), *lane.block_table.shape, lane.k.shape[0], k.data_ptr(), v.data_ptr(), n, lane.page_size, nkv, head_dim, sm_count(),
+             _stream())
     return k, v
 
 

@@ -27,7 +27,7 @@ _SIGNATURES: dict[str, list] = {
     "ns_linear_i8": [_P, _L, _I, _P, _P, _L, _P, _P, _P, _L, _I, _I, _I, _I, _I, _I, _I, _I, _P, _P],
     "ns_kv4_store": [_P, _L, _P, _L, _P, _P, _P, _I, _P, _I, _P, _P, _I, _I, _I, _I, _I, _I, _I, _P],
     "ns_kv4_unfold": [_P, _P, _P, _I, _P, _I, _P, _P, _P, _I, _I, _I, _I, _I, _P],
-    "ns_kv4_read": [_P, _P, _P, _P, _P, _I, _P, _P, _I, _I, _I, _I, _I, _P],
+    "ns_kv4_read": [_P, _P, _P, _P, _P, _I, _I, _I, _I, _P, _P, _I, _I, _I, _I, _I, _P],
     "ns_attention_kv4_tc": [_P, _L, _P, _P, _P, _I, _P, _P, _P, _P, _I, _P, _L, _I, _I, _I, _I, _F, _I, _P, _I, _I, _I, _P, _P, _I, _I, _P],
     "ns_attention_kv4": [_P, _L, _P, _P, _P, _I, _P, _P, _P, _I, _P, _L, _I, _I, _I, _I, _F, _I, _P, _I, _I, _P],
     "ns_embed": [_P, _P, _P, _I, _I, _I, _I, _P],

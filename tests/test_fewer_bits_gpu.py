@@ -779,3 +779,20 @@ def test_features_of_q_that_are_not_rotated_stay_as_they_are(pairs, dtype):
         got = got.reshape(3, 2, 64)
         assert torch.equal(got[..., still].isnan(), q[..., still].isnan())
         assert torch.equal(got[..., still].nan_to_num(0.25), q[..., still].nan_to_num(0.25)) and got[..., ~still].isfinite().all()
+
+
+@pytest.mark.parametrize("page", [8, 5])
+def test_reading_where_the_cache_holds_nothing(page):
+    """Pages given back, positions and requests that the table does not have, entries beyond the pool: zeros, and nothing of the pool's surroundings is read."""
+    from nanospec_b200 import ops
+    ctx, lane, _ = step([(40, 1), (23, 1)], page, 2, 64)
+    held, _ = fill(ctx, lane, 1, 2, 64)
+    lane.block_table[0, :2] = -1
+    lane.block_table[1, 1] = lane.k.shape[0]
+    rows, columns = lane.block_table.shape
+    asked = [(0, 0, False), (0, 2 * page - 1, False), (0, 2 * page, True), (0, 40, True), (1, page, False), (1, 2, True), (1, 23, True), (rows, 0, False), (1 << 30, 3, False),
+             (0, columns * page, False), (0, 2 ** 31 - 1, False), (1, -1, False), (1, -2 ** 31, False), (-1, 5, False)]
+    i32 = lambda i: torch.tensor([a[i] for a in asked], dtype=torch.int32, device="cuda")  # noqa: E731
+    for k, v in (ops.kv4_read(lane, i32(1), i32(0), 2, 64), ops.kv4_read(lane, i32(1).repeat(400), i32(0).repeat(400), 2, 64)):
+        for n, (req, pos, there) in enumerate(asked):
+            assert torch.equal(k[n].double(), held[41 * req + pos]) if there else not k[n].any() and not v[n].any()
