@@ -258,6 +258,7 @@ def _plan_on_this_stream(plan: dict, stream: int) -> None:
         return
     here = torch.cuda.current_stream()
     here.wait_event(plan["ready"])
+    lib.load().ns_full_launch_next()  # (it has a prerequisite beside its predecessor in the stream)
     for t in plan["lists"]:
         t.record_stream(here)
     streams.add(stream)

@@ -2,6 +2,9 @@
 
 from __future__ import annotations
 
+from concurrent.futures import ThreadPoolExecutor
+from types import SimpleNamespace
+
 import pytest
 import torch
 
@@ -119,3 +122,48 @@ def test_shape_of_a_launch(head_dim, n_blocks, resident):
     assert ops.kv4_shape((100000,) + (500,) * 63, 64, 8, 148, 128)[1] > 50  # (one request would outlast all others)
     assert ops.kv4_shape((100000,), 1, 1, 148, 128)[1] > 200  # (one kv head: more blocks than are joined would find a place)
     assert ops.kv4_shape((100000,), 1, 8, 148, 128)[1] > 60 and ops.kv4_shape((16,), 1, 8, 148, 128) == (8, 1, 0)
+
+
+def _in_a_thread(fn):
+    """(What a launch asks of its thread ends with the thread.)"""
+    with ThreadPoolExecutor(1) as pool:
+        return pool.submit(fn).result()
+
+
+class _Stream:
+    """A stream that notes what is asked of it, and whether the thread's next launch is a full one by then."""
+
+    def __init__(self, seen):
+        self.seen = seen
+
+    def wait_event(self, event):
+        self.seen.append((event, self.pending()))
+
+    @staticmethod
+    def pending():
+        from nanospec_b200.ops import lib
+        return lib.load().ns_full_launch_pending()
+
+
+def test_a_call_that_waits_for_a_steps_lists_starts_when_they_are_there(monkeypatch):
+    """The launch behind the wait is not made to overlap its predecessor in the stream: it has a prerequisite beside it."""
+    from nanospec_b200.ops import kv4
+    seen, kept = [], []
+    here = _Stream(seen)
+    monkeypatch.setattr(kv4.torch.cuda, "current_stream", lambda *a: here)
+    monkeypatch.setattr(kv4.torch.cuda, "is_current_stream_capturing", lambda: False)
+    held = SimpleNamespace(record_stream=kept.append)
+    plan = {"lists": [held, held], "ready": "copied", "streams": {7}}
+
+    def calls():
+        kv4._plan_on_this_stream({"lists": []}, 7), kv4._plan_on_this_stream(plan, 7)  # no lists; the stream that copied them
+        before = here.pending()
+        kv4._plan_on_this_stream(plan, 8)
+        return before, here.pending()
+    assert _in_a_thread(calls) == (0, 1)
+    assert seen == [("copied", 0)] and kept == [here, here] and plan["streams"] == {7, 8}
+
+    def again():
+        kv4._plan_on_this_stream(plan, 8)
+        return here.pending()
+    assert _in_a_thread(again) == 0 and len(seen) == 1

@@ -796,3 +796,27 @@ def test_reading_where_the_cache_holds_nothing(page):
     for k, v in (ops.kv4_read(lane, i32(1), i32(0), 2, 64), ops.kv4_read(lane, i32(1).repeat(400), i32(0).repeat(400), 2, 64)):
         for n, (req, pos, there) in enumerate(asked):
             assert torch.equal(k[n].double(), held[41 * req + pos]) if there else not k[n].any() and not v[n].any()
+
+
+@pytest.mark.parametrize("lens", [[(9, 1), (900, 1), (100, 1)], [(20, 1), (200, 3), (40, 90)]])
+@pytest.mark.parametrize("dim,dtype", [(128, BF16), (64, F32)])
+def test_a_step_whose_calls_follow_other_kernels_on_their_streams(lens, dim, dtype):
+    """The lists are late, and a kernel stands ready on each later stream that the attention's launch could overlap."""
+    from nanospec_b200 import ops
+    ctx, lane, qkv = step(lens, 16, 2, dim, dtype, 8)
+    fill(ctx, lane, 8, 2, dim, dtype)
+    want = ops.attention_kv4(qkv, lane, ctx, torch.zeros((ctx.n_tokens, 8 * dim), dtype=dtype, device="cuda"), 8, 2, dim)
+    x, w = _rand(64, 1024, dtype=BF16), ops.quantize_rows(_rand(1024, 1024, seed=2))
+    outs, products = [torch.zeros_like(want) for _ in range(3)], [torch.empty((64, 1024), dtype=BF16, device="cuda") for _ in range(3)]
+    ctx.extras = {}
+    torch.cuda.synchronize()
+    for i, (out, product, s) in enumerate(zip(outs, products, [torch.cuda.Stream() for _ in outs])):
+        with torch.cuda.stream(s):
+            if i == 0:
+                torch.cuda._sleep(20_000_000)
+            ops.linear_i8(x, w, product)
+            ops.attention_kv4(qkv, lane, ctx, out, 8, 2, dim)
+            ops.linear_i8(x, w, product)
+    torch.cuda.synchronize()
+    assert all(torch.equal(out, want) for out in outs) and all(torch.equal(p, products[0]) for p in products)
+    ops.check_kernel_errors()
