@@ -18,6 +18,15 @@ NS_API int ns_full_launch_next() {
 }
 // Whether that is still to come (1) or has been taken by a launch of this thread (0).
 NS_API int ns_full_launch_pending() { return ns_pdl_skip_one; }
+// Waits on the host until `event` has completed, also while the thread captures a stream (an event that belongs to no capture).
+NS_API int ns_event_synchronize(void* event) {
+    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+    NS_CUDA(cudaThreadExchangeStreamCaptureMode(&mode));
+    const cudaError_t waited = cudaEventSynchronize((cudaEvent_t)event);
+    NS_CUDA(cudaThreadExchangeStreamCaptureMode(&mode));
+    NS_CUDA(waited);
+    return NS_OK;
+}
 // 1 (default): kernels are launched so that they may overlap the tail of their predecessor
 // (programmatic dependent launch); 0: plain stream order.
 NS_API int ns_set_pdl(int enabled) {

@@ -207,6 +207,9 @@ def _kv4_plan(ctx, lane, group: int, nkv: int, head_dim: int, window: int, tenso
     def on_device(v):
         if not v:
             return None
+        if torch.cuda.is_current_stream_capturing():
+            raise KernelError("attention_kv4: a step's lists cannot go to the device while a graph is captured; ctx.extras['graph'] says that every row is a "
+                              "request's one token, which needs none, and another step has a call before the capture")
         made.append(torch.tensor(v, dtype=torch.int32).to(ctx.device, non_blocking=True))
         return made[-1]
 
@@ -251,10 +254,23 @@ def _kv4_plan(ctx, lane, group: int, nkv: int, head_dim: int, window: int, tenso
     return plan
 
 
+_captured_lists: list = []  # of steps that were captured without `ctx.extras["graph"]`: a graph reads them for as long as it lives
+
+
 def _plan_on_this_stream(plan: dict, stream: int) -> None:
-    """The plan's lists go to the device on the stream of the step's first call; a call on another one waits for them there."""
+    """The plan's lists go to the device on the stream of the step's first call; a call on another one waits for them there.  One that is captured
+    waits on the host, once (its graph then finds them in place wherever it is replayed), and the lists stay."""
     streams = plan.get("streams")
-    if streams is None or stream in streams or torch.cuda.is_current_stream_capturing():
+    if streams is None:
+        return
+    if torch.cuda.is_current_stream_capturing():
+        if not plan.get("captured"):
+            if lib.load().ns_event_synchronize(plan["ready"].cuda_event):
+                raise KernelError(f"attention_kv4: waiting for the step's lists failed: {lib.load().ns_last_error().decode(errors='replace')}")
+            _captured_lists.append(plan["lists"])
+            plan["captured"] = True
+        return
+    if stream in streams:
         return
     here = torch.cuda.current_stream()
     here.wait_event(plan["ready"])
@@ -321,6 +337,10 @@ def attention_kv4(qkv: torch.Tensor, lane, ctx, out: torch.Tensor, nq: int, nkv:
     """Attention of the step's queries (the first nq * head_dim columns of `qkv`, rotated) over a lane in 4 bits: every token sees the positions
     up to its own (with `window` the last so many of them), which `kv4_store` has filled.  `sink` (float32 [nq]): the softmax's denominator also
     holds exp(sink[h]).  `scale` is head_dim ** -0.5 when None.  float32 and bfloat16; rows of padding (token_req < 0) are left as they are.
+
+    Captured steps: ctx.extras["graph"] says that every row is a request's one token and that the device alone knows the lengths (`positions`), so that a graph
+    serves the lengths that it is replayed with.  Another step has a call before its capture, and its graph serves the tokens and lengths of that call; what the
+    call copied to the device for them is kept until the process ends.
 
     bfloat16, softmax weights in bfloat16: single tokens and a few of a request on the tensor cores from the cache's bytes (csrc/attention_kv4_tc.cu: heads
     of 64, 128 or 256, pages of 8, 16 or a multiple of 32 tokens); longer portions of prompts unfold the keys and values that they see into bfloat16 once

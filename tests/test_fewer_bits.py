@@ -167,3 +167,38 @@ def test_a_call_that_waits_for_a_steps_lists_starts_when_they_are_there(monkeypa
         kv4._plan_on_this_stream(plan, 8)
         return here.pending()
     assert _in_a_thread(again) == 0 and len(seen) == 1
+
+
+def test_a_captured_call_keeps_a_steps_lists(monkeypatch):
+    """Without the mark of captured steps: waited for on the host, once, and kept beyond the step."""
+    from nanospec_b200.ops import KernelError, kv4
+    status, waited = [0], []
+
+    def wait(event):
+        waited.append(event)
+        return status[0]
+    monkeypatch.setattr(kv4.lib, "load", lambda: SimpleNamespace(ns_event_synchronize=wait, ns_last_error=lambda: b"why"))
+    monkeypatch.setattr(kv4.torch.cuda, "is_current_stream_capturing", lambda: True)
+    monkeypatch.setattr(kv4, "_captured_lists", [])
+    lists = ["rows", "jobs"]
+    plan = {"lists": lists, "ready": SimpleNamespace(cuda_event=5), "streams": {7}}
+    kv4._plan_on_this_stream({"lists": []}, 7)
+    assert kv4._captured_lists == []
+    for stream in (7, 8, 8):
+        kv4._plan_on_this_stream(plan, stream)
+    assert waited == [5] and len(kv4._captured_lists) == 1 and kv4._captured_lists[0] is lists and plan["streams"] == {7}
+    status[0] = 1
+    with pytest.raises(KernelError, match="why"):
+        kv4._plan_on_this_stream({"lists": lists, "ready": SimpleNamespace(cuda_event=6), "streams": {7}}, 7)
+
+
+def test_a_steps_lists_are_not_made_in_a_capture(monkeypatch):
+    from nanospec_b200.ops import KernelError, kv4
+    ctx, lane, _ = step([(40, 1), (100, 1)], 16, 2, 64, nq=4, device="cpu")
+    monkeypatch.setattr(kv4, "sm_count", lambda: 148)
+    monkeypatch.setattr(kv4.torch.cuda, "is_current_stream_capturing", lambda: True)
+    with pytest.raises(KernelError, match="captured"):
+        kv4._kv4_plan(ctx, lane, 2, 2, 64, 0, True, True)
+    assert not ctx.extras
+    ctx.extras["graph"] = True
+    assert kv4._kv4_plan(ctx, lane, 2, 2, 64, 0, True, True)["runs"]

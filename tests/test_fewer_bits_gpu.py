@@ -820,3 +820,65 @@ def test_a_step_whose_calls_follow_other_kernels_on_their_streams(lens, dim, dty
     torch.cuda.synchronize()
     assert all(torch.equal(out, want) for out in outs) and all(torch.equal(p, products[0]) for p in products)
     ops.check_kernel_errors()
+
+
+@pytest.mark.parametrize("lens", [[(9, 1), (900, 1), (100, 1)], [(5000, 1)], [(30, 5), (2000, 3)], [(20, 1), (200, 3), (40, 90)]])
+@pytest.mark.parametrize("dim,dtype", [(128, BF16), (64, F32)])
+def test_a_step_captured_without_its_mark(lens, dim, dtype):
+    """Its graph finds the step's lists whatever becomes of the step."""
+    from nanospec_b200 import ops
+    ctx, lane, qkv = step(lens, 16, 2, dim, dtype, 8)
+    fill(ctx, lane, 8, 2, dim, dtype)
+    out = torch.zeros((ctx.n_tokens, 8 * dim), dtype=dtype, device="cuda")
+    call = lambda: ops.attention_kv4(qkv, lane, ctx, out, 8, 2, dim)  # noqa: E731
+    want = call().clone()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        call()
+    ctx.extras = {}
+    other = [torch.zeros(n, dtype=torch.int32, device="cuda") for n in (1, 2, 3, 5, 8, 40, 130, 500, 2000) for _ in range(8)]  # what the lists would have made room for
+    call(), out.zero_()  # (the step anew, with lists of its own)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out, want) and not any(o.any() for o in other)
+
+
+def test_a_capture_waits_for_lists_that_are_on_their_way():
+    from nanospec_b200 import ops
+    ctx, lane, qkv = step([(9, 1), (900, 1), (40, 3)], 16, 2, 128, BF16, 8)
+    fill(ctx, lane, 8, 2, 128)
+    out = torch.zeros((ctx.n_tokens, 1024), dtype=BF16, device="cuda")
+    call = lambda: ops.attention_kv4(qkv, lane, ctx, out, 8, 2, 128)  # noqa: E731
+    want = call().clone()
+    torch.cuda.synchronize()
+    ctx.extras = {}
+    first, second, graph = torch.cuda.Stream(), torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    with torch.cuda.stream(first):
+        torch.cuda._sleep(20_000_000)
+        call()
+    plan = next(iter(ctx.extras.values()))
+    with torch.cuda.stream(second):
+        graph.capture_begin()
+        call()
+        graph.capture_end()
+    assert plan["ready"].query()
+    first.synchronize()
+    out.zero_()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out, want)
+
+
+def test_a_first_call_in_a_capture_is_refused():
+    from nanospec_b200 import ops
+    from nanospec_b200.ops import KernelError
+    ctx, lane, qkv = step([(9, 1), (900, 1)], 16, 2, 128, BF16, 8)
+    fill(ctx, lane, 8, 2, 128)
+    out, x = torch.zeros((2, 1024), dtype=BF16, device="cuda"), torch.zeros(3, device="cuda")
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):  # (and the capture goes on)
+        with pytest.raises(KernelError, match="captured"):
+            ops.attention_kv4(qkv, lane, ctx, out, 8, 2, 128)
+        x += 1
+    graph.replay()
+    assert (x == 1).all() and not any(k[0] == "kv4_plan" for k in ctx.extras)
