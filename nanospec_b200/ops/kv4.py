@@ -96,10 +96,10 @@ def kv4_tensor_core_ok(dtype: torch.dtype, head_dim: int, page_size: int) -> boo
 KV4_PARTS_MAX = 256  # blocks of a row and kv head
 
 
-def kv4_shape(lengths: tuple[int, ...] | None, rows: int, per_row: int, sms: int, head_dim: int, n_blocks: int = 1) -> tuple[int, int, int]:
+def kv4_shape(lengths: tuple[int, ...] | None, rows: int, per_row: int, sms: int, head_dim: int, n_blocks: int = 1, window: int = 0) -> tuple[int, int, int]:
     """(warps of a block, blocks of a row's kv head, tiles of 32 keys that such a block takes at least, or 0: one block, which needs no joining).
 
-    `lengths`: keys of each row (or tile of tokens), None when the device alone knows them; `per_row`: (kv head, column tile) pairs.  Us on a B200, the requests
+    `lengths`: keys of each row (or tile of tokens), None when the device alone knows them, at most `window` where there is one; `per_row`: (kv head, column tile) pairs.  Us on a B200, the requests
     ragged down to a fifth of the length, 8 kv heads of 128:
     Several blocks while one each would take no more than half of the places, or while one request would outlast the others.  One request on 1,000 keys: one block of
     eight warps 14.4, several 12.3; on 100,000: a cluster of sixteen blocks 71.7, several 46.6; 16 requests on 1,000: 16.4, 18.4; on 4,000: 34.8, 30.7; one on 100,000
@@ -109,6 +109,11 @@ def kv4_shape(lengths: tuple[int, ...] | None, rows: int, per_row: int, sms: int
     slots = sms * (2 if head_dim > 128 else 3 if n_blocks > 1 else 6 if head_dim == 64 else 4)  # blocks of four warps that the SMs hold
     total = rows * per_row
     if lengths is None:
+        # The window's keys stand for the lengths only while a block then has no more than eight tiles: a window beyond all contexts would leave them few blocks (one request
+        # on 5,000 keys, a window of 131,072: 3 of 74, 28.7 us, now 18.4; 8 on 30,000: 305, now 90; 8 on 2,000, a window of 32,768: 36.9, now 24.6).
+        full = kv4_shape((window,) * rows, rows, per_row, sms, head_dim, n_blocks) if window else None
+        if full and full[2] <= 8:
+            return full
         return (4, min(KV4_PARTS_MAX, slots // total), 8) if total * 2 <= slots else (8 if total <= 2 * sms else 4, 1, 0)
     tiles = [-(-n // KV4_TILE) for n in lengths]
     longest, all_tiles = max(tiles), sum(tiles)
@@ -215,7 +220,7 @@ def _kv4_plan(ctx, lane, group: int, nkv: int, head_dim: int, window: int, tenso
 
     if ctx.extras.get("graph"):  # every row is a request's one token, and lengths are the device's
         plan = {"rows": None, "n_rows": total, "longest": None, "held": 0, "requests": 0, "portions": [],
-                "runs": [_kv4_run(None, None, total, (window,) * total if window else None, nkv, group, head_dim, 1 if group <= 8 else 2)] if tensor_core and total else []}
+                "runs": [_kv4_run(None, None, total, None, nkv, group, head_dim, 1 if group <= 8 else 2, window=window)] if tensor_core and total else []}
     else:
         if sum(ctx.q_lens) > total:
             raise KernelError(f"attention_kv4: the requests bring {sum(ctx.q_lens)} tokens, the step holds {total}")
@@ -280,11 +285,11 @@ def _plan_on_this_stream(plan: dict, stream: int) -> None:
     streams.add(stream)
 
 
-def _kv4_run(rows, items, count: int, lengths, nkv: int, group: int, head_dim: int, n_blocks: int, on_device=None, taken=None) -> tuple:
-    """What the launch for `count` rows, or tiles of tokens (`taken`: (first row, tokens) of them, where the host knows their lengths), is: (rows, items, how many,
+def _kv4_run(rows, items, count: int, lengths, nkv: int, group: int, head_dim: int, n_blocks: int, on_device=None, taken=None, window: int = 0) -> tuple:
+    """What the launch for `count` rows, or tiles of tokens (`taken`: (first row, tokens) of them, where the host knows their `lengths`, which are within the window), is: (rows, items, how many,
     n-blocks of columns, shape, jobs, how many, floats of the workspace)."""
     per_row = nkv * -(-group // (8 * n_blocks))
-    warps, splits, least = kv4_shape(lengths, count, per_row, sm_count(), head_dim, n_blocks)
+    warps, splits, least = kv4_shape(lengths, count, per_row, sm_count(), head_dim, n_blocks, window)
     units, jobs = (count * splits, None) if least else (0, None)
     if least and on_device:
         listed = kv4_jobs(taken, lengths, least)

@@ -202,3 +202,27 @@ def test_a_steps_lists_are_not_made_in_a_capture(monkeypatch):
     assert not ctx.extras
     ctx.extras["graph"] = True
     assert kv4._kv4_plan(ctx, lane, 2, 2, 64, 0, True, True)["runs"]
+
+
+def test_shape_of_a_captured_step_with_a_window():
+    """A window far beyond the contexts hides nothing: as without one.  One that decides how many keys there are at most: as if all requests held it."""
+    from nanospec_b200 import ops
+    for head_dim, n_blocks in ((64, 1), (128, 1), (128, 2), (256, 1)):
+        for rows in (1, 2, 8, 30, 64, 200):
+            for per_row in (1, 2, 8):
+                free = ops.kv4_shape(None, rows, per_row, 148, head_dim, n_blocks)
+                for window in (1, 40, 200, 1000, 4096, 32768, 131072, 1 << 30):
+                    shape = ops.kv4_shape(None, rows, per_row, 148, head_dim, n_blocks, window)
+                    known = ops.kv4_shape((window,) * rows, rows, per_row, 148, head_dim, n_blocks)
+                    assert shape == (known if known[2] <= 8 else free)  # never fewer blocks for a short context than one for each eight tiles
+    for rows, window, splits in ((1, 131072, 74), (8, 131072, 9), (8, 32768, 9)):
+        assert ops.kv4_shape(None, rows, 8, 148, 128, 1, window) == ops.kv4_shape(None, rows, 8, 148, 128) == (4, splits, 8)
+
+
+def test_a_captured_steps_plan_with_a_window(monkeypatch):
+    from nanospec_b200.ops import kv4
+    monkeypatch.setattr(kv4, "sm_count", lambda: 148)
+    ctx, lane, _ = step([(40, 1)], 16, 8, 128, nq=32, device="cpu")
+    ctx.extras["graph"] = True
+    wide, none = (kv4._kv4_plan(ctx, lane, 4, 8, 128, window, True, True)["runs"] for window in (131072, 0))
+    assert wide == none and none[0][4] == (4, 74, 8)
