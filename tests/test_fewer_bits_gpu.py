@@ -882,3 +882,49 @@ def test_a_first_call_in_a_capture_is_refused():
         x += 1
     graph.replay()
     assert (x == 1).all() and not any(k[0] == "kv4_plan" for k in ctx.extras)
+
+
+@pytest.mark.parametrize("nq,nkv,dim,page,dtype", [(32, 8, 128, 16, BF16), (16, 2, 64, 8, BF16), (6, 2, 96, 16, BF16), (4, 2, 64, 16, F32)])
+@pytest.mark.parametrize("lens,window,padding", [([(60, 0), (500, 1), (0, 0), (90, 3), (33, 0), (100, 200), (3, 1), (7, 0)], 0, 2),
+                                                 ([(60, 0), (0, 1), (31, 0)], 20, 0), ([(60, 0), (40, 0)], 0, 1)])
+def test_requests_that_bring_nothing(lens, window, padding, nq, nkv, dim, page, dtype):
+    from nanospec_b200 import ops
+    ctx, lane, qkv = step(lens, page, nkv, dim, dtype, nq, padding=padding)
+    lane.k.fill_(255), lane.v.fill_(255)
+    k, v = fill(ctx, lane, nq, nkv, dim, dtype)
+    n = ctx.n_tokens - padding
+    out = torch.full((ctx.n_tokens, nq * dim), 5.0, dtype=dtype, device="cuda")
+    ops.attention_kv4(qkv, lane, ctx, out, nq, nkv, dim, window=window)
+    held = [(a, kv) for a, kv in zip(ctx.q_lens, ctx.kv_lens) if kv]  # (the plain statement takes requests that hold something)
+    at = type(ctx)(**{**vars(ctx), "q_lens": [a for a, _ in held], "kv_lens": [kv for _, kv in held]})
+    want, tol8, tol32 = attend(qkv[:n, : nq * dim], k, v, at, nq, dim ** -0.5, window)
+    if n:
+        _near(out[:n], want, (tol32 if dtype == F32 else tol8) + want.abs() * 1.01 * half_step(dtype))
+    assert (out[n:] == 5).all()
+
+
+@pytest.mark.parametrize("window", [0, 40, 100000])
+@pytest.mark.parametrize("dim,dtype", [(128, BF16), (64, BF16), (96, BF16), (64, F32)])
+def test_captured_steps_with_windows_and_sinks(window, dim, dtype):
+    from nanospec_b200 import ops
+    nq, nkv = 8, 2
+    ctx, lane, qkv = step([(2900, 1), (17, 1), (0, 1), (300, 1)], 16, nkv, dim, dtype, nq, padding=1)
+    k, v = fill(ctx, lane, nq, nkv, dim, dtype)
+    sink = _rand(nq, seed=6)
+    ctx.extras = {"graph": True}
+    out = torch.full((5, nq * dim), 5.0, dtype=dtype, device="cuda")
+    call = lambda: ops.attention_kv4(qkv, lane, ctx, out, nq, nkv, dim, window=window, sink=sink)  # noqa: E731
+    call()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        call()
+    for shift in (0, 3):
+        ctx.positions[:2] -= shift  # read at replay
+        out[:4] = 0
+        graph.replay()
+        at = type(ctx)(**{**vars(ctx), "kv_lens": [n - (shift if i < 2 else 0) for i, n in enumerate(ctx.kv_lens)], "extras": {}})
+        rows = torch.cat([torch.arange(n, device="cuda") + sum(ctx.kv_lens[:i]) for i, n in enumerate(at.kv_lens)])
+        want, tol8, tol32 = attend(qkv[:4, : nq * dim], k[rows], v[rows], at, nq, dim ** -0.5, window, sink)
+        tol = (tol32 if dtype == F32 else tol8) + want.abs() * 1.01 * half_step(dtype)
+        _near(out[:4], want, tol)
+        assert (out[4] == 5).all()
