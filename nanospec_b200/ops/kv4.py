@@ -232,6 +232,12 @@ def _kv4_plan(ctx, lane, group: int, nkv: int, head_dim: int, window: int, tenso
             row += n
         requests = list(zip(starts, ctx.q_lens, ctx.kv_lens))
         long = kv4_unfolded(list(zip(ctx.q_lens, ctx.kv_lens)), group, nkv, head_dim, window, sm_count(), tensor_core) if unfold else []
+        if long:
+            for name, t, least in (("kv_len", ctx.kv_len, len(requests)), ("qo_indptr", ctx.qo_indptr, len(requests) + 1)):
+                _i32(t, name)
+                if t.numel() < least:
+                    raise KernelError(f"attention_kv4: {name} holds {t.numel()} numbers for {len(requests)} requests")
+            _on_current_device(ctx.kv_len, ctx.qo_indptr)
         unfolded = set(long)
         rest = [(s, n, kv) for i, (s, n, kv) in enumerate(requests) if i not in unfolded]
         rest.sort(key=lambda r: -r[2])  # the longest first: blocks are scheduled in this order

@@ -226,3 +226,16 @@ def test_a_captured_steps_plan_with_a_window(monkeypatch):
     ctx.extras["graph"] = True
     wide, none = (kv4._kv4_plan(ctx, lane, 4, 8, 128, window, True, True)["runs"] for window in (131072, 0))
     assert wide == none and none[0][4] == (4, 74, 8)
+
+
+def test_the_lengths_of_portions_are_checked(monkeypatch):
+    """The device's lengths and first rows of requests, which the kernels of unfolded portions read: a number to each request, 32 bits, on the device."""
+    from nanospec_b200.ops import KernelError, kv4
+    monkeypatch.setattr(kv4, "sm_count", lambda: 148)
+    ctx, lane, _ = step([(2000, 300), (5, 1)], 16, 2, 64, nq=4, device="cpu")
+    for name, bad in (("kv_len", ctx.kv_len.long()), ("kv_len", ctx.kv_len[:1]), ("qo_indptr", ctx.qo_indptr.long()), ("qo_indptr", ctx.qo_indptr[:2])):
+        with pytest.raises(KernelError, match=name):
+            kv4._kv4_plan(SimpleNamespace(**{**vars(ctx), name: bad}), lane, 2, 2, 64, 0, True, True)
+    with pytest.raises(KernelError, match="CUDA"):
+        kv4._kv4_plan(ctx, lane, 2, 2, 64, 0, True, True)
+    assert not ctx.extras
