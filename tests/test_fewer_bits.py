@@ -232,6 +232,7 @@ def test_the_lengths_of_portions_are_checked(monkeypatch):
     """The device's lengths and first rows of requests, which the kernels of unfolded portions read: a number to each request, 32 bits, on the device."""
     from nanospec_b200.ops import KernelError, kv4
     monkeypatch.setattr(kv4, "sm_count", lambda: 148)
+    monkeypatch.setattr(kv4, "kv4_unfolded", lambda *a: [0])
     ctx, lane, _ = step([(2000, 300), (5, 1)], 16, 2, 64, nq=4, device="cpu")
     for name, bad in (("kv_len", ctx.kv_len.long()), ("kv_len", ctx.kv_len[:1]), ("qo_indptr", ctx.qo_indptr.long()), ("qo_indptr", ctx.qo_indptr[:2])):
         with pytest.raises(KernelError, match=name):
