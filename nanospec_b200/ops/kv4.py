@@ -333,18 +333,18 @@ class _Unfolded:
     page_size: int = KV4_UNFOLD_PAGE
 
 
-def _attend_unfolded(qkv, lane, ctx, out, nkv: int, group: int, head_dim: int, scale: float, window: int, sink, portion: dict) -> None:
+def _attend_unfolded(qkv, lane, ctx, out, nkv: int, group: int, head_dim: int, scale: float, window: int, sink, portion: dict, wide_weights: bool) -> None:
     head, heads, n = portion["head"], portion["heads"], portion["n"]
     k, v = torch.empty((2, n, heads, KV4_UNFOLD_PAGE, head_dim), dtype=torch.bfloat16, device=out.device).unbind(0)
     lib.call("ns_kv4_unfold", lane.k.data_ptr(), lane.v.data_ptr(), lane.block_table.data_ptr(), lane.block_table.stride(0), portion["items"].data_ptr(), n,
              ctx.kv_len.data_ptr(), k.data_ptr(), v.data_ptr(), lane.page_size, nkv, head, heads, head_dim, _stream())
     at, width = head * group * head_dim, heads * group * head_dim
     attention_prefill(qkv[:, at: at + width], _Unfolded(k, v, portion["table"]), ctx, out[:, at: at + width], heads * group, heads, head_dim, scale, window,
-                      portion["tiles"], portion["tiles_tc"], sink=None if sink is None else sink[head * group: (head + heads) * group])
+                      portion["tiles"], portion["tiles_tc"], wide_weights=wide_weights, sink=None if sink is None else sink[head * group: (head + heads) * group])
 
 
 def attention_kv4(qkv: torch.Tensor, lane, ctx, out: torch.Tensor, nq: int, nkv: int, head_dim: int, scale: float | None = None, window: int = 0,
-                  sink: torch.Tensor | None = None) -> torch.Tensor:
+                  sink: torch.Tensor | None = None, wide_weights: bool = False) -> torch.Tensor:
     """Attention of the step's queries (the first nq * head_dim columns of `qkv`, rotated) over a lane in 4 bits: every token sees the positions
     up to its own (with `window` the last so many of them), which `kv4_store` has filled.  `sink` (float32 [nq]): the softmax's denominator also
     holds exp(sink[h]).  `scale` is head_dim ** -0.5 when None.  float32 and bfloat16; rows of padding (token_req < 0) are left as they are.
@@ -356,7 +356,7 @@ def attention_kv4(qkv: torch.Tensor, lane, ctx, out: torch.Tensor, nq: int, nkv:
     bfloat16, softmax weights in bfloat16: single tokens and a few of a request on the tensor cores from the cache's bytes (csrc/attention_kv4_tc.cu: heads
     of 64, 128 or 256, pages of 8, 16 or a multiple of 32 tokens); longer portions of prompts unfold the keys and values that they see into bfloat16 once
     and take the attention over such a cache (heads up to 128, rows of q on 16-byte boundaries).  Everything else, float32 above all: float
-    throughout (csrc/attention_kv4.cu)."""
+    throughout (csrc/attention_kv4.cu).  `wide_weights`: bfloat16 in float too, portions with weights of about 16 bits, as `attention` has it."""
     _on_current_device(qkv, out, lane.k, lane.v, lane.block_table, ctx.positions, ctx.token_req, sink)
     _check_lane("attention_kv4", lane, nkv, head_dim)
     if qkv.dim() != 2 or out.dim() != 2:
@@ -373,7 +373,7 @@ def attention_kv4(qkv: torch.Tensor, lane, ctx, out: torch.Tensor, nq: int, nkv:
         raise KernelError("attention_kv4: the sink is one contiguous float32 number per query head")
     scale = 1.0 / math.sqrt(head_dim) if scale is None else float(scale)
     group, sms, window = nq // nkv, sm_count(), min(int(window), 1 << 30)
-    tensor_core = kv4_tensor_core_ok(qkv.dtype, head_dim, lane.page_size)
+    tensor_core = not wide_weights and kv4_tensor_core_ok(qkv.dtype, head_dim, lane.page_size)
     unfold = code == BF16 and head_dim <= 128 and ldq % 8 == 0 and ldo % 2 == 0 and qkv.data_ptr() % 16 == 0 and out.data_ptr() % 4 == 0
     plan, stream = _kv4_plan(ctx, lane, group, nkv, head_dim, window, tensor_core, unfold), _stream()
     _check_table(lane, plan["held"], plan["requests"])
@@ -394,5 +394,5 @@ def attention_kv4(qkv: torch.Tensor, lane, ctx, out: torch.Tensor, nq: int, nkv:
                  ctx.token_req.data_ptr(), ctx.positions.data_ptr(), _ptr(rows), _ptr(items), count, out.data_ptr(), ldo, nq, nkv, head_dim, lane.page_size,
                  scale, window, _ptr(sink), n_blocks, warps, splits, _ptr(part), _ptr(jobs), n_jobs, least, stream)
     for portion in plan["portions"]:
-        _attend_unfolded(qkv, lane, ctx, out, nkv, group, head_dim, scale, window, sink, portion)
+        _attend_unfolded(qkv, lane, ctx, out, nkv, group, head_dim, scale, window, sink, portion, wide_weights)
     return out

@@ -928,3 +928,22 @@ def test_captured_steps_with_windows_and_sinks(window, dim, dtype):
         tol = (tol32 if dtype == F32 else tol8) + want.abs() * 1.01 * half_step(dtype)
         _near(out[:4], want, tol)
         assert (out[4] == 5).all()
+
+
+@pytest.mark.parametrize("lens", [[(300, 1), (2000, 1), (0, 1)], [(200, 3), (31, 6)], [(500, 1), (0, 200), (90, 3), (1200, 300)]])
+@pytest.mark.parametrize("nq,nkv,dim,page,dtype", [(32, 8, 128, 16, BF16), (8, 2, 64, 8, BF16), (4, 1, 256, 16, BF16), (6, 2, 96, 16, BF16), (4, 2, 64, 16, F32)])
+@pytest.mark.parametrize("window", [0, 150])
+def test_weights_in_more_than_eight_bits(lens, nq, nkv, dim, page, dtype, window):
+    """In float, or, in portions, as two bfloat16: the first is off by 2^-8 of the weight, which the second holds but for 2^-8 of itself."""
+    from nanospec_b200 import ops
+    ctx, lane, qkv = step(lens, page, nkv, dim, dtype, nq, padding=1)
+    lane.k.fill_(255), lane.v.fill_(255)
+    k, v = fill(ctx, lane, nq, nkv, dim, dtype)
+    n, sink = ctx.n_tokens - 1, _rand(nq, seed=8)
+    want, tol8, tol32 = attend(qkv[:n, : nq * dim], k, v, ctx, nq, dim ** -0.5, window, sink)
+    rounding = want.abs() * 1.01 * half_step(dtype)
+    for wide in (True, False, True):  # (the two forms of a step do not meet in its plan)
+        out = torch.full((ctx.n_tokens, nq * dim), 5.0, dtype=dtype, device="cuda")
+        ops.attention_kv4(qkv, lane, ctx, out, nq, nkv, dim, window=window, sink=sink, wide_weights=wide)
+        _near(out[:n], want, (tol32 + (tol8 - tol32) * (2.0 ** -8 if wide else 1.0)) + rounding)
+        assert (out[n:] == 5).all()
