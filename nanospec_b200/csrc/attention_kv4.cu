@@ -5,8 +5,10 @@
 // turn, each with a running maximum and sum of its own, and are joined at the end in a fixed order.  Scores: a lane holds a key; weighted values: a lane holds
 // features, and asks for the codes of eight keys before it uses the first (one at a time, the latency of each bounds the kernel: 2,236 keys of 16 heads of 32 168 us).
 //
-// Bound by its float arithmetic, two fused multiply-adds a feature, key and head, and by the reads of shared memory that feed them.  64 requests on up to 2,000 keys,
-// four heads to each of 8 kv heads of 128: 162 us, 256 where every block computed for eight heads; four portions of up to 64 tokens on up to 500: 145, 273.
+// 64 requests on up to 2,000 keys, four heads to each of 8 kv heads of 128: 162 us, 256 where every block computed for eight heads; four portions of up to 64 tokens on
+// up to 500: 145, 273.  No pipe is near its limit there: its fused multiply-adds, two a feature, key and head, would take some 18 us.  While an SM has work, which is 71 %
+// of the time on these ragged lengths, its schedulers issue in 57 % of the cycles (logic pipe 37 % busy, multiply-adds 27 %); the registers leave them four warps each,
+// which wait for the codes (long scoreboard 1.3 an instruction), for one another's results (wait 1.2) and for q in shared memory (short scoreboard 0.8).
 #include "kv4.cuh"
 #include "tcgen05_utils.cuh"
 

@@ -18,10 +18,12 @@
 //
 // The weights meet the values as bfloat16, as in the attention over a bfloat16 cache; sums, maximum and outputs are float.
 //
-// Bound by the SMs' integer pipe, not by memory: 384 of a tile's about 690 instructions a warp (heads of 128) make values of codes, more than half of those in the logic
+// Where all SMs have as much to do, bound by their integer pipe, not by memory: 384 of a tile's about 690 instructions a warp (heads of 128) make values of codes, more than half of those in the logic
 // pipe, which issues every second cycle and is busy for 60 % of 1,160 cycles a tile and scheduler; the rest is four warps a scheduler that wait for it or for
 // one another's turn.  74 requests on 4,096 keys of 8 kv heads: 86 us (pages of 64 tokens; 94 of 16), 4.5 TB/s, the same where all requests read the same
-// page.  The ragged 64 on up to 2,300 keys, 111 MB: 43 us; 2 on 100,000, 170 MB: 53 us.
+// page.  On ragged lengths nothing is near a limit: 64 on up to 2,300 keys, 111 MB, 49 us (SMs 38 % busy, memory 30 %: the blocks of the longest requests outlast the
+// others); two, on 100,001 and 33,428, 171 MB, 49 us with the join (49 and 47 %); 18 tiles of a few tokens on up to 3,000, 43 MB, 31 us (34 and 19 %: a block's five tiles a
+// warp stand between a chain of dependent loads and the merging of its warps).
 #include "kv4.cuh"
 #include "mma_utils.cuh"
 #include "tcgen05_utils.cuh"

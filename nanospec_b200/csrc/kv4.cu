@@ -2,10 +2,11 @@
 //
 // What the cache holds is the definition's to the last bit: k rotated exactly and rounded once to the activations' type, S and B rounded once, codes decided by
 // exact remainders.  One rounding that fell on the other side of a border would move a feature by a whole code, or a group by its S.  Computed in double
-// throughout, a prompt is bound by its instructions (3,739 tokens of 32 + 2 x 8 heads of 128, 96 MB: 53 us); so everything is first done in float, with a bound of
-// its error, and again in double where a border between two roundings lies within the bound - one element in some thousands.  The same tokens now take 37.9
-// us, of which 14.7 are their bytes at the rate of a copy: instructions still bound it, the schedulers issue in two cycles of three.  float32 activations, which
-// have no bits to spare in float, are rotated in double.  q, which is rounded to the activations' type and not quantised, is rotated in float.
+// throughout, a prompt is bound by its instructions (3,739 tokens of 32 + 2 x 8 heads of 128, 81 MB: 53 us, as all times here of a launch alone, 6 of which an empty
+// one takes too); so everything is first done in float, with a bound of its error, and again in double where a border between two roundings lies within the
+// bound - one element in some thousands.  The same tokens now take 38.9 us, of which 12.4 are their bytes at the rate of a copy: instructions still bound it, the
+// schedulers issue in two cycles of three.  float32 activations, which have no bits to spare in float, are rotated in double (71.7 us, 158 MB, 24.1 at the rate of
+// a copy).  q, which is rounded to the activations' type and not quantised, is rotated in float in both.
 #include "kv4.cuh"
 
 namespace {
@@ -181,7 +182,7 @@ template <> struct Angle<float> { using type = double; };
 
 // One block (or `gridDim.y` blocks, which share its heads) per token.  For keys and values a lane holds four neighbouring features of every 128, eight lanes a group.
 // kD: the size of a head, where it is a usual one (3,739 tokens of 32 + 2 x 8 heads of 128: 44.0 us without, 39.9), or 0.  bfloat16 in 48 registers, which spills a
-// little, holds five blocks an SM rather than four (37.9).
+// little, holds five blocks an SM rather than four (37.9 to 38.9).
 template <typename T, int kChunks, int kD>
 __global__ void __launch_bounds__(kThreads, sizeof(T) == 2 && kChunks == 1 ? 5 : 1)
 kv4_store_kernel(const T* __restrict__ qkv, long long ld, T* __restrict__ q_out, long long ldq, const int* __restrict__ positions,

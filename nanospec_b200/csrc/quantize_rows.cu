@@ -6,8 +6,10 @@
 // The maximum is taken over the bit patterns of |x|, in whose order infinities and NaN come last.
 //
 // A row is read once (its pieces stay in registers where the block holds them) and written once in a byte per element; one block a row, since a row's maximum
-// stands before its first quotient.  4,096 x 4,096 bfloat16 take 16.2 us (7.7 at the rate of a copy).  Instructions bound it more than memory does: with a test of
-// each element's remainder in place of each piece's, on numbers unpacked for the maximum too, the same rows took 32.
+// stands before its first quotient.  4,096 x 4,096 bfloat16 take 16.4 us (7.7 at the rate of a copy), float32 18.5 (12.8), from rows off 16-byte boundaries, which
+// are read an element at a time, 20.5 both.  Neither instructions nor memory are at their limit (SMs 54 % busy, memory 27 %; 512 x 14,336: 24 and 13 %): a block first
+// waits for its row, then for its maximum, then computes, and the few blocks of an SM overlap these in part.  Instructions count all the same: with a test
+// of each element's remainder in place of each piece's, on numbers unpacked for the maximum too, the same rows took 32.
 #include "common.cuh"
 
 namespace {

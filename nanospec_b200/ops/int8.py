@@ -16,7 +16,7 @@ I8_MAX_K = 131072  # 127 * 127 * K stays within 32 bits
 
 @dataclass
 class RowsI8:
-    """A matrix in 8-bit integers from -127 to 127: `q` [R, K] int8 (rows on 16-byte boundaries) and `scale` [R] float32; row r stands for q[r] * scale[r]."""
+    """A matrix in 8-bit integers from -127 to 127 (not -128, with which the sum over the largest K could leave 32 bits): `q` [R, K] int8 (rows on 16-byte boundaries) and `scale` [R] float32; row r stands for q[r] * scale[r]."""
 
     q: torch.Tensor
     scale: torch.Tensor
